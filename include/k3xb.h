@@ -49,6 +49,9 @@ enum { K3XB_ACT_SWIGLU = 0, K3XB_ACT_SITU = 1 };
  * accumulators); SIMT = CUDA-core FP4 decode + FP32 FMA (cross-check). */
 enum { K3XB_ENGINE_MXF4 = 0, K3XB_ENGINE_SIMT = 1 };
 
+/* Element types of the calls that take more than one (void* arrays). */
+enum { K3XB_TYPE_F32 = 0, K3XB_TYPE_BF16 = 1, K3XB_TYPE_F16 = 2 };
+
 typedef struct k3xb_ctx k3xb_ctx;
 
 /* ---- context ------------------------------------------------------------ */
@@ -115,6 +118,7 @@ enum {
     K3XB_PHASE_ACCEPT,             /* greedy / rejection acceptance */
     K3XB_PHASE_COMMIT,             /* state commit of the accepted path */
     K3XB_PHASE_LATENT,             /* LatentMoE projections and routed norm */
+    K3XB_PHASE_ATTENTION,          /* attention over a shared prefix and own rows */
     K3XB_PHASE_COUNT
 };
 typedef struct {
@@ -525,6 +529,89 @@ int k3xb_kda_commit(k3xb_ctx* ctx, const float* state, const int32_t* parent,
                     uint32_t head_dim, const float* q, const float* k,
                     const float* v, const float* log_decay, const float* beta,
                     const int32_t* commit_node, float* state_out);
+
+/* The gated delta rule of k3xb_kda_tree (official_kda.cpp:319-369) over the
+ * tokens of whole prompts: S ragged sequences packed one after the other,
+ * sequence s holding tokens offsets[s] .. offsets[s+1]-1 (offsets: DEVICE
+ * array [S+1], non-decreasing, at most `tokens`; a sequence may be empty).
+ * q, k, v: rows of h*d values of `type` (f32 or bf16), row_stride elements
+ * apart (0: packed), so that they may be column slices of one projection.
+ * log_decay [tokens][h*d] and beta [tokens][h] float. The state before
+ * (state [S][h][d][d], V-first, NULL: zeros) and after (state_out, NULL: not
+ * kept; may be `state`) are float; an empty sequence's state is copied.
+ * out [tokens][h*d] of `type`, each value rounded once. head_dim 32, 64 or
+ * 128; states 16-byte aligned. All sums are float-precision sums in an order of their own:
+ * results agree with the token-by-token calls to float tolerance, not bit
+ * for bit (k3xb_kda_tree keeps the reference's order). Offsets that are no
+ * ranges leave their sequences out and k3xb_sync reports INVALID_EXTENT. */
+int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
+                     uint64_t row_stride, int32_t type, const float* log_decay,
+                     const float* beta, const uint32_t* offsets, uint32_t sequences,
+                     uint32_t tokens, uint32_t heads, uint32_t head_dim,
+                     const float* state, float* state_out, void* out);
+/* The same rule for one token of each sequence, the state advanced IN PLACE
+ * (the plain decode step of official_kda, backend.hpp:402-408). Row s of q, k,
+ * v, log_decay, beta and out is sequence s, whose state is state[slots[s]]
+ * of `states` states (slots: DEVICE array [S], NULL: state[s]). A negative
+ * slot is an idle sequence: no state changes and its out row is zero. Two
+ * sequences with one slot race. Slots past the pool are left out like idle
+ * ones and k3xb_sync reports INVALID_EXTENT. */
+int k3xb_kda_step(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
+                  uint64_t row_stride, int32_t type, const float* log_decay,
+                  const float* beta, uint32_t sequences, uint32_t heads,
+                  uint32_t head_dim, const int32_t* slots, uint32_t states,
+                  float* state, void* out);
+
+/* ---- attention over a shared prefix ---------------------------------------- */
+/* Key and value rows of a cache. Position p of sequence s has, for each of
+ * kv_heads heads, a key k[s*k_seq + p*k_row + head*k_head ..+main_dim] and a
+ * value v[..+value_dim], and one extra[s*extra_seq + p*extra_row ..+extra_dim]
+ * that the heads share (the q_extra part of the gated MLA layer, model.cpp:
+ * 755-811). Strides in elements; 0: packed [seq][rows][kv_heads][dim]. Any
+ * order of rows and heads is allowed. */
+typedef struct {
+    const void *k, *v, *extra;     /* extra: NULL when extra_dim is 0 */
+    uint64_t k_row, k_head, k_seq, v_row, v_head, v_seq, extra_row, extra_seq;
+    uint32_t rows;                 /* the prefix's length / a sequence's capacity */
+} k3xb_kv_rows;
+
+/* The attention of Engine::mla (model.cpp:785-810, without its gate and
+ * output projection) for S sequences that begin with one shared prefix and
+ * each check N draft nodes of a common topology (parent: HOST array as for
+ * k3xb_kda_tree, at most 64 nodes; one decoded token: N = 1). Node n of
+ * sequence s sees every prefix row, the suffix rows below suffix_len[s], and
+ * of the suffix rows suffix_len[s] + m, m < N (the drafts' own rows, which
+ * the caller has stored there), those on its path to the root, itself
+ * included. A negative suffix_len is an idle sequence: zero rows, lse -inf.
+ * Nothing else of the suffix is read into a result, whatever it holds.
+ *   out[s][n][head] = softmax(scale * q . [k, extra]) v
+ *   lse[s][n][head] = log of the sum of the exponentials (may be NULL)
+ * q rows [S][N] of heads * (main_dim + extra_dim) values, q_row elements
+ * apart (0: packed); out [S][N][heads][value_dim]. type (f32, bf16, f16) is
+ * that of q, the caches and out; scores, the softmax and all sums are float.
+ * heads is a multiple of kv_heads (head h reads kv head h / (heads /
+ * kv_heads)); main_dim + extra_dim and value_dim at most 256. bf16 and f16
+ * calls with main_dim and value_dim 64 or 128, extra_dim 0 or 64, and rows that start at
+ * 16-byte boundaries run on the tensor cores, where the prefix is read once
+ * for all sequences and the probabilities enter the second product rounded
+ * to `type`; other shapes take a slower general form. A suffix_len that
+ * leaves no room for the drafts counts as idle and k3xb_sync reports
+ * INVALID_EXTENT. */
+typedef struct {
+    uint32_t sequences, nodes, heads, kv_heads;
+    uint32_t main_dim, extra_dim, value_dim;
+    int32_t type;                  /* K3XB_TYPE_* */
+    float scale;
+    const int32_t* parent;         /* HOST [nodes] */
+    const void* q;
+    uint64_t q_row;
+    k3xb_kv_rows prefix;           /* *_seq unused; rows 0: no prefix */
+    k3xb_kv_rows suffix;
+    const int32_t* suffix_len;     /* [S] */
+    void* out;
+    float* lse;                    /* [S][N][heads], or NULL */
+} k3xb_prefix_attention_io;
+int k3xb_prefix_attention(k3xb_ctx* ctx, const k3xb_prefix_attention_io* io);
 
 /* ---- full KDA block and the KDA + MoE layer -------------------------------- */
 /* Weights of one official KDA block (official_kda.hpp / official_kda.cpp:

@@ -24,6 +24,8 @@ ACT_SITU = 1
 ENGINE_MXF4 = 0
 ENGINE_SIMT = 1
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2   # K3XB_TYPE_*
+
 STATUS_NAMES = {0: "OK", 9: "INVALID_EXTENT", 15: "INVALID_MXFP4", 16: "INVALID_STATE",
                 17: "BACKEND_UNAVAILABLE", 19: "UNSUPPORTED_ARCHITECTURE"}
 
@@ -96,6 +98,19 @@ class SpeculativeIO(C.Structure):
                                   "committed_count", "logits")]
 
 
+class KvRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "extra")] + [
+        (n, C.c_uint64) for n in ("k_row", "k_head", "k_seq", "v_row", "v_head", "v_seq", "extra_row", "extra_seq")] + [
+        ("rows", C.c_uint32)]
+
+
+class PrefixAttentionIO(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("sequences", "nodes", "heads", "kv_heads", "main_dim", "extra_dim",
+                                          "value_dim")] + [
+        ("type", C.c_int32), ("scale", C.c_float), ("parent", C.c_void_p), ("q", C.c_void_p), ("q_row", C.c_uint64),
+        ("prefix", KvRows), ("suffix", KvRows), ("suffix_len", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p)]
+
+
 KDA_SEED, KDA_CONTINUE, KDA_PUBLISH = 0, 1, 2   # k3xb_kda_block_held modes
 KDA_HELD_SLOTS = 8
 
@@ -122,7 +137,7 @@ class Stats(C.Structure):
         "peak_resident_weight_bytes", "weight_h2d_bytes")]
 
 
-PHASE_COUNT = 20   # K3XB_PHASE_COUNT
+PHASE_COUNT = 21   # K3XB_PHASE_COUNT
 
 
 class PhaseTime(C.Structure):
@@ -177,6 +192,9 @@ def library() -> C.CDLL:
             "k3xb_moe_experts": [vp, C.POINTER(MoeLayer), vp, u32, C.POINTER(Plan), vp],
             "k3xb_kda_tree": [vp, vp, vp, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp],
             "k3xb_kda_commit": [vp, vp, vp, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp, vp],
+            "k3xb_kda_prefill": [vp, vp, vp, vp, u64, C.c_int32, vp, vp, vp, u32, u32, u32, u32, vp, vp, vp],
+            "k3xb_kda_step": [vp, vp, vp, vp, u64, C.c_int32, vp, vp, u32, u32, u32, vp, u32, vp, vp],
+            "k3xb_prefix_attention": [vp, C.POINTER(PrefixAttentionIO)],
             "k3xb_accept_greedy": [vp, vp, vp, u32, u32, u32, vp, vp, vp, vp],
             "k3xb_accept_rejection": [vp, vp, vp, vp, u32, u32, u32, f32, u64, u64, vp, vp, vp],
             "k3xb_fill_normal_f32": [vp, vp, sz, u64, u64, f32, f32],
@@ -244,6 +262,30 @@ def _p(t):
     if not t.is_contiguous():
         raise K3xbError(INVALID_EXTENT, "expected a contiguous tensor")
     return C.c_void_p(t.data_ptr())
+
+
+def _a(t, dtype, shape, name):
+    """Address of a contiguous CUDA tensor of this type and shape (None ->
+    NULL)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda:
+        raise K3xbError(INVALID_EXTENT, f"{name}: expected a contiguous CUDA tensor {dtype} {shape}, got {t.dtype} "
+                                        f"{tuple(t.shape)}")
+    return t.data_ptr()
+
+
+_TYPES = {}
+
+
+def _type(t, name):
+    """K3XB_TYPE_* of a CUDA tensor."""
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16})
+    if t.dtype not in _TYPES or not t.is_cuda:
+        raise K3xbError(INVALID_EXTENT, f"{name}: expected a CUDA tensor of float32, bfloat16 or float16")
+    return _TYPES[t.dtype]
 
 
 class Context:
@@ -340,6 +382,93 @@ class Context:
         com = (C.c_int32 * S)(*[int(x) for x in commit_node])
         self._check(self.lib.k3xb_kda_commit(self.h, _p(state), par, N, S, heads, d, _p(q), _p(k), _p(v),
                                              _p(log_decay), _p(beta), com, _p(state_out)), "kda_commit")
+
+    def _kda_rows(self, q, k, v, log_decay, beta, out):
+        """Checks shared by kda_prefill and kda_step; returns (tokens, heads,
+        head_dim, row_stride, type)."""
+        import torch
+        if q.dim() != 2 or beta.dim() != 2 or not beta.shape[1] or q.shape[1] % beta.shape[1]:
+            raise K3xbError(INVALID_EXTENT, "q must be [tokens][heads * head_dim] and beta [tokens][heads]")
+        (T, P), h = q.shape, beta.shape[1]
+        kind, stride = _type(q, "q"), q.stride(0) if T > 1 else P
+        for t in (q, k, v):
+            if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device or t.stride(1) != 1 or (
+                    T > 1 and t.stride(0) != stride):
+                raise K3xbError(INVALID_EXTENT, "q, k and v must be rows of one shape, type and row stride")
+        f32 = torch.float32
+        return T, h, P // h, stride, kind, _a(log_decay, f32, (T, P), "log_decay"), _a(beta, f32, (T, h), "beta"), _a(
+            out, q.dtype, (T, P), "out")
+
+    def kda_prefill(self, q, k, v, log_decay, beta, offsets, out, state=None, state_out=None):
+        """The gated delta rule over packed prompts: q/k/v [tokens][h*d] (rows
+        may be strided alike), log_decay [tokens][h*d], beta [tokens][h],
+        offsets [S+1] int32 on the device, out [tokens][h*d]; state and
+        state_out [S][h][d][d] (None: zeros / not kept; may be one tensor)."""
+        import torch
+        T, h, d, stride, kind, ld, be, o = self._kda_rows(q, k, v, log_decay, beta, out)
+        S = offsets.shape[0] - 1
+        self._check(self.lib.k3xb_kda_prefill(
+            self.h, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride, kind, ld, be,
+            _a(offsets, torch.int32, (S + 1,), "offsets"), S, T, h, d,
+            _a(state, torch.float32, (S, h, d, d), "state"), _a(state_out, torch.float32, (S, h, d, d), "state_out"), o),
+            "kda_prefill")
+
+    def kda_step(self, q, k, v, log_decay, beta, state, out, slots=None):
+        """One token of each sequence, its state advanced in place: q/k/v
+        [S][h*d], state [states][h][d][d]; slots [S] int32 (None: state s;
+        negative: idle)."""
+        import torch
+        S, h, d, stride, kind, ld, be, o = self._kda_rows(q, k, v, log_decay, beta, out)
+        states = state.shape[0]
+        self._check(self.lib.k3xb_kda_step(
+            self.h, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride, kind, ld, be, S, h, d,
+            _a(slots, torch.int32, (S,), "slots"), states, _a(state, torch.float32, (states, h, d, d), "state"), o),
+            "kda_step")
+
+    @staticmethod
+    def _kv_rows(k, v, extra, sequences, kv_heads, main, value, extra_dim, dtype):
+        """KvRows of [rows][kv_heads][dim] tensors (sequences None) or of
+        [S][rows][kv_heads][dim] ones; any strides with a contiguous last
+        dimension."""
+        if k is None or not k.numel():
+            return KvRows()
+        lead = () if sequences is None else (sequences,)
+        rows = k.shape[len(lead)]
+        for t, want, name in ((k, (*lead, rows, kv_heads, main), "k"), (v, (*lead, rows, kv_heads, value), "v"),
+                              (extra, (*lead, rows, extra_dim), "extra")):
+            if t is None and not extra_dim and name == "extra":
+                continue
+            if t is None or tuple(t.shape) != want or t.dtype != dtype or not t.is_cuda or t.stride(-1) != 1:
+                raise K3xbError(INVALID_EXTENT, f"cache {name}: expected {want} of {dtype} on the GPU with a contiguous "
+                                                "last dimension")
+        ks, vs, es = k.stride(), v.stride(), (0,) * (len(lead) + 2) if extra is None else extra.stride()
+        return KvRows(k.data_ptr(), v.data_ptr(), None if extra is None else extra.data_ptr(), ks[-3], ks[-2],
+                      ks[0] if lead else 0, vs[-3], vs[-2], vs[0] if lead else 0, es[-2], es[0] if lead else 0, rows)
+
+    def prefix_attention(self, q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_len, parent, out, prefix_extra=None,
+                         suffix_extra=None, lse=None, scale=None):
+        """Attention of draft nodes over a shared prefix, own rows and
+        ancestors: q [S][N][heads][main + extra]; prefix_k/_v/_extra
+        [rows][kv_heads][dim] / [rows][extra] (None or empty: no prefix);
+        suffix_k/_v/_extra [S][capacity][kv_heads][dim] / [S][capacity][extra];
+        suffix_len [S] int32 on the device; parent [N] on the host; out
+        [S][N][heads][value]; lse [S][N][heads] or None; scale default
+        1 / sqrt(main + extra)."""
+        import torch
+        S, N, heads, width = q.shape
+        kv_heads, main, value = suffix_k.shape[2], suffix_k.shape[3], suffix_v.shape[3]
+        extra = width - main
+        if not q.is_contiguous() or extra < 0 or len(parent) != N:
+            raise K3xbError(INVALID_EXTENT, "q must be contiguous, as wide as a key, with one parent per node")
+        par = (C.c_int32 * N)(*parent)
+        io = PrefixAttentionIO(
+            S, N, heads, kv_heads, main, extra, value, _type(q, "q"), width ** -0.5 if scale is None else scale,
+            C.addressof(par), q.data_ptr(), 0,
+            self._kv_rows(prefix_k, prefix_v, prefix_extra, None, kv_heads, main, value, extra, q.dtype),
+            self._kv_rows(suffix_k, suffix_v, suffix_extra, S, kv_heads, main, value, extra, q.dtype),
+            _a(suffix_len, torch.int32, (S,), "suffix_len"), _a(out, q.dtype, (S, N, heads, value), "out"),
+            _a(lse, torch.float32, (S, N, heads), "lse"))
+        self._check(self.lib.k3xb_prefix_attention(self.h, C.byref(io)), "prefix_attention")
 
     def select_routing(self, scores, bias, natural_k, ids, weights, selected, escalated=None, stats=None,
                        mode=ROUTING_NATURAL, fixed_k=0, mass_target=0.9, minimum_gap=0.0, quality_floor_k=0):
