@@ -758,6 +758,21 @@ int make_byte_map(k3xb_ctx* ctx, void* map, const void* base, uint64_t row_bytes
     return make_map(ctx, static_cast<CUtensorMap*>(map), base, row_bytes, rows, box_rows);
 }
 
+int make_row_map(k3xb_ctx* ctx, void* map, const void* base, uint64_t dim_bytes, uint64_t heads, uint64_t rows,
+                 uint64_t head_bytes, uint64_t row_bytes, uint32_t box_rows) {
+    EncodeFn encode;
+    if (const int st = get_encode(ctx, &encode)) return st;
+    const cuuint64_t dims[3] = {dim_bytes, heads, rows};
+    const cuuint64_t strides[2] = {head_bytes, row_bytes};
+    const cuuint32_t box[3] = {128, 1, box_rows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = encode(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base),
+                              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ctx, K3XB_BACKEND_UNAVAILABLE, "cuTensorMapEncodeTiled failed");
+    return K3XB_OK;
+}
+
 int prepare_mxfp4_scales(k3xb_ctx* ctx, const uint8_t* scales, size_t rows, size_t cols, uint8_t* out) {
     if (!scales || !out || !rows || rows % 128 || !cols || cols % 128)
         return fail(ctx, K3XB_INVALID_MXFP4, "prepare scales: rows and cols must be multiples of 128");

@@ -93,6 +93,11 @@ void release_mxf4_resources(k3xb_ctx* ctx);
 int prepare_mxfp4_scales(k3xb_ctx* ctx, const uint8_t* scales, size_t rows, size_t cols, uint8_t* out);
 // 2-D byte tensor map (128B swizzle, box {128 B, box_rows}); map is a CUtensorMap*
 int make_byte_map(k3xb_ctx* ctx, void* map, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_rows);
+// 3-D byte tensor map [rows][heads][dim_bytes] (128B swizzle, box {128 B, one
+// head, box_rows}); base and strides multiples of 16 bytes, rows past the end
+// read as zeros.
+int make_row_map(k3xb_ctx* ctx, void* map, const void* base, uint64_t dim_bytes, uint64_t heads, uint64_t rows,
+                 uint64_t head_bytes, uint64_t row_bytes, uint32_t box_rows);
 // linear_tc.cu — out[T][rows] = (round_bf16)(W . x), x split into two bf16 terms
 size_t linear_scratch_bytes(uint32_t T, uint32_t K);
 int launch_linear_bf16(k3xb_ctx* ctx, const float* x, const uint16_t* W, uint32_t T, uint32_t rows, uint32_t K,

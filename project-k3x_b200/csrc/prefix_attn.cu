@@ -16,33 +16,14 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "prefix_attn.cuh"
 #include "profile.cuh"
 
 namespace k3xb {
 
 namespace {
 
-constexpr uint32_t kMaxNodes = 64, kMaxDim = 256;
-
-// One source of key and value rows; strides in elements.
-struct KvSource {
-    const void *k, *v, *extra;
-    uint64_t k_row, k_head, k_seq, v_row, v_head, v_seq, extra_row, extra_seq;
-};
-
-struct AttnArgs {
-    uint32_t S, N, heads, kv_heads, main, extra, value;
-    float scale;
-    uint64_t q_row;
-    uint32_t prefix_len, capacity;
-    KvSource prefix, suffix;
-    const int32_t* suffix_len;
-    const void* q;
-    void* out;
-    float* lse;
-    int32_t* status;
-    uint64_t ancestors[kMaxNodes];   // bit m: node m is n or on n's path to its root
-};
+constexpr uint32_t kMaxDim = 256;
 
 template <typename E>
 __device__ __forceinline__ float to_f(E x) {
@@ -56,16 +37,6 @@ __device__ __forceinline__ E from_f(float x) {
     if constexpr (std::is_same_v<E, float>) return x;
     else if constexpr (std::is_same_v<E, __half>) return __float2half_rn(x);
     else return __float2bfloat16_rn(x);
-}
-
-// A sequence's committed rows: -1 where it is idle. A length that the cache
-// cannot hold together with the draft rows is an error and counts as idle.
-__device__ __forceinline__ int32_t own_rows(const AttnArgs& a, uint32_t s) {
-    const int32_t len = a.suffix_len[s];
-    if (len < 0) return -1;
-    if (static_cast<uint64_t>(len) + a.N <= a.capacity) return len;
-    if (threadIdx.x == 0) atomicExch(a.status, K3XB_INVALID_EXTENT);
-    return -1;
 }
 
 // The general form: one CTA per (sequence, node, head), its four warps take
@@ -209,6 +180,7 @@ extern "C" int k3xb_prefix_attention(k3xb_ctx* ctx, const k3xb_prefix_attention_
         a.ancestors[n] = (p >= 0 ? a.ancestors[p] : 0) | (1ull << n);
     }
     PhaseScope ph(ctx, K3XB_PHASE_ATTENTION);
+    if (attend_tc_takes(a, io->type)) return launch_attend_tc(ctx, a, io->type == K3XB_TYPE_BF16);
     switch (io->type) {
         case K3XB_TYPE_F32: return launch_rows<float>(ctx, a);
         case K3XB_TYPE_BF16: return launch_rows<__nv_bfloat16>(ctx, a);

@@ -1,0 +1,867 @@
+// prefix_attn_tc.cu — the tensor-core form of the shared-prefix attention
+// (bf16 and f16, key parts of 64 or 128 and values of 64 or 128).
+//
+// The rows of one kv head are r = (sequence * N + node) * group + g, R in
+// all. Three kernels:
+//
+// 1. prefix_kernel: all R rows against the prefix, 128 rows a tile on
+//    tcgen05, so that a prefix row crosses HBM once for up to 256 rows. The
+//    work is one flat list of 128-key steps over (kv head, row tiles), cut
+//    into equal ranges, one per CTA; a range that ends inside a row tile
+//    leaves a part: the running maximum m, sum l and unnormalised output o
+//    of its keys.
+// 2. own_kernel: a sequence's own rows and its draft rows for 16 rows at a
+//    time on mma.sync (a sequence has few rows; the bound is the read of its
+//    cache). It runs beside the tail of 1 and then joins the parts:
+//       M = max m_i,  out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
+// 3. join_kernel, only where 2 split a long cache into several CTAs.
+//
+// Scores stay float; m is kept in log2 units (score * scale * log2 e).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "kernels.cuh"
+#include "prefix_attn.cuh"
+#include "tc.cuh"
+
+namespace k3xb {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two floats rounded to the 16-bit type, `lo` in the low half.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// ---- the split of the prefix ---------------------------------------------------
+
+constexpr uint32_t kTile = 128;          // rows and keys of a tile
+constexpr uint32_t kAtom = kTile * 128;  // bytes of 128 rows x 64 values
+constexpr uint32_t kMaxSlots = 12;       // ring slots of one atom
+
+// Row tiles are taken in pairs that share a step's keys; a last odd tile
+// takes two key blocks a step instead, one per half of the CTA.
+struct PrefixPlan {
+    uint32_t rows, group;
+    uint32_t blocks;           // 128-key blocks of the prefix
+    uint32_t pairs, odd;       // row tile pairs; 1: a last single tile
+    uint32_t steps_per_head;
+    uint32_t ctas, max_seg;    // parts a CTA may leave
+    uint64_t total;            // steps in all; 0: no prefix
+};
+
+__host__ __device__ __forceinline__ uint64_t first_step(const PrefixPlan& p, uint32_t cta) { return cta * p.total / p.ctas; }
+
+// A (kv head, row tile pair) and where its steps lie in the flat list.
+struct Job {
+    uint32_t head, pair, index;
+    uint64_t begin;
+    uint32_t steps;
+};
+__device__ __forceinline__ Job job_of(const PrefixPlan& p, uint64_t step) {
+    Job j;
+    j.head = static_cast<uint32_t>(step / p.steps_per_head);
+    const uint32_t off = static_cast<uint32_t>(step % p.steps_per_head);
+    j.pair = min(off / p.blocks, p.pairs);
+    j.index = j.head * (p.pairs + p.odd) + j.pair;
+    j.begin = static_cast<uint64_t>(j.head) * p.steps_per_head + static_cast<uint64_t>(j.pair) * p.blocks;
+    j.steps = j.pair < p.pairs ? p.blocks : (p.blocks + 1) / 2;
+    return j;
+}
+
+struct Parts {
+    float* o;     // [cta][seg][half][128][value]
+    float2* ml;   // [cta][seg][half][128]: m, l
+};
+
+struct PrefixBars {
+    uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], q_ready[2], o_done[2], teardown;
+    uint32_t tmem_base;
+    int abort;
+};
+
+__host__ __device__ constexpr uint32_t ring_slots(uint32_t key_atoms) { return key_atoms == 3 ? 8 : key_atoms == 2 ? 10 : 12; }
+constexpr size_t prefix_smem(uint32_t key_atoms) {
+    return (2 * key_atoms + ring_slots(key_atoms)) * size_t(kAtom) + sizeof(PrefixBars) + 1024;
+}
+
+// One segment of a CTA's range: steps [first, first + n) of a job. In key
+// mode half t of the CTA takes block 2 * step + t, else both take block
+// `step`; active(t) counts the steps in which the half has a block.
+struct Segment {
+    Job job;
+    uint32_t first, n;
+    bool keys;
+    __device__ __forceinline__ uint32_t active(uint32_t t, uint32_t blocks) const {
+        if (!keys || t == 0) return n;
+        return 2 * (first + n - 1) + 1 < blocks ? n : n - 1;
+    }
+    __device__ __forceinline__ uint32_t block(uint32_t t, uint32_t i) const { return keys ? 2 * (first + i) + t : first + i; }
+};
+__device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint64_t x, uint64_t end) {
+    Segment s;
+    s.job = job_of(p, x);
+    s.first = static_cast<uint32_t>(x - s.job.begin);
+    s.n = static_cast<uint32_t>(min(end, s.job.begin + s.job.steps) - x);
+    s.keys = s.job.pair == p.pairs;
+    return s;
+}
+
+// Warps 0-3 and 4-7 are the softmax of row tile (or key half) 0 and 1, a
+// thread per row; warp 8 loads, warp 9 issues the MMAs. TMEM: output 0, 1 and
+// scores 0, 1, 128 columns each; the probabilities overwrite the scores they
+// come from (two per column), and the next score tile is issued behind the
+// product that reads them.
+//
+// The running maximum is lazy: rows keep an old m until a score passes it by
+// more than 2^8, so that the accumulator is rescaled a few times per row
+// instead of once per block; p <= 2^8 then, which float sums and both 16-bit
+// types hold. The sum is of the unrounded p.
+template <bool BF16>
+__global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                        const __grid_constant__ CUtensorMap map_e,
+                                                        const __grid_constant__ CUtensorMap map_v,
+                                                        const __grid_constant__ AttnArgs a, const PrefixPlan p,
+                                                        const Parts parts) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t nm = a.main / 64, nk = nm + a.extra / 64, nv = a.value / 64;
+    const uint32_t slots = ring_slots(nk);
+    uint8_t* q_smem = base;                       // [2][nk] atoms
+    uint8_t* ring = base + 2 * nk * kAtom;        // [slots] atoms
+    PrefixBars& bar = *reinterpret_cast<PrefixBars*>(ring + slots * kAtom);
+    volatile int* abort = &bar.abort;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < slots; ++s) {
+            tc::mbar_init(&bar.full[s], 1);
+            tc::mbar_init(&bar.empty[s], 1);
+        }
+        for (uint32_t t = 0; t < 2; ++t) {
+            tc::mbar_init(&bar.s_full[t], 1);
+            tc::mbar_init(&bar.p_ready[t], 128);
+            tc::mbar_init(&bar.q_ready[t], 128);
+            tc::mbar_init(&bar.o_done[t], 1);
+        }
+        tc::mbar_init(&bar.teardown, 1);
+        bar.abort = 0;
+        tc::fence_barrier_init();
+    }
+    if (warp == 9) tc::tmem_alloc(&bar.tmem_base, 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = bar.tmem_base;
+    const uint64_t lo = first_step(p, blockIdx.x), hi = first_step(p, blockIdx.x + 1);
+
+    if (warp == 8 && lane == 0) {
+        // ---------------- loads, in the order the MMAs use them ----------------
+        uint32_t pos = 0;
+        bool ok = true;
+        auto slot_for = [&](uint32_t& st) {
+            st = pos % slots;
+            ok = ok && tc::mbar_wait(&bar.empty[st], ((pos / slots) & 1u) ^ 1u, abort);
+            if (ok) {
+                tc::mbar_arrive_expect_tx(&bar.full[st], kAtom);
+                ++pos;
+            }
+            return ok;
+        };
+        auto load_k = [&](uint32_t head, uint32_t block) {
+            for (uint32_t i = 0; i < nk; ++i) {
+                uint32_t st;
+                if (!slot_for(st)) return;
+                if (i < nm) tc::tma_load_3d(ring + st * kAtom, &map_k, &bar.full[st], i * 128, head, block * kTile);
+                else tc::tma_load_3d(ring + st * kAtom, &map_e, &bar.full[st], 0, 0, block * kTile);
+            }
+        };
+        auto load_v = [&](uint32_t head, uint32_t block) {
+            for (uint32_t i = 0; i < nv; ++i) {
+                uint32_t st;
+                if (!slot_for(st)) return;
+                tc::tma_load_3d(ring + st * kAtom, &map_v, &bar.full[st], i * 128, head, block * kTile);
+            }
+        };
+        tc::prefetch_tensormap(&map_k);
+        tc::prefetch_tensormap(&map_v);
+        for (uint64_t x = lo; x < hi && ok;) {
+            const Segment s = segment_at(p, x, hi);
+            const uint32_t h = s.job.head, n1 = s.active(1, p.blocks);
+            load_k(h, s.block(0, 0));
+            if (s.keys && n1) load_k(h, s.block(1, 0));
+            for (uint32_t i = 0; i < s.n && ok; ++i) {
+                load_v(h, s.block(0, i));
+                if (i + 1 < s.n) load_k(h, s.block(0, i + 1));
+                if (s.keys && i < n1) {
+                    load_v(h, s.block(1, i));
+                    if (i + 1 < n1) load_k(h, s.block(1, i + 1));
+                }
+            }
+            x += s.n;
+        }
+        volatile int never = 0;   // these waits must not be cut short by the abort flag
+        for (uint32_t i = 0; i < slots && i < pos; ++i) {
+            const uint32_t j = pos - 1 - i;
+            tc::mbar_wait(&bar.full[j % slots], (j / slots) & 1u, &never, 200000000ull);
+        }
+    } else if (warp == 9 && lane == 0) {
+        // ---------------- MMA issue ----------------
+        const uint32_t id_s = tc::idesc_f16(kTile, BF16, false), id_o = tc::idesc_f16(64, BF16, true);
+        uint32_t pos = 0, seg = 0, p_uses[2] = {0, 0};
+        bool ok = true, issued = false;
+        // scores of half t from the key atoms at ring position k0
+        auto scores = [&](uint32_t t, uint32_t k0, bool release) {
+            for (uint32_t i = 0; i < nk && ok; ++i) {
+                const uint32_t st = (k0 + i) % slots;
+                ok = tc::mbar_wait(&bar.full[st], ((k0 + i) / slots) & 1u, abort);
+                if (!ok) return;
+                tc::fence_after_sync();
+                const uint64_t qd = tc::desc_sw128(q_smem + (t * nk + i) * kAtom), kd = tc::desc_sw128(ring + st * kAtom);
+                for (uint32_t j = 0; j < 4; ++j) tc::mma_bf16(tmem + 256 + t * 128, qd + 2 * j, kd + 2 * j, id_s, i || j);
+                issued = true;
+                if (release) tc::commit(&bar.empty[st]);
+            }
+            if (ok) tc::commit(&bar.s_full[t]);
+        };
+        // output of half t: probabilities times the value atoms at v0
+        auto values = [&](uint32_t t, uint32_t v0, bool accumulate, bool release) {
+            ok = ok && tc::mbar_wait(&bar.p_ready[t], p_uses[t]++ & 1u, abort);
+            for (uint32_t i = 0; i < nv && ok; ++i) {
+                const uint32_t st = (v0 + i) % slots;
+                ok = tc::mbar_wait(&bar.full[st], ((v0 + i) / slots) & 1u, abort);
+                if (!ok) return;
+                tc::fence_after_sync();
+                const uint64_t vd = tc::desc_sw128_n(ring + st * kAtom);
+                for (uint32_t j = 0; j < 8; ++j)   // 16 keys: 8 columns of p, 2 KB of values
+                    tc::mma_f16_ts(tmem + t * 128 + i * 64, tmem + 256 + t * 128 + 8 * j, vd + 128 * j, id_o, accumulate || j);
+                issued = true;
+                if (release) tc::commit(&bar.empty[st]);
+            }
+        };
+        for (uint64_t x = lo; x < hi && ok; ++seg) {
+            const Segment s = segment_at(p, x, hi);
+            const uint32_t n1 = s.active(1, p.blocks);
+            for (uint32_t t = 0; t < 2; ++t) ok = ok && tc::mbar_wait(&bar.q_ready[t], seg & 1u, abort);
+            tc::fence_after_sync();
+            uint32_t k[2], v0;
+            k[0] = pos;
+            pos += nk;
+            k[1] = k[0];
+            if (s.keys && n1) {
+                k[1] = pos;
+                pos += nk;
+            }
+            scores(0, k[0], s.keys);
+            if (n1) scores(1, k[1], true);
+            for (uint32_t i = 0; i < s.n && ok; ++i) {
+                v0 = pos;
+                pos += nv;
+                values(0, v0, i > 0, s.keys);
+                if (i + 1 < s.n) {
+                    k[0] = pos;
+                    pos += nk;
+                    if (ok) scores(0, k[0], s.keys);
+                } else if (ok) {
+                    tc::commit(&bar.o_done[0]);
+                }
+                if (i >= n1) continue;
+                if (s.keys) {
+                    v0 = pos;
+                    pos += nv;
+                }
+                if (ok) values(1, v0, i > 0, true);
+                if (i + 1 < n1) {
+                    k[1] = k[0];
+                    if (s.keys) {
+                        k[1] = pos;
+                        pos += nk;
+                    }
+                    if (ok) scores(1, k[1], true);
+                } else if (ok) {
+                    tc::commit(&bar.o_done[1]);
+                }
+            }
+            if (!n1 && ok) tc::commit(&bar.o_done[1]);   // keeps the halves' phases in step
+            x += s.n;
+        }
+        if (issued) {   // all issued MMAs finish before TMEM is freed
+            volatile int never = 0;
+            tc::commit(&bar.teardown);
+            tc::mbar_wait(&bar.teardown, 0, &never, 200000000ull);
+        }
+    } else if (warp < 8) {
+        // ---------------- softmax ----------------
+        const uint32_t t = warp / 4, tid = threadIdx.x % 128, row = tid;
+        const uint32_t lanes = (32u * (warp % 4)) << 16;
+        const float c = fabsf(a.scale) * kLog2e;
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale: -q
+        const uint32_t width = a.main + a.extra;
+        uint32_t s_uses = 0, seg = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* b, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(b, parity, abort));
+            tc::fence_after_sync();
+            return ok;
+        };
+        for (uint64_t x = lo; x < hi && ok; ++seg) {
+            const Segment s = segment_at(p, x, hi);
+            const uint32_t tile = 2 * s.job.pair + (s.keys ? 0 : t), n = s.active(t, p.blocks);
+            // the tile's query rows, swizzled as the MMA reads them
+            for (uint32_t i = tid; i < kTile * nk * 8; i += 128) {
+                const uint32_t ch = i % (nk * 8), r = i / (nk * 8), gr = tile * kTile + r;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (gr < p.rows) {
+                    const uint64_t at = gr / p.group * a.q_row + static_cast<uint64_t>(s.job.head * p.group + gr % p.group) * width;
+                    w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at) + ch);
+                    w = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+                }
+                *reinterpret_cast<uint4*>(q_smem + (t * nk + ch / 8) * kAtom + r * 128 + (((ch % 8) ^ (r % 8)) << 4)) = w;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc::fence_before_sync();
+            tc::mbar_arrive(&bar.q_ready[t]);
+            float m = -INFINITY, l = 0.0f;
+            for (uint32_t i = 0; i < n; ++i) {
+                if (!wait(&bar.s_full[t], s_uses++ & 1u)) break;
+                uint32_t v[128];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tc::tmem_ld32(tmem + lanes + 256 + t * 128 + 32 * j, v + 32 * j);
+                tc::tmem_wait_ld();
+                const uint32_t valid = min(kTile, a.prefix_len - s.block(t, i) * kTile);
+                if (valid < kTile)
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j >= static_cast<int>(valid)) v[j] = 0xff800000u;
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 128; ++j) top[j % 4] = fmaxf(top[j % 4], __uint_as_float(v[j]));
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                if (i == 0) {
+                    m = mx;
+                } else if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+                    // the product of the block before is done: its scores' successor is
+                    const float mn = mx > m + 8.0f ? mx : m;
+                    const float keep = mn == -INFINITY ? 1.0f : ex2(m - mn);
+                    l *= keep;
+                    m = mn;
+                    for (uint32_t cc = 0; cc < a.value; cc += 32) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(tmem + lanes + t * 128 + cc, o);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                        tc::tmem_st32(tmem + lanes + t * 128 + cc, o);
+                    }
+                }
+                const float off = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q4 = 0; q4 < 2; ++q4) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float p0 = ex2(fmaf(__uint_as_float(v[64 * q4 + 2 * j]), c, -off));
+                        const float p1 = ex2(fmaf(__uint_as_float(v[64 * q4 + 2 * j + 1]), c, -off));
+                        sum[j % 2] += p0;
+                        sum[2 + j % 2] += p1;
+                        w[j] = pack2<BF16>(p0, p1);
+                    }
+                    tc::tmem_st32(tmem + lanes + 256 + t * 128 + 32 * q4, w);
+                }
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                tc::mbar_arrive(&bar.p_ready[t]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (!ok) break;
+            // the segment's part
+            const size_t part = (static_cast<size_t>(blockIdx.x) * p.max_seg + seg) * 2 + t;
+            parts.ml[part * kTile + row] = make_float2(m, l);
+            if (!wait(&bar.o_done[t], seg & 1u)) break;
+            if (n) {
+                float* dst = parts.o + (part * kTile + row) * a.value;
+                for (uint32_t cc = 0; cc < a.value; cc += 32) {
+                    uint32_t o[32];
+                    tc::tmem_ld32(tmem + lanes + t * 128 + cc, o);
+                    tc::tmem_wait_ld();
+                    if (tile * kTile + row < p.rows)
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<uint4*>(dst + cc + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
+                tc::fence_before_sync();
+            }
+            x += s.n;
+        }
+    }
+    __syncthreads();
+    if (*abort && threadIdx.x == 0) atomicExch(a.status, K3XB_BACKEND_UNAVAILABLE);
+    if (warp == 9) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- own rows, draft rows and the join --------------------------------------------
+
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1, bool bf16) {
+    if (bf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+}
+
+struct OwnPlan {
+    uint32_t row_tiles;   // 16-row tiles of a sequence's rows per kv head
+    uint32_t splits;      // CTAs along a sequence's keys
+    float* o;             // [seq][kv head][row tile][split][16][value] where splits > 1
+    float2* ml;           // [seq][kv head][row tile][split][16]
+};
+
+// A running join of parts for one row and `C` of its columns.
+template <int C>
+struct Join {
+    float m = -INFINITY, l = 0.0f, o[C];
+    __device__ __forceinline__ Join() {
+#pragma unroll
+        for (int i = 0; i < C; ++i) o[i] = 0.0f;
+    }
+    __device__ __forceinline__ void add(float2 ml, const float* src) {
+        if (ml.x == -INFINITY && ml.y == 0.0f) return;   // no visible key: o was never written
+        const float mn = fmaxf(m, ml.x), at = mn == -INFINITY ? 0.0f : mn;
+        const float w0 = ex2(m - at), w1 = ex2(ml.x - at);
+        l = fmaf(l, w0, ml.y * w1);
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < C; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(src + i);
+            o[i] = fmaf(o[i], w0, x.x * w1);
+            o[i + 1] = fmaf(o[i + 1], w0, x.y * w1);
+            o[i + 2] = fmaf(o[i + 2], w0, x.z * w1);
+            o[i + 3] = fmaf(o[i + 3], w0, x.w * w1);
+        }
+    }
+};
+
+// Adds the prefix's parts of row r (of kv head h), columns col .. col + C.
+template <int C>
+__device__ __forceinline__ void join_prefix(Join<C>& j, const PrefixPlan& p, const Parts& parts, uint32_t h, uint32_t r,
+                                            uint32_t col, uint32_t value) {
+    if (!p.total) return;
+    const uint32_t tile = r / kTile, pair = min(tile / 2, p.pairs), jobs = p.pairs + p.odd;
+    const bool keys = pair == p.pairs;
+    const uint64_t begin = static_cast<uint64_t>(h) * p.steps_per_head + static_cast<uint64_t>(pair) * p.blocks;
+    const uint64_t end = begin + (keys ? (p.blocks + 1) / 2 : p.blocks);
+    const uint32_t c1 = static_cast<uint32_t>((end * p.ctas - 1) / p.total);
+    for (uint32_t c = static_cast<uint32_t>(((begin + 1) * p.ctas - 1) / p.total); c <= c1; ++c) {
+        const uint32_t seg = h * jobs + pair - job_of(p, first_step(p, c)).index;
+        for (uint32_t t = keys ? 0u : tile % 2; t <= (keys ? 1u : tile % 2); ++t) {
+            const size_t at = ((static_cast<size_t>(c) * p.max_seg + seg) * 2 + t) * kTile + r % kTile;
+            j.add(parts.ml[at], parts.o + at * value + col);
+        }
+    }
+}
+
+template <bool BF16, int C>
+__device__ __forceinline__ void write_row(const AttnArgs& a, const Join<C>& j, uint32_t s, uint32_t node, uint32_t head,
+                                          uint32_t col) {
+    const size_t row = (static_cast<size_t>(s) * a.N + node) * a.heads + head;
+    const float inv = j.l == 0.0f ? 0.0f : 1.0f / j.l;   // nothing visible: a zero row
+    uint32_t w[C / 2];
+#pragma unroll
+    for (int i = 0; i < C; i += 2) w[i / 2] = pack2<BF16>(j.o[i] * inv, j.o[i + 1] * inv);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.value + col);
+#pragma unroll
+    for (int i = 0; i < C / 8; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    if (a.lse && col == 0) a.lse[row] = j.l == 0.0f ? -INFINITY : (j.m + __log2f(j.l)) * kLn2;
+}
+
+// Replaces the infinities and NaN of two values by zeros; whether there were.
+template <bool BF16>
+__device__ __forceinline__ bool drop_nonfinite(uint32_t& w) {
+    constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
+    if (lo) w &= 0xffff0000u;
+    if (hi) w &= 0x0000ffffu;
+    return lo || hi;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float half_of(uint16_t w) {
+    if constexpr (BF16) return decode_bf16(w);
+    else return __half2float(__ushort_as_half(w));
+}
+
+constexpr uint32_t kOwnThreads = 128;
+
+// A CTA takes 16 rows of one sequence and kv head; its four warps take 16
+// keys at a time in turn. Key and value rows go straight from global memory
+// to MMA fragments, 16 bytes a lane: the contraction over key dimensions may
+// run in any order, so lane t of a quad reads 8 neighbouring dimensions and
+// feeds them to two steps of 16 (the queries are read alike), and value
+// column g of an output tile j stands for dimension 8 g + j.
+//
+// Draft rows are masked by the node's ancestors. A masked key's probability
+// is zero, but zero times a value that is infinite or NaN is not, so the
+// product takes such values of draft rows as zeros, and the rows that do see
+// them add them one by one.
+template <int DQ, int DV, bool BF16>
+__global__ void __launch_bounds__(kOwnThreads) own_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
+                                                          const Parts parts, const OwnPlan own) {
+    constexpr int SEG = DQ / 32, H = DV / 64, LD = DV + 4;
+    __shared__ float sm_o[4][16][LD];
+    __shared__ float2 sm_ml[4][16];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const uint32_t split = blockIdx.x % own.splits, rt = blockIdx.x / own.splits % own.row_tiles;
+    const uint32_t h = blockIdx.x / own.splits / own.row_tiles, s = blockIdx.y;
+    const uint32_t group = a.heads / a.kv_heads, rows = a.N * group;
+    const int32_t len = own_rows(a, s);
+    const uint32_t keys = len < 0 ? 0u : static_cast<uint32_t>(len) + a.N;
+    const float c = fabsf(a.scale) * kLog2e;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    // this split's keys, in tiles of 16
+    const uint32_t tiles = (keys + 15) / 16;
+    const uint32_t k_end = min(keys, (split + 1) * ((tiles + own.splits - 1) / own.splits) * 16);
+
+    uint4 q[SEG][2];
+    uint64_t seen[2];   // draft rows that rows g and g + 8 see
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t r = rt * 16 + g + 8 * i;
+        const bool there = r < rows;
+        const uint32_t node = there ? r / group : 0;
+        seen[i] = there ? a.ancestors[node] : 0;
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (static_cast<size_t>(s) * a.N + node) * a.q_row +
+                              static_cast<size_t>(h * group + r % group) * DQ + t * 8;
+#pragma unroll
+        for (int j = 0; j < SEG; ++j) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (there) w = __ldg(reinterpret_cast<const uint4*>(src + j * 32));
+            q[j][i] = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+        }
+    }
+    const uint16_t* kp = static_cast<const uint16_t*>(a.suffix.k) + s * a.suffix.k_seq + h * a.suffix.k_head + t * 8;
+    const uint16_t* ep = static_cast<const uint16_t*>(a.suffix.extra) + s * a.suffix.extra_seq + t * 8;
+    const uint16_t* vp = static_cast<const uint16_t*>(a.suffix.v) + s * a.suffix.v_seq + h * a.suffix.v_head + g * 8;
+    const uint32_t main_seg = a.main / 32;
+    float o[H][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < H; ++x)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[x][j][e] = 0.0f;
+
+    for (uint32_t k0 = split * ((tiles + own.splits - 1) / own.splits) * 16 + 16 * warp; k0 < k_end; k0 += 64) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        uint4 kr[2][SEG], vr[4][H];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint64_t key = k0 + 8 * x + g;
+#pragma unroll
+            for (int j = 0; j < SEG; ++j) {
+                const uint16_t* src = static_cast<uint32_t>(j) < main_seg ? kp + key * a.suffix.k_row + j * 32
+                                                                        : ep + key * a.suffix.extra_row + (j - main_seg) * 32;
+                kr[x][j] = key < keys ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint64_t key = k0 + 2 * t + (x & 1) + 8 * (x >> 1);
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+                vr[x][j] = key < keys ? __ldg(reinterpret_cast<const uint4*>(vp + key * a.suffix.v_row + j * 64)) : zero;
+        }
+        float sc[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            sc[x][0] = sc[x][1] = sc[x][2] = sc[x][3] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < SEG; ++j) {
+                const uint32_t a0[4] = {q[j][0].x, q[j][1].x, q[j][0].y, q[j][1].y}, a1[4] = {q[j][0].z, q[j][1].z, q[j][0].w, q[j][1].w};
+                mma16(sc[x], a0, kr[x][j].x, kr[x][j].y, BF16);
+                mma16(sc[x], a1, kr[x][j].z, kr[x][j].w, BF16);
+            }
+        }
+        const bool drafts = k0 + 16 > static_cast<uint32_t>(len);
+        uint32_t vis = 0xffu;   // bit 4 x + e: key of sc[x][e] is visible to its row
+        if (drafts) {
+            vis = 0;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t key = k0 + 8 * x + 2 * t + (e & 1);
+                    const bool see = key < static_cast<uint32_t>(len) || (key < keys && (seen[e >> 1] >> (key - len) & 1u));
+                    if (see) vis |= 1u << (4 * x + e);
+                    else sc[x][e] = -INFINITY;
+                }
+        }
+        float top[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float v = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+            top[i] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2)) * c;
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float mn = fmaxf(m[i], top[i]), keep = mn == -INFINITY ? 1.0f : ex2(m[i] - mn);
+                m[i] = mn;
+                l[i] *= keep;
+#pragma unroll
+                for (int x = 0; x < H; ++x)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[x][j][2 * i] *= keep;
+                        o[x][j][2 * i + 1] *= keep;
+                    }
+            }
+        }
+        const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        float pr[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pr[x][e] = ex2(fmaf(sc[x][e], c, -off[e >> 1]));
+                l[e >> 1] += pr[x][e];
+            }
+        bool odd_values = false;
+        if (drafts) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int j = 0; j < H; ++j)
+                    odd_values |= drop_nonfinite<BF16>(vr[x][j].x) | drop_nonfinite<BF16>(vr[x][j].y) |
+                                  drop_nonfinite<BF16>(vr[x][j].z) | drop_nonfinite<BF16>(vr[x][j].w);
+        }
+        if (drafts && __any_sync(0xffffffffu, odd_values)) {
+            // one key at a time: its probabilities from the lane that has
+            // them, its values from memory
+            for (uint32_t kk = 0; kk < 16 && k0 + kk < keys; ++kk) {
+                const uint32_t src = (lane & ~3u) | (kk % 8 / 2), bit = 4 * (kk / 8) + kk % 2;
+                const uint32_t sv = __shfl_sync(0xffffffffu, vis, src);
+                float pk[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float lo = kk % 2 ? pr[0][2 * i + 1] : pr[0][2 * i], hi = kk % 2 ? pr[1][2 * i + 1] : pr[1][2 * i];
+                    pk[i] = __shfl_sync(0xffffffffu, kk < 8 ? lo : hi, src);
+                }
+                const uint16_t* row = static_cast<const uint16_t*>(a.suffix.v) + s * a.suffix.v_seq + h * a.suffix.v_head +
+                                      static_cast<uint64_t>(k0 + kk) * a.suffix.v_row;
+#pragma unroll
+                for (int x = 0; x < H; ++x)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float v = half_of<BF16>(row[x * 64 + (2 * t + e) * 8 + j]);
+                            if (isfinite(v)) continue;
+                            if (sv >> bit & 1u) o[x][j][e] = fmaf(pk[0], v, o[x][j][e]);
+                            if (sv >> (bit + 2) & 1u) o[x][j][2 + e] = fmaf(pk[1], v, o[x][j][2 + e]);
+                        }
+            }
+        }
+        const uint32_t pa[4] = {pack2<BF16>(pr[0][0], pr[0][1]), pack2<BF16>(pr[0][2], pr[0][3]),
+                                pack2<BF16>(pr[1][0], pr[1][1]), pack2<BF16>(pr[1][2], pr[1][3])};
+#pragma unroll
+        for (int x = 0; x < H; ++x) {
+            const uint32_t v0[4] = {vr[0][x].x, vr[0][x].y, vr[0][x].z, vr[0][x].w}, v1[4] = {vr[1][x].x, vr[1][x].y, vr[1][x].z, vr[1][x].w};
+            const uint32_t v2[4] = {vr[2][x].x, vr[2][x].y, vr[2][x].z, vr[2][x].w}, v3[4] = {vr[3][x].x, vr[3][x].y, vr[3][x].z, vr[3][x].w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t pick = j % 2 ? 0x7632u : 0x5410u;
+                mma16(o[x][j], pa, __byte_perm(v0[j / 2], v1[j / 2], pick), __byte_perm(v2[j / 2], v3[j / 2], pick), BF16);
+            }
+        }
+    }
+    // the four warps' results, then the row's parts
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (t == 0) sm_ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int x = 0; x < H; ++x)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < 8; j += 4)
+                    *reinterpret_cast<float4*>(&sm_o[warp][g + 8 * i][x * 64 + (2 * t + e) * 8 + j]) =
+                        make_float4(o[x][j][2 * i + e], o[x][j + 1][2 * i + e], o[x][j + 2][2 * i + e], o[x][j + 3][2 * i + e]);
+    }
+    __syncthreads();
+    constexpr int C = DV / 8;
+    const uint32_t row = threadIdx.x / 8, col = threadIdx.x % 8 * C, r = rt * 16 + row;
+    Join<C> j;
+    for (int w = 0; w < 4; ++w) j.add(sm_ml[w][row], &sm_o[w][row][col]);
+    if (own.splits > 1) {
+        const size_t at = (((static_cast<size_t>(s) * a.kv_heads + h) * own.row_tiles + rt) * own.splits + split) * 16 + row;
+        if (col == 0) own.ml[at] = make_float2(j.m, j.l);
+#pragma unroll
+        for (int i = 0; i < C; i += 4)
+            *reinterpret_cast<float4*>(own.o + at * DV + col + i) = make_float4(j.o[i], j.o[i + 1], j.o[i + 2], j.o[i + 3]);
+        return;
+    }
+    if (p.total) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (r >= rows) return;
+    if (len >= 0) join_prefix(j, p, parts, h, (s * a.N) * group + r, col, DV);
+    write_row<BF16>(a, j, s, r / group, h * group + r % group, col);
+}
+
+// The join on its own, where own_kernel split the keys.
+template <int DV, bool BF16>
+__global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
+                                                           const Parts parts, const OwnPlan own) {
+    constexpr int C = DV / 8;
+    const uint32_t rt = blockIdx.x % own.row_tiles, h = blockIdx.x / own.row_tiles, s = blockIdx.y;
+    const uint32_t group = a.heads / a.kv_heads, rows = a.N * group;
+    const uint32_t row = threadIdx.x / 8, col = threadIdx.x % 8 * C, r = rt * 16 + row;
+    if (r >= rows) return;
+    Join<C> j;
+    if (own_rows(a, s) >= 0) {
+        const size_t at = ((static_cast<size_t>(s) * a.kv_heads + h) * own.row_tiles + rt) * own.splits * 16 + row;
+        for (uint32_t i = 0; i < own.splits; ++i) j.add(own.ml[at + 16 * i], own.o + (at + 16 * i) * DV + col);
+        join_prefix(j, p, parts, h, (s * a.N) * group + r, col, DV);
+    }
+    write_row<BF16>(a, j, s, r / group, h * group + r % group, col);
+}
+
+template <int DQ, int DV, bool BF16>
+int launch_own(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.kv_heads * own.row_tiles * own.splits, a.S);
+    cfg.blockDim = dim3(kOwnThreads);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    // beside the prefix kernel's tail (it waits there before it joins); a
+    // split launch leaves the join, and the wait, to join_kernel
+    cfg.numAttrs = p.total && own.splits == 1 ? 1 : 0;
+    K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16>, a, p, parts, own));
+    ++ctx->stats.kernel_launches;
+    if (own.splits > 1) {
+        join_kernel<DV, BF16><<<dim3(a.kv_heads * own.row_tiles, a.S), kOwnThreads, 0, ctx->stream>>>(a, p, parts, own);
+        K3XB_LAUNCHED(ctx);
+    }
+    return K3XB_OK;
+}
+
+template <bool BF16>
+int launch_typed(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
+    if (p.total) {
+        const uint32_t nk = (a.main + a.extra) / 64;
+        static std::atomic<uint64_t> configured{0};   // per type
+        const int cst = configure_once(ctx, configured, [&]() -> int {
+            K3XB_CUDA(ctx, cudaFuncSetAttribute(prefix_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                static_cast<int>(std::max({prefix_smem(1), prefix_smem(2), prefix_smem(3)}))));
+            return K3XB_OK;
+        });
+        if (cst) return cst;
+        CUtensorMap map_k, map_v, map_e;
+        const KvSource& x = a.prefix;
+        int st;
+        if ((st = make_row_map(ctx, &map_k, x.k, 2ull * a.main, a.kv_heads, a.prefix_len, 2 * x.k_head, 2 * x.k_row, kTile))) return st;
+        if ((st = make_row_map(ctx, &map_v, x.v, 2ull * a.value, a.kv_heads, a.prefix_len, 2 * x.v_head, 2 * x.v_row, kTile))) return st;
+        map_e = map_k;
+        if (a.extra && (st = make_row_map(ctx, &map_e, x.extra, 2ull * a.extra, 1, a.prefix_len, 2 * x.extra_row, 2 * x.extra_row, kTile)))
+            return st;
+        prefix_kernel<BF16><<<p.ctas, 320, prefix_smem(nk), ctx->stream>>>(map_k, map_e, map_v, a, p, parts);
+        K3XB_LAUNCHED(ctx);
+    }
+    const uint32_t dq = a.main + a.extra;
+    if (a.value == 64)
+        return dq == 64 ? launch_own<64, 64, BF16>(ctx, a, p, parts, own)
+               : dq == 128 ? launch_own<128, 64, BF16>(ctx, a, p, parts, own) : launch_own<192, 64, BF16>(ctx, a, p, parts, own);
+    return dq == 64 ? launch_own<64, 128, BF16>(ctx, a, p, parts, own)
+           : dq == 128 ? launch_own<128, 128, BF16>(ctx, a, p, parts, own) : launch_own<192, 128, BF16>(ctx, a, p, parts, own);
+}
+
+bool whole16(const void* ptr, std::initializer_list<uint64_t> strides) {
+    bool ok = reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
+    for (uint64_t s : strides) ok = ok && s % 8 == 0 && s < (1ull << 38);
+    return ok;
+}
+
+}  // namespace
+
+bool attend_tc_takes(const AttnArgs& a, int32_t type) {
+    if (type != K3XB_TYPE_BF16 && type != K3XB_TYPE_F16) return false;
+    if ((a.main != 64 && a.main != 128) || (a.extra != 0 && a.extra != 64) || (a.value != 64 && a.value != 128)) return false;
+    bool ok = whole16(a.q, {a.q_row}) && whole16(a.out, {});
+    for (const KvSource* x : {&a.prefix, &a.suffix}) {
+        if (x == &a.prefix && !a.prefix_len) continue;
+        ok = ok && whole16(x->k, {x->k_row, x->k_head, x->k_seq}) && whole16(x->v, {x->v_row, x->v_head, x->v_seq}) &&
+             (!a.extra || whole16(x->extra, {x->extra_row, x->extra_seq}));
+    }
+    // masked scores are -inf times the scale, and row indices of a kv head 32-bit
+    return ok && a.scale != 0.0f && static_cast<uint64_t>(a.S) * a.N * (a.heads / a.kv_heads) < (1ull << 31);
+}
+
+int launch_attend_tc(k3xb_ctx* ctx, const AttnArgs& a, bool bf16) {
+    const uint32_t sms = static_cast<uint32_t>(ctx->sm_count), group = a.heads / a.kv_heads;
+    PrefixPlan p{};
+    p.rows = a.S * a.N * group;
+    p.group = group;
+    p.blocks = static_cast<uint32_t>((static_cast<uint64_t>(a.prefix_len) + kTile - 1) / kTile);
+    const uint32_t tiles = (p.rows + kTile - 1) / kTile;
+    p.pairs = tiles / 2;
+    p.odd = tiles % 2;
+    const uint64_t per_head = static_cast<uint64_t>(p.pairs) * p.blocks + p.odd * ((p.blocks + 1) / 2);
+    if (per_head >= (1ull << 31)) return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: rows times prefix too large");
+    p.steps_per_head = static_cast<uint32_t>(per_head);
+    p.total = per_head * a.kv_heads;
+    if (p.total) {
+        p.ctas = static_cast<uint32_t>(std::min<uint64_t>(sms, p.total));
+        const uint64_t range = (p.total + p.ctas - 1) / p.ctas;
+        p.max_seg = static_cast<uint32_t>(range / (p.odd ? (p.blocks + 1) / 2 : p.blocks) + 2);
+    }
+    OwnPlan own{};
+    own.row_tiles = (a.N * group + 15) / 16;
+    // Enough CTAs for two per SM; a split has 256 cache rows at least
+    // (by the capacity: lengths are on the device).
+    const uint64_t ctas = static_cast<uint64_t>(a.S) * a.kv_heads * own.row_tiles;
+    own.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((2 * sms + ctas - 1) / ctas, a.capacity / 256)));
+    Parts parts{};
+    auto carve = [&](auto& c) {
+        const size_t n = static_cast<size_t>(p.total ? p.ctas : 0) * p.max_seg * 2 * kTile;
+        const size_t k = own.splits > 1 ? static_cast<size_t>(ctas) * own.splits * 16 : 0;
+        parts.o = c.template take<float>(n * a.value);
+        parts.ml = c.template take<float2>(n);
+        own.o = c.template take<float>(k * a.value);
+        own.ml = c.template take<float2>(k);
+    };
+    Sizer sz;
+    carve(sz);
+    void* mem;
+    if (const int st = ensure_scratch(ctx, sz.used, &mem)) return st;
+    Carver cv(mem);
+    carve(cv);
+    return bf16 ? launch_typed<true>(ctx, a, p, parts, own) : launch_typed<false>(ctx, a, p, parts, own);
+}
+
+}  // namespace k3xb
