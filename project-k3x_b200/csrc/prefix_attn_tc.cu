@@ -39,6 +39,31 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
+// Two floats in one register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t pair_bits(uint32_t x, uint32_t y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_of(float x, float y) { return pair_bits(__float_as_uint(x), __float_as_uint(y)); }
+__device__ __forceinline__ void split_pair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
 // Two floats rounded to the 16-bit type, `lo` in the low half.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -53,6 +78,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 constexpr uint32_t kTile = 128;          // rows and keys of a tile
 constexpr uint32_t kAtom = kTile * 128;  // bytes of 128 rows x 64 values
 constexpr uint32_t kMaxSlots = 12;       // ring slots of one atom
+// Three warpgroups, launched with 168 registers a thread (64,512 in all):
+// the two softmax ones take 208, the third keeps 88 (64,512).
+constexpr uint32_t kPrefixThreads = 384;
 
 // Row tiles are taken in pairs that share a step's keys; a last odd tile
 // takes two key blocks a step instead, one per half of the CTA.
@@ -90,7 +118,7 @@ struct Parts {
 };
 
 struct PrefixBars {
-    uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2], q_ready[2], o_done[2], teardown;
+    uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2][2], q_ready[2], o_done[2], teardown;
     uint32_t tmem_base;
     int abort;
 };
@@ -123,7 +151,8 @@ __device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint64_t x, u
 }
 
 // Warps 0-3 and 4-7 are the softmax of row tile (or key half) 0 and 1, a
-// thread per row; warp 8 loads, warp 9 issues the MMAs. TMEM: output 0, 1 and
+// thread per row; warp 8 loads, warp 9 issues the MMAs (10 and 11 only fill
+// the warpgroup). TMEM: output 0, 1 and
 // scores 0, 1, 128 columns each; the probabilities overwrite the scores they
 // come from (two per column), and the next score tile is issued behind the
 // product that reads them.
@@ -132,18 +161,17 @@ __device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint64_t x, u
 // more than 2^8, so that the accumulator is rescaled a few times per row
 // instead of once per block; p <= 2^8 then, which float sums and both 16-bit
 // types hold. The sum is of the unrounded p.
-template <bool BF16>
-__global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ CUtensorMap map_k,
+template <bool BF16, uint32_t NK, uint32_t NV>
+__global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_constant__ CUtensorMap map_k,
                                                         const __grid_constant__ CUtensorMap map_e,
                                                         const __grid_constant__ CUtensorMap map_v,
                                                         const __grid_constant__ AttnArgs a, const PrefixPlan p,
                                                         const Parts parts) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t nm = a.main / 64, nk = nm + a.extra / 64, nv = a.value / 64;
-    const uint32_t slots = ring_slots(nk);
-    uint8_t* q_smem = base;                       // [2][nk] atoms
-    uint8_t* ring = base + 2 * nk * kAtom;        // [slots] atoms
+    constexpr uint32_t slots = ring_slots(NK), value = 64 * NV;
+    uint8_t* q_smem = base;                       // [2][NK] atoms
+    uint8_t* ring = base + 2 * NK * kAtom;        // [slots] atoms
     PrefixBars& bar = *reinterpret_cast<PrefixBars*>(ring + slots * kAtom);
     volatile int* abort = &bar.abort;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -155,7 +183,8 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
         }
         for (uint32_t t = 0; t < 2; ++t) {
             tc::mbar_init(&bar.s_full[t], 1);
-            tc::mbar_init(&bar.p_ready[t], 128);
+            tc::mbar_init(&bar.p_ready[t][0], 128);
+            tc::mbar_init(&bar.p_ready[t][1], 128);
             tc::mbar_init(&bar.q_ready[t], 128);
             tc::mbar_init(&bar.o_done[t], 1);
         }
@@ -170,168 +199,207 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
     const uint32_t tmem = bar.tmem_base;
     const uint64_t lo = first_step(p, blockIdx.x), hi = first_step(p, blockIdx.x + 1);
 
-    if (warp == 8 && lane == 0) {
-        // ---------------- loads, in the order the MMAs use them ----------------
-        uint32_t pos = 0;
-        bool ok = true;
-        auto slot_for = [&](uint32_t& st) {
-            st = pos % slots;
-            ok = ok && tc::mbar_wait(&bar.empty[st], ((pos / slots) & 1u) ^ 1u, abort);
-            if (ok) {
-                tc::mbar_arrive_expect_tx(&bar.full[st], kAtom);
-                ++pos;
-            }
-            return ok;
-        };
-        auto load_k = [&](uint32_t head, uint32_t block) {
-            for (uint32_t i = 0; i < nk; ++i) {
-                uint32_t st;
-                if (!slot_for(st)) return;
-                if (i < nm) tc::tma_load_3d(ring + st * kAtom, &map_k, &bar.full[st], i * 128, head, block * kTile);
-                else tc::tma_load_3d(ring + st * kAtom, &map_e, &bar.full[st], 0, 0, block * kTile);
-            }
-        };
-        auto load_v = [&](uint32_t head, uint32_t block) {
-            for (uint32_t i = 0; i < nv; ++i) {
-                uint32_t st;
-                if (!slot_for(st)) return;
-                tc::tma_load_3d(ring + st * kAtom, &map_v, &bar.full[st], i * 128, head, block * kTile);
-            }
-        };
-        tc::prefetch_tensormap(&map_k);
-        tc::prefetch_tensormap(&map_v);
-        for (uint64_t x = lo; x < hi && ok;) {
-            const Segment s = segment_at(p, x, hi);
-            const uint32_t h = s.job.head, n1 = s.active(1, p.blocks);
-            load_k(h, s.block(0, 0));
-            if (s.keys && n1) load_k(h, s.block(1, 0));
-            for (uint32_t i = 0; i < s.n && ok; ++i) {
-                load_v(h, s.block(0, i));
-                if (i + 1 < s.n) load_k(h, s.block(0, i + 1));
-                if (s.keys && i < n1) {
-                    load_v(h, s.block(1, i));
-                    if (i + 1 < n1) load_k(h, s.block(1, i + 1));
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8 && lane == 0) {
+            // ---------------- loads, in the order the MMAs use them ----------------
+            const uint32_t nm = a.main / 64;
+            uint32_t pos = 0;
+            bool ok = true;
+            auto slot_for = [&](uint32_t& st) {
+                st = pos % slots;
+                ok = ok && tc::mbar_wait(&bar.empty[st], ((pos / slots) & 1u) ^ 1u, abort);
+                if (ok) {
+                    tc::mbar_arrive_expect_tx(&bar.full[st], kAtom);
+                    ++pos;
                 }
-            }
-            x += s.n;
-        }
-        volatile int never = 0;   // these waits must not be cut short by the abort flag
-        for (uint32_t i = 0; i < slots && i < pos; ++i) {
-            const uint32_t j = pos - 1 - i;
-            tc::mbar_wait(&bar.full[j % slots], (j / slots) & 1u, &never, 200000000ull);
-        }
-    } else if (warp == 9 && lane == 0) {
-        // ---------------- MMA issue ----------------
-        const uint32_t id_s = tc::idesc_f16(kTile, BF16, false), id_o = tc::idesc_f16(64, BF16, true);
-        uint32_t pos = 0, seg = 0, p_uses[2] = {0, 0};
-        bool ok = true, issued = false;
-        // scores of half t from the key atoms at ring position k0
-        auto scores = [&](uint32_t t, uint32_t k0, bool release) {
-            for (uint32_t i = 0; i < nk && ok; ++i) {
-                const uint32_t st = (k0 + i) % slots;
-                ok = tc::mbar_wait(&bar.full[st], ((k0 + i) / slots) & 1u, abort);
-                if (!ok) return;
-                tc::fence_after_sync();
-                const uint64_t qd = tc::desc_sw128(q_smem + (t * nk + i) * kAtom), kd = tc::desc_sw128(ring + st * kAtom);
-                for (uint32_t j = 0; j < 4; ++j) tc::mma_bf16(tmem + 256 + t * 128, qd + 2 * j, kd + 2 * j, id_s, i || j);
-                issued = true;
-                if (release) tc::commit(&bar.empty[st]);
-            }
-            if (ok) tc::commit(&bar.s_full[t]);
-        };
-        // output of half t: probabilities times the value atoms at v0
-        auto values = [&](uint32_t t, uint32_t v0, bool accumulate, bool release) {
-            ok = ok && tc::mbar_wait(&bar.p_ready[t], p_uses[t]++ & 1u, abort);
-            for (uint32_t i = 0; i < nv && ok; ++i) {
-                const uint32_t st = (v0 + i) % slots;
-                ok = tc::mbar_wait(&bar.full[st], ((v0 + i) / slots) & 1u, abort);
-                if (!ok) return;
-                tc::fence_after_sync();
-                const uint64_t vd = tc::desc_sw128_n(ring + st * kAtom);
-                for (uint32_t j = 0; j < 8; ++j)   // 16 keys: 8 columns of p, 2 KB of values
-                    tc::mma_f16_ts(tmem + t * 128 + i * 64, tmem + 256 + t * 128 + 8 * j, vd + 128 * j, id_o, accumulate || j);
-                issued = true;
-                if (release) tc::commit(&bar.empty[st]);
-            }
-        };
-        for (uint64_t x = lo; x < hi && ok; ++seg) {
-            const Segment s = segment_at(p, x, hi);
-            const uint32_t n1 = s.active(1, p.blocks);
-            for (uint32_t t = 0; t < 2; ++t) ok = ok && tc::mbar_wait(&bar.q_ready[t], seg & 1u, abort);
-            tc::fence_after_sync();
-            uint32_t k[2], v0;
-            k[0] = pos;
-            pos += nk;
-            k[1] = k[0];
-            if (s.keys && n1) {
-                k[1] = pos;
-                pos += nk;
-            }
-            scores(0, k[0], s.keys);
-            if (n1) scores(1, k[1], true);
-            for (uint32_t i = 0; i < s.n && ok; ++i) {
-                v0 = pos;
-                pos += nv;
-                values(0, v0, i > 0, s.keys);
-                if (i + 1 < s.n) {
-                    k[0] = pos;
-                    pos += nk;
-                    if (ok) scores(0, k[0], s.keys);
-                } else if (ok) {
-                    tc::commit(&bar.o_done[0]);
+                return ok;
+            };
+            auto load_k = [&](uint32_t head, uint32_t block) {
+#pragma unroll
+                for (uint32_t i = 0; i < NK; ++i) {
+                    uint32_t st;
+                    if (!slot_for(st)) return;
+                    if (i < nm) tc::tma_load_3d(ring + st * kAtom, &map_k, &bar.full[st], i * 128, head, block * kTile);
+                    else tc::tma_load_3d(ring + st * kAtom, &map_e, &bar.full[st], 0, 0, block * kTile);
                 }
-                if (i >= n1) continue;
-                if (s.keys) {
-                    v0 = pos;
-                    pos += nv;
+            };
+            auto load_v = [&](uint32_t head, uint32_t block) {
+#pragma unroll
+                for (uint32_t i = 0; i < NV; ++i) {   // a slot: 64 keys of 128 values, or 128 keys of 64
+                    uint32_t st;
+                    if (!slot_for(st)) return;
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e)
+                        tc::tma_load_3d(ring + st * kAtom + e * (kAtom / 2), &map_v, &bar.full[st], NV == 2 ? e * 128 : 0, head,
+                                        block * kTile + (NV == 2 ? i : e) * 64);
                 }
-                if (ok) values(1, v0, i > 0, true);
-                if (i + 1 < n1) {
-                    k[1] = k[0];
-                    if (s.keys) {
-                        k[1] = pos;
-                        pos += nk;
+            };
+            for (uint64_t x = lo; x < hi && ok;) {
+                const Segment s = segment_at(p, x, hi);
+                const uint32_t h = s.job.head, n1 = s.active(1, p.blocks);
+                load_k(h, s.block(0, 0));
+                if (s.keys && n1) load_k(h, s.block(1, 0));
+                for (uint32_t i = 0; i < s.n && ok; ++i) {
+                    load_v(h, s.block(0, i));
+                    if (i + 1 < s.n) load_k(h, s.block(0, i + 1));
+                    if (s.keys && i < n1) {
+                        load_v(h, s.block(1, i));
+                        if (i + 1 < n1) load_k(h, s.block(1, i + 1));
                     }
-                    if (ok) scores(1, k[1], true);
-                } else if (ok) {
-                    tc::commit(&bar.o_done[1]);
                 }
+                x += s.n;
             }
-            if (!n1 && ok) tc::commit(&bar.o_done[1]);   // keeps the halves' phases in step
-            x += s.n;
+            volatile int never = 0;   // these waits must not be cut short by the abort flag
+            for (uint32_t i = 0; i < slots && i < pos; ++i) {
+                const uint32_t j = pos - 1 - i;
+                tc::mbar_wait(&bar.full[j % slots], (j / slots) & 1u, &never, 200000000ull);
+            }
+        } else if (warp == 9) {
+            // ---------------- MMA issue, by one lane of the whole warp ----------------
+            constexpr uint32_t id_s = tc::idesc_f16(kTile, BF16, false), id_o = tc::idesc_f16(value, BF16, true);
+            const uint64_t q0 = tc::desc_sw128(q_smem), k0 = tc::desc_sw128(ring), v0 = tc::desc_sw128_n(ring, kAtom / 2);
+            uint32_t pos = 0, seg = 0, p_phase = 0;   // ring position; segments; bit t: phase of p_ready[t]
+            bool ok = true, issued = false;
+            // scores of half t from the key atoms at ring position `at`
+            auto scores = [&](uint32_t t, uint32_t at, bool release) {
+                const uint32_t d = tmem + 256 + t * 128;
+#pragma unroll
+                for (uint32_t i = 0; i < NK; ++i) {
+                    const uint32_t st = (at + i) % slots;
+                    ok = ok && tc::mbar_wait_warp(&bar.full[st], ((at + i) / slots) & 1u, abort);
+                    if (!ok) return;
+                    tc::fence_after_sync();
+                    const uint64_t qd = q0 + (t * NK + i) * (kAtom >> 4), kd = k0 + st * (kAtom >> 4);
+                    if (tc::elect_one()) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) tc::mma_bf16(d, qd + 2 * j, kd + 2 * j, id_s, i || j);
+                        if (release) tc::commit(&bar.empty[st]);
+                        if (i == NK - 1) tc::commit(&bar.s_full[t]);
+                    }
+                    __syncwarp();
+                    issued = true;
+                }
+            };
+            // output of half t: its probabilities times the value atoms at
+            // `at`, 64 keys at a time (the softmax hands them over so)
+            auto values = [&](uint32_t t, uint32_t at, bool accumulate, bool release, bool last) {
+                const uint32_t d = tmem + t * 128, pr = tmem + 256 + t * 128;
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    const uint32_t st = (at + (NV == 2 ? i : 0)) % slots;
+                    ok = ok && tc::mbar_wait_warp(&bar.p_ready[t][i], p_phase >> t & 1u, abort);
+                    if (NV == 2 || !i) ok = ok && tc::mbar_wait_warp(&bar.full[st], ((at + (NV == 2 ? i : 0)) / slots) & 1u, abort);
+                    if (!ok) return;
+                    tc::fence_after_sync();
+                    const uint64_t vd = v0 + st * (kAtom >> 4) + (NV == 2 ? 0 : i * (kAtom >> 5));
+                    if (tc::elect_one()) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j)   // 16 keys: 8 columns of p, 2 KB of values
+                            tc::mma_f16_ts(d, pr + 32 * i + 8 * j, vd + 128 * j, id_o, i || j ? 1u : accumulate);
+                        if (release && (NV == 2 || i)) tc::commit(&bar.empty[st]);
+                        if (last && i) tc::commit(&bar.o_done[t]);
+                    }
+                    __syncwarp();
+                }
+                p_phase ^= 1u << t;
+            };
+            for (uint64_t x = lo; x < hi && ok; ++seg) {
+                const Segment s = segment_at(p, x, hi);
+                const uint32_t n1 = s.active(1, p.blocks);
+                for (uint32_t t = 0; t < 2; ++t) ok = ok && tc::mbar_wait_warp(&bar.q_ready[t], seg & 1u, abort);
+                tc::fence_after_sync();
+                uint32_t ka = pos;
+                pos += NK;
+                scores(0, ka, s.keys);
+                if (n1) {
+                    if (s.keys) {
+                        ka = pos;
+                        pos += NK;
+                    }
+                    scores(1, ka, true);
+                }
+                for (uint32_t i = 0; i < s.n && ok; ++i) {
+                    uint32_t va = pos;
+                    pos += NV;
+                    values(0, va, i > 0, s.keys, i + 1 == s.n);
+                    if (i + 1 < s.n) {
+                        ka = pos;
+                        pos += NK;
+                        scores(0, ka, s.keys);
+                    }
+                    if (i >= n1) continue;
+                    if (s.keys) {
+                        va = pos;
+                        pos += NV;
+                    }
+                    values(1, va, i > 0, true, i + 1 == n1);
+                    if (i + 1 < n1) {
+                        if (s.keys) {
+                            ka = pos;
+                            pos += NK;
+                        }
+                        scores(1, ka, true);
+                    }
+                }
+                if (!n1 && ok && tc::elect_one()) tc::commit(&bar.o_done[1]);   // keeps the halves' phases in step
+                __syncwarp();
+                x += s.n;
+            }
+            if (issued) {   // all issued MMAs finish before TMEM is freed
+                volatile int never = 0;
+                if (tc::elect_one()) tc::commit(&bar.teardown);
+                __syncwarp();
+                tc::mbar_wait(&bar.teardown, 0, &never, 200000000ull);
+                __syncwarp();
+            }
         }
-        if (issued) {   // all issued MMAs finish before TMEM is freed
-            volatile int never = 0;
-            tc::commit(&bar.teardown);
-            tc::mbar_wait(&bar.teardown, 0, &never, 200000000ull);
-        }
-    } else if (warp < 8) {
+    } else {
         // ---------------- softmax ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t t = warp / 4, tid = threadIdx.x % 128, row = tid;
         const uint32_t lanes = (32u * (warp % 4)) << 16;
+        const uint32_t scores_at = tmem + lanes + 256 + t * 128, out_at = tmem + lanes + t * 128;
         const float c = fabsf(a.scale) * kLog2e;
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale: -q
-        const uint32_t width = a.main + a.extra;
         uint32_t s_uses = 0, seg = 0;
         bool ok = true;
         auto wait = [&](uint64_t* b, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(b, parity, abort));
+            ok = tc::mbar_wait_warp(b, parity, abort);
             tc::fence_after_sync();
             return ok;
         };
         for (uint64_t x = lo; x < hi && ok; ++seg) {
             const Segment s = segment_at(p, x, hi);
             const uint32_t tile = 2 * s.job.pair + (s.keys ? 0 : t), n = s.active(t, p.blocks);
-            // the tile's query rows, swizzled as the MMA reads them
-            for (uint32_t i = tid; i < kTile * nk * 8; i += 128) {
-                const uint32_t ch = i % (nk * 8), r = i / (nk * 8), gr = tile * kTile + r;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (gr < p.rows) {
-                    const uint64_t at = gr / p.group * a.q_row + static_cast<uint64_t>(s.job.head * p.group + gr % p.group) * width;
-                    w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at) + ch);
-                    w = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+            // the tile's query rows, swizzled as the MMA reads them: eight
+            // threads a row, the loads of four rows in flight
+            {
+                const uint32_t ch = tid % 8;
+#pragma unroll
+                for (uint32_t r0 = tid / 8; r0 < kTile; r0 += 64) {
+                    uint4 w[4][NK];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t gr = tile * kTile + r0 + 16 * u;
+                        const uint64_t at = gr / p.group * a.q_row +
+                                            static_cast<uint64_t>(s.job.head * p.group + gr % p.group) * (64 * NK);
+#pragma unroll
+                        for (uint32_t i = 0; i < NK; ++i) {
+                            w[u][i] = make_uint4(0, 0, 0, 0);
+                            if (gr < p.rows)
+                                w[u][i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at) + 8 * i + ch);
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t r = r0 + 16 * u;
+#pragma unroll
+                        for (uint32_t i = 0; i < NK; ++i)
+                            *reinterpret_cast<uint4*>(q_smem + (t * NK + i) * kAtom + r * 128 + ((ch ^ (r % 8)) << 4)) =
+                                make_uint4(w[u][i].x ^ flip, w[u][i].y ^ flip, w[u][i].z ^ flip, w[u][i].w ^ flip);
+                    }
                 }
-                *reinterpret_cast<uint4*>(q_smem + (t * nk + ch / 8) * kAtom + r * 128 + (((ch % 8) ^ (r % 8)) << 4)) = w;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc::fence_before_sync();
@@ -341,16 +409,22 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
                 if (!wait(&bar.s_full[t], s_uses++ & 1u)) break;
                 uint32_t v[128];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) tc::tmem_ld32(tmem + lanes + 256 + t * 128 + 32 * j, v + 32 * j);
+                for (int j = 0; j < 4; ++j) tc::tmem_ld32(scores_at + 32 * j, v + 32 * j);
                 tc::tmem_wait_ld();
                 const uint32_t valid = min(kTile, a.prefix_len - s.block(t, i) * kTile);
                 if (valid < kTile)
 #pragma unroll
                     for (int j = 0; j < 128; ++j)
                         if (j >= static_cast<int>(valid)) v[j] = 0xff800000u;
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float top[4];
 #pragma unroll
-                for (int j = 0; j < 128; ++j) top[j % 4] = fmaxf(top[j % 4], __uint_as_float(v[j]));
+                for (int j = 0; j < 4; ++j) top[j] = __uint_as_float(v[j]);
+#pragma unroll
+                for (int j = 4; j < 124; j += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(v[j + e]), __uint_as_float(v[j + 4 + e]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(v[124 + e]));
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
                 if (i == 0) {
                     m = mx;
@@ -360,34 +434,41 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
                     const float keep = mn == -INFINITY ? 1.0f : ex2(m - mn);
                     l *= keep;
                     m = mn;
-                    for (uint32_t cc = 0; cc < a.value; cc += 32) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(tmem + lanes + t * 128 + cc, o);
+                    for (uint32_t cc = 0; cc < value; cc += 16) {
+                        float o[16];
+                        tc::tmem_ld16(out_at + cc, o);
                         tc::tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                        tc::tmem_st32(tmem + lanes + t * 128 + cc, o);
+                        for (int j = 0; j < 16; ++j) o[j] *= keep;
+                        tc::tmem_st16(out_at + cc, o);
                     }
                 }
                 const float off = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // x * c - off for two columns at a time, the sums too
+                const uint64_t c2 = pair_of(c, c), off2 = pair_of(-off, -off);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int q4 = 0; q4 < 2; ++q4) {
-                    uint32_t w[32];
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float p0 = ex2(fmaf(__uint_as_float(v[64 * q4 + 2 * j]), c, -off));
-                        const float p1 = ex2(fmaf(__uint_as_float(v[64 * q4 + 2 * j + 1]), c, -off));
-                        sum[j % 2] += p0;
-                        sum[2 + j % 2] += p1;
+                    for (int j = 0; j < 16; ++j) {
+                        float p0, p1;
+                        split_pair(fma2(pair_bits(v[32 * q4 + 2 * j], v[32 * q4 + 2 * j + 1]), c2, off2), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        sum[j % 2] = add2(sum[j % 2], pair_of(p0, p1));
                         w[j] = pack2<BF16>(p0, p1);
                     }
-                    tc::tmem_st32(tmem + lanes + 256 + t * 128 + 32 * q4, w);
+                    tc::tmem_st16(scores_at + 16 * q4, w);
+                    if (q4 % 2) {   // 64 keys for the product
+                        tc::tmem_wait_st();
+                        tc::fence_before_sync();
+                        tc::mbar_arrive(&bar.p_ready[t][q4 / 2]);
+                    }
                 }
-                tc::tmem_wait_st();
-                tc::fence_before_sync();
-                tc::mbar_arrive(&bar.p_ready[t]);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float s0, s1;
+                split_pair(add2(sum[0], sum[1]), s0, s1);
+                l += s0 + s1;
             }
             if (!ok) break;
             // the segment's part
@@ -395,10 +476,11 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
             parts.ml[part * kTile + row] = make_float2(m, l);
             if (!wait(&bar.o_done[t], seg & 1u)) break;
             if (n) {
-                float* dst = parts.o + (part * kTile + row) * a.value;
-                for (uint32_t cc = 0; cc < a.value; cc += 32) {
+                float* dst = parts.o + (part * kTile + row) * value;
+#pragma unroll
+                for (uint32_t cc = 0; cc < value; cc += 32) {
                     uint32_t o[32];
-                    tc::tmem_ld32(tmem + lanes + t * 128 + cc, o);
+                    tc::tmem_ld32(out_at + cc, o);
                     tc::tmem_wait_ld();
                     if (tile * kTile + row < p.rows)
 #pragma unroll
@@ -463,7 +545,8 @@ struct Join {
     }
 };
 
-// Adds the prefix's parts of row r (of kv head h), columns col .. col + C.
+// Adds the prefix's parts of row r (of kv head h), columns col .. col + C,
+// four parts' loads at a time in flight.
 template <int C>
 __device__ __forceinline__ void join_prefix(Join<C>& j, const PrefixPlan& p, const Parts& parts, uint32_t h, uint32_t r,
                                             uint32_t col, uint32_t value) {
@@ -472,13 +555,30 @@ __device__ __forceinline__ void join_prefix(Join<C>& j, const PrefixPlan& p, con
     const bool keys = pair == p.pairs;
     const uint64_t begin = static_cast<uint64_t>(h) * p.steps_per_head + static_cast<uint64_t>(pair) * p.blocks;
     const uint64_t end = begin + (keys ? (p.blocks + 1) / 2 : p.blocks);
+    const uint32_t c0 = static_cast<uint32_t>(((begin + 1) * p.ctas - 1) / p.total);
     const uint32_t c1 = static_cast<uint32_t>((end * p.ctas - 1) / p.total);
-    for (uint32_t c = static_cast<uint32_t>(((begin + 1) * p.ctas - 1) / p.total); c <= c1; ++c) {
-        const uint32_t seg = h * jobs + pair - job_of(p, first_step(p, c)).index;
-        for (uint32_t t = keys ? 0u : tile % 2; t <= (keys ? 1u : tile % 2); ++t) {
-            const size_t at = ((static_cast<size_t>(c) * p.max_seg + seg) * 2 + t) * kTile + r % kTile;
-            j.add(parts.ml[at], parts.o + at * value + col);
+    // the job is the last one that CTA c0 begins, or its only one, and the
+    // first one of the CTAs behind it
+    const uint32_t seg0 = h * jobs + pair - job_of(p, first_step(p, c0)).index;
+    const uint32_t halves = keys ? 2 : 1, n = (c1 - c0 + 1) * halves;
+    for (uint32_t i0 = 0; i0 < n; i0 += 4) {
+        size_t at[4];
+        float2 ml[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t k = min(i0 + i, n - 1), c = k / halves;
+            at[i] = ((static_cast<size_t>(c0 + c) * p.max_seg + (c ? 0 : seg0)) * 2 + (keys ? k % 2 : tile % 2)) * kTile + r % kTile;
+            ml[i] = parts.ml[at[i]];
         }
+        float4 x[4][C / 4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < C / 4; ++e)
+                x[i][e] = reinterpret_cast<const float4*>(parts.o + at[i] * value + col)[e];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (i0 + i < n) j.add(ml[i], reinterpret_cast<const float*>(x[i]));
     }
 }
 
@@ -526,11 +626,12 @@ constexpr uint32_t kOwnThreads = 128;
 // product takes such values of draft rows as zeros, and the rows that do see
 // them add them one by one.
 template <int DQ, int DV, bool BF16>
-__global__ void __launch_bounds__(kOwnThreads) own_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
+__global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
                                                           const Parts parts, const OwnPlan own) {
     constexpr int SEG = DQ / 32, H = DV / 64, LD = DV + 4;
     __shared__ float sm_o[4][16][LD];
     __shared__ float2 sm_ml[4][16];
+    __shared__ uint4 sm_q[SEG][2][32];   // the queries, as each lane's fragments need them
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const uint32_t split = blockIdx.x % own.splits, rt = blockIdx.x / own.splits % own.row_tiles;
     const uint32_t h = blockIdx.x / own.splits / own.row_tiles, s = blockIdx.y;
@@ -543,7 +644,6 @@ __global__ void __launch_bounds__(kOwnThreads) own_kernel(const __grid_constant_
     const uint32_t tiles = (keys + 15) / 16;
     const uint32_t k_end = min(keys, (split + 1) * ((tiles + own.splits - 1) / own.splits) * 16);
 
-    uint4 q[SEG][2];
     uint64_t seen[2];   // draft rows that rows g and g + 8 see
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -553,13 +653,13 @@ __global__ void __launch_bounds__(kOwnThreads) own_kernel(const __grid_constant_
         seen[i] = there ? a.ancestors[node] : 0;
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + (static_cast<size_t>(s) * a.N + node) * a.q_row +
                               static_cast<size_t>(h * group + r % group) * DQ + t * 8;
-#pragma unroll
-        for (int j = 0; j < SEG; ++j) {
+        for (uint32_t j = warp; j < SEG; j += 4) {
             uint4 w = make_uint4(0, 0, 0, 0);
             if (there) w = __ldg(reinterpret_cast<const uint4*>(src + j * 32));
-            q[j][i] = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+            sm_q[j][i][lane] = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
         }
     }
+    __syncthreads();
     const uint16_t* kp = static_cast<const uint16_t*>(a.suffix.k) + s * a.suffix.k_seq + h * a.suffix.k_head + t * 8;
     const uint16_t* ep = static_cast<const uint16_t*>(a.suffix.extra) + s * a.suffix.extra_seq + t * 8;
     const uint16_t* vp = static_cast<const uint16_t*>(a.suffix.v) + s * a.suffix.v_seq + h * a.suffix.v_head + g * 8;
@@ -592,13 +692,13 @@ __global__ void __launch_bounds__(kOwnThreads) own_kernel(const __grid_constant_
             for (int j = 0; j < H; ++j)
                 vr[x][j] = key < keys ? __ldg(reinterpret_cast<const uint4*>(vp + key * a.suffix.v_row + j * 64)) : zero;
         }
-        float sc[2][4];
+        float sc[2][4] = {};
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            sc[x][0] = sc[x][1] = sc[x][2] = sc[x][3] = 0.0f;
+        for (int j = 0; j < SEG; ++j) {
+            const uint4 q0 = sm_q[j][0][lane], q1 = sm_q[j][1][lane];
+            const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
 #pragma unroll
-            for (int j = 0; j < SEG; ++j) {
-                const uint32_t a0[4] = {q[j][0].x, q[j][1].x, q[j][0].y, q[j][1].y}, a1[4] = {q[j][0].z, q[j][1].z, q[j][0].w, q[j][1].w};
+            for (int x = 0; x < 2; ++x) {
                 mma16(sc[x], a0, kr[x][j].x, kr[x][j].y, BF16);
                 mma16(sc[x], a1, kr[x][j].z, kr[x][j].w, BF16);
             }
@@ -771,14 +871,13 @@ int launch_own(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Part
     return K3XB_OK;
 }
 
-template <bool BF16>
-int launch_typed(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
+template <uint32_t NK, uint32_t NV, bool BF16>
+int launch_both(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
     if (p.total) {
-        const uint32_t nk = (a.main + a.extra) / 64;
-        static std::atomic<uint64_t> configured{0};   // per type
+        static std::atomic<uint64_t> configured{0};   // per template instance
         const int cst = configure_once(ctx, configured, [&]() -> int {
-            K3XB_CUDA(ctx, cudaFuncSetAttribute(prefix_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                static_cast<int>(std::max({prefix_smem(1), prefix_smem(2), prefix_smem(3)}))));
+            K3XB_CUDA(ctx, cudaFuncSetAttribute(prefix_kernel<BF16, NK, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                static_cast<int>(prefix_smem(NK))));
             return K3XB_OK;
         });
         if (cst) return cst;
@@ -786,19 +885,26 @@ int launch_typed(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Pa
         const KvSource& x = a.prefix;
         int st;
         if ((st = make_row_map(ctx, &map_k, x.k, 2ull * a.main, a.kv_heads, a.prefix_len, 2 * x.k_head, 2 * x.k_row, kTile))) return st;
-        if ((st = make_row_map(ctx, &map_v, x.v, 2ull * a.value, a.kv_heads, a.prefix_len, 2 * x.v_head, 2 * x.v_row, kTile))) return st;
+        if ((st = make_row_map(ctx, &map_v, x.v, 2ull * a.value, a.kv_heads, a.prefix_len, 2 * x.v_head, 2 * x.v_row, kTile / 2))) return st;
         map_e = map_k;
         if (a.extra && (st = make_row_map(ctx, &map_e, x.extra, 2ull * a.extra, 1, a.prefix_len, 2 * x.extra_row, 2 * x.extra_row, kTile)))
             return st;
-        prefix_kernel<BF16><<<p.ctas, 320, prefix_smem(nk), ctx->stream>>>(map_k, map_e, map_v, a, p, parts);
+        prefix_kernel<BF16, NK, NV><<<p.ctas, kPrefixThreads, prefix_smem(NK), ctx->stream>>>(map_k, map_e, map_v, a, p, parts);
         K3XB_LAUNCHED(ctx);
     }
-    const uint32_t dq = a.main + a.extra;
-    if (a.value == 64)
-        return dq == 64 ? launch_own<64, 64, BF16>(ctx, a, p, parts, own)
-               : dq == 128 ? launch_own<128, 64, BF16>(ctx, a, p, parts, own) : launch_own<192, 64, BF16>(ctx, a, p, parts, own);
-    return dq == 64 ? launch_own<64, 128, BF16>(ctx, a, p, parts, own)
-           : dq == 128 ? launch_own<128, 128, BF16>(ctx, a, p, parts, own) : launch_own<192, 128, BF16>(ctx, a, p, parts, own);
+    return launch_own<64 * NK, 64 * NV, BF16>(ctx, a, p, parts, own);
+}
+
+template <bool BF16>
+int launch_typed(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
+    switch ((a.main + a.extra) / 64 * 10 + a.value / 64) {
+        case 11: return launch_both<1, 1, BF16>(ctx, a, p, parts, own);
+        case 12: return launch_both<1, 2, BF16>(ctx, a, p, parts, own);
+        case 21: return launch_both<2, 1, BF16>(ctx, a, p, parts, own);
+        case 22: return launch_both<2, 2, BF16>(ctx, a, p, parts, own);
+        case 31: return launch_both<3, 1, BF16>(ctx, a, p, parts, own);
+        default: return launch_both<3, 2, BF16>(ctx, a, p, parts, own);
+    }
 }
 
 bool whole16(const void* ptr, std::initializer_list<uint64_t> strides) {

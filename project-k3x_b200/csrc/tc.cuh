@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace k3xb {
 namespace tc {
@@ -71,6 +72,25 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
             return false;
         }
     }
+}
+
+// One lane of a converged warp. Control flow that the whole warp follows
+// leaves descriptors in uniform registers, where the MMA wants them; a
+// branch on the lane number around the whole issue loop moves every operand
+// there anew (measured: 150 cycles per MMA instead of about 30).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
+// mbar_wait for a whole warp; the same answer in every lane.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
 }
 
 // ---- TMA / bulk copies (no multicast) -------------------------------------------
@@ -196,14 +216,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+template <typename W>
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const W* w) {
+    static_assert(sizeof(W) == 4, "32-bit columns");
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if constexpr (std::is_same_v<W, float>) r[i] = __float_as_uint(w[i]);
+        else r[i] = w[i];
+    }
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
@@ -239,17 +264,18 @@ __host__ __device__ __forceinline__ uint32_t idesc_bf16(uint32_t n) {
 
 // The same for either 16-bit type, and with B stored N-major (rows of N
 // contiguous values, one row per K).
-__host__ __device__ __forceinline__ uint32_t idesc_f16(uint32_t n, bool bf16, bool b_n_major) {
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t n, bool bf16, bool b_n_major) {
     const uint32_t f = bf16 ? 1u : 0u;
     return (1u << 4) | (f << 7) | (f << 10) | ((b_n_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// N-major operand tile of 64 values (128 bytes, 128-byte swizzle) per K row;
-// groups of 8 K rows are 1024 B apart. With one 64-value tile the other
-// offset is not used.
-__device__ __forceinline__ uint64_t desc_sw128_n(const void* smem) {
+// N-major operand tile: rows of 64 values (128 bytes, 128-byte swizzle), one
+// per K, groups of 8 K rows 1024 B apart; the next 64 values of N stand
+// `next_n` bytes on.
+__device__ __forceinline__ uint64_t desc_sw128_n(const void* smem, uint32_t next_n) {
     const uint64_t addr = smem_u32(smem);
-    return ((addr >> 4) & 0x3fffull) | ((1024ull >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    return ((addr >> 4) & 0x3fffull) | (static_cast<uint64_t>(next_n >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
 }
 
 }  // namespace tc
