@@ -78,6 +78,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 constexpr uint32_t kTile = 128;          // rows and keys of a tile
 constexpr uint32_t kAtom = kTile * 128;  // bytes of 128 rows x 64 values
 constexpr uint32_t kMaxSlots = 12;       // ring slots of one atom
+constexpr uint32_t kFullBars = 16;       // more than the blocks that the ring can hold
 // Three warpgroups, launched with 168 registers a thread (64,512 in all):
 // the two softmax ones take 208, the third keeps 88 (64,512).
 constexpr uint32_t kPrefixThreads = 384;
@@ -118,7 +119,7 @@ struct Parts {
 };
 
 struct PrefixBars {
-    uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_ready[2][2], q_ready[2], o_done[2], teardown;
+    uint64_t full[kFullBars], empty[kMaxSlots], s_full[2], p_ready[2][2], q_ready[2], o_done[2], teardown;
     uint32_t tmem_base;
     int abort;
 };
@@ -150,6 +151,10 @@ __device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint64_t x, u
     return s;
 }
 
+// A wait that runs out sets the abort flag; every later one returns at once
+// then, the loops run to their end on what is in memory (the loads stop), and
+// the status word reports it.
+//
 // Warps 0-3 and 4-7 are the softmax of row tile (or key half) 0 and 1, a
 // thread per row; warp 8 loads, warp 9 issues the MMAs (10 and 11 only fill
 // the warpgroup). TMEM: output 0, 1 and
@@ -174,18 +179,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
     uint8_t* ring = base + 2 * NK * kAtom;        // [slots] atoms
     PrefixBars& bar = *reinterpret_cast<PrefixBars*>(ring + slots * kAtom);
     volatile int* abort = &bar.abort;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // the shuffle tells the compiler that a warp agrees on its role
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < slots; ++s) {
-            tc::mbar_init(&bar.full[s], 1);
-            tc::mbar_init(&bar.empty[s], 1);
-        }
+        for (uint32_t s = 0; s < kFullBars; ++s) tc::mbar_init(&bar.full[s], 1);
+        for (uint32_t s = 0; s < slots; ++s) tc::mbar_init(&bar.empty[s], 1);
         for (uint32_t t = 0; t < 2; ++t) {
             tc::mbar_init(&bar.s_full[t], 1);
-            tc::mbar_init(&bar.p_ready[t][0], 128);
-            tc::mbar_init(&bar.p_ready[t][1], 128);
-            tc::mbar_init(&bar.q_ready[t], 128);
+            tc::mbar_init(&bar.p_ready[t][0], 4);
+            tc::mbar_init(&bar.p_ready[t][1], 4);
+            tc::mbar_init(&bar.q_ready[t], 4);
             tc::mbar_init(&bar.o_done[t], 1);
         }
         tc::mbar_init(&bar.teardown, 1);
@@ -204,36 +208,34 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
         if (warp == 8 && lane == 0) {
             // ---------------- loads, in the order the MMAs use them ----------------
             const uint32_t nm = a.main / 64;
-            uint32_t pos = 0;
+            uint32_t pos = 0, blk = 0;   // atoms and key or value blocks so far
             bool ok = true;
-            auto slot_for = [&](uint32_t& st) {
-                st = pos % slots;
-                ok = ok && tc::mbar_wait(&bar.empty[st], ((pos / slots) & 1u) ^ 1u, abort);
-                if (ok) {
-                    tc::mbar_arrive_expect_tx(&bar.full[st], kAtom);
-                    ++pos;
-                }
+            // slots for a block's N atoms; its barrier counts their bytes
+            auto begin = [&](uint32_t n) {
+                for (uint32_t i = 0; i < n; ++i)
+                    ok = ok && tc::mbar_wait(&bar.empty[(pos + i) % slots], (((pos + i) / slots) & 1u) ^ 1u, abort);
+                if (ok) tc::mbar_arrive_expect_tx(&bar.full[blk++ % kFullBars], n * kAtom);
                 return ok;
             };
             auto load_k = [&](uint32_t head, uint32_t block) {
+                uint64_t* full = &bar.full[blk % kFullBars];
+                if (!begin(NK)) return;
 #pragma unroll
-                for (uint32_t i = 0; i < NK; ++i) {
-                    uint32_t st;
-                    if (!slot_for(st)) return;
-                    if (i < nm) tc::tma_load_3d(ring + st * kAtom, &map_k, &bar.full[st], i * 128, head, block * kTile);
-                    else tc::tma_load_3d(ring + st * kAtom, &map_e, &bar.full[st], 0, 0, block * kTile);
+                for (uint32_t i = 0; i < NK; ++i, ++pos) {
+                    uint8_t* dst = ring + pos % slots * kAtom;
+                    if (i < nm) tc::tma_load_3d(dst, &map_k, full, i * 128, head, block * kTile);
+                    else tc::tma_load_3d(dst, &map_e, full, 0, 0, block * kTile);
                 }
             };
             auto load_v = [&](uint32_t head, uint32_t block) {
+                uint64_t* full = &bar.full[blk % kFullBars];
+                if (!begin(NV)) return;
 #pragma unroll
-                for (uint32_t i = 0; i < NV; ++i) {   // a slot: 64 keys of 128 values, or 128 keys of 64
-                    uint32_t st;
-                    if (!slot_for(st)) return;
+                for (uint32_t i = 0; i < NV; ++i, ++pos)   // an atom: 64 keys of 128 values, or 128 keys of 64
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e)
-                        tc::tma_load_3d(ring + st * kAtom + e * (kAtom / 2), &map_v, &bar.full[st], NV == 2 ? e * 128 : 0, head,
+                        tc::tma_load_3d(ring + pos % slots * kAtom + e * (kAtom / 2), &map_v, full, NV == 2 ? e * 128 : 0, head,
                                         block * kTile + (NV == 2 ? i : e) * 64);
-                }
             };
             for (uint64_t x = lo; x < hi && ok;) {
                 const Segment s = segment_at(p, x, hi);
@@ -251,48 +253,54 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 x += s.n;
             }
             volatile int never = 0;   // these waits must not be cut short by the abort flag
-            for (uint32_t i = 0; i < slots && i < pos; ++i) {
-                const uint32_t j = pos - 1 - i;
-                tc::mbar_wait(&bar.full[j % slots], (j / slots) & 1u, &never, 200000000ull);
+            for (uint32_t i = 0; i < slots && i < blk; ++i) {
+                const uint32_t j = blk - 1 - i;
+                tc::mbar_wait(&bar.full[j % kFullBars], (j / kFullBars) & 1u, &never, 200000000ull);
             }
         } else if (warp == 9) {
             // ---------------- MMA issue, by one lane of the whole warp ----------------
             constexpr uint32_t id_s = tc::idesc_f16(kTile, BF16, false), id_o = tc::idesc_f16(value, BF16, true);
             const uint64_t q0 = tc::desc_sw128(q_smem), k0 = tc::desc_sw128(ring), v0 = tc::desc_sw128_n(ring, kAtom / 2);
-            uint32_t pos = 0, seg = 0, p_phase = 0;   // ring position; segments; bit t: phase of p_ready[t]
-            bool ok = true, issued = false;
-            // scores of half t from the key atoms at ring position `at`
-            auto scores = [&](uint32_t t, uint32_t at, bool release) {
-                const uint32_t d = tmem + 256 + t * 128;
-#pragma unroll
-                for (uint32_t i = 0; i < NK; ++i) {
-                    const uint32_t st = (at + i) % slots;
-                    ok = ok && tc::mbar_wait_warp(&bar.full[st], ((at + i) / slots) & 1u, abort);
-                    if (!ok) return;
-                    tc::fence_after_sync();
-                    const uint64_t qd = q0 + (t * NK + i) * (kAtom >> 4), kd = k0 + st * (kAtom >> 4);
-                    if (tc::elect_one()) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) tc::mma_bf16(d, qd + 2 * j, kd + 2 * j, id_s, i || j);
-                        if (release) tc::commit(&bar.empty[st]);
-                        if (i == NK - 1) tc::commit(&bar.s_full[t]);
-                    }
-                    __syncwarp();
-                    issued = true;
-                }
+            uint32_t pos = 0, blk = 0, seg = 0, p_phase = 0;   // atoms, blocks, segments; bit t: phase of p_ready[t]
+            uint32_t ka = 0, va = 0;                           // where the key and value blocks in use start
+            auto next_k = [&]() {
+                tc::mbar_pass(&bar.full[blk % kFullBars], blk / kFullBars & 1u, abort);
+                ++blk;
+                ka = pos;
+                pos += NK;
             };
-            // output of half t: its probabilities times the value atoms at
-            // `at`, 64 keys at a time (the softmax hands them over so)
-            auto values = [&](uint32_t t, uint32_t at, bool accumulate, bool release, bool last) {
+            auto next_v = [&]() {
+                tc::mbar_pass(&bar.full[blk % kFullBars], blk / kFullBars & 1u, abort);
+                ++blk;
+                va = pos;
+                pos += NV;
+            };
+            // scores of half t from the key block at ka
+            auto scores = [&](uint32_t t, bool release) {
+                tc::fence_after_sync();
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (uint32_t i = 0; i < NK; ++i) {
+                        const uint32_t st = (ka + i) % slots;
+                        const uint64_t qd = q0 + (t * NK + i) * (kAtom >> 4), kd = k0 + st * (kAtom >> 4);
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) tc::mma_bf16(tmem + 256 + t * 128, qd + 2 * j, kd + 2 * j, id_s, i || j);
+                        if (release) tc::commit(&bar.empty[st]);
+                    }
+                    tc::commit(&bar.s_full[t]);
+                }
+                __syncwarp();
+            };
+            // output of half t: its probabilities times the value block at
+            // va, 64 keys at a time (the softmax hands them over so)
+            auto values = [&](uint32_t t, bool accumulate, bool release, bool last) {
                 const uint32_t d = tmem + t * 128, pr = tmem + 256 + t * 128;
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i) {
-                    const uint32_t st = (at + (NV == 2 ? i : 0)) % slots;
-                    ok = ok && tc::mbar_wait_warp(&bar.p_ready[t][i], p_phase >> t & 1u, abort);
-                    if (NV == 2 || !i) ok = ok && tc::mbar_wait_warp(&bar.full[st], ((at + (NV == 2 ? i : 0)) / slots) & 1u, abort);
-                    if (!ok) return;
-                    tc::fence_after_sync();
+                    const uint32_t st = (va + (NV == 2 ? i : 0)) % slots;
                     const uint64_t vd = v0 + st * (kAtom >> 4) + (NV == 2 ? 0 : i * (kAtom >> 5));
+                    tc::mbar_pass(&bar.p_ready[t][i], p_phase >> t & 1u, abort);
+                    tc::fence_after_sync();
                     if (tc::elect_one()) {
 #pragma unroll
                         for (uint32_t j = 0; j < 4; ++j)   // 16 keys: 8 columns of p, 2 KB of values
@@ -304,55 +312,40 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 }
                 p_phase ^= 1u << t;
             };
-            for (uint64_t x = lo; x < hi && ok; ++seg) {
+            for (uint64_t x = lo; x < hi; ++seg) {
                 const Segment s = segment_at(p, x, hi);
                 const uint32_t n1 = s.active(1, p.blocks);
-                for (uint32_t t = 0; t < 2; ++t) ok = ok && tc::mbar_wait_warp(&bar.q_ready[t], seg & 1u, abort);
-                tc::fence_after_sync();
-                uint32_t ka = pos;
-                pos += NK;
-                scores(0, ka, s.keys);
+                for (uint32_t t = 0; t < 2; ++t) tc::mbar_pass(&bar.q_ready[t], seg & 1u, abort);
+                next_k();
+                scores(0, s.keys);
                 if (n1) {
-                    if (s.keys) {
-                        ka = pos;
-                        pos += NK;
-                    }
-                    scores(1, ka, true);
+                    if (s.keys) next_k();
+                    scores(1, true);
                 }
-                for (uint32_t i = 0; i < s.n && ok; ++i) {
-                    uint32_t va = pos;
-                    pos += NV;
-                    values(0, va, i > 0, s.keys, i + 1 == s.n);
+                for (uint32_t i = 0; i < s.n; ++i) {
+                    next_v();
+                    values(0, i > 0, s.keys, i + 1 == s.n);
                     if (i + 1 < s.n) {
-                        ka = pos;
-                        pos += NK;
-                        scores(0, ka, s.keys);
+                        next_k();
+                        scores(0, s.keys);
                     }
                     if (i >= n1) continue;
-                    if (s.keys) {
-                        va = pos;
-                        pos += NV;
-                    }
-                    values(1, va, i > 0, true, i + 1 == n1);
+                    if (s.keys) next_v();
+                    values(1, i > 0, true, i + 1 == n1);
                     if (i + 1 < n1) {
-                        if (s.keys) {
-                            ka = pos;
-                            pos += NK;
-                        }
-                        scores(1, ka, true);
+                        if (s.keys) next_k();
+                        scores(1, true);
                     }
                 }
-                if (!n1 && ok && tc::elect_one()) tc::commit(&bar.o_done[1]);   // keeps the halves' phases in step
+                if (!n1 && tc::elect_one()) tc::commit(&bar.o_done[1]);   // keeps the halves' phases in step
                 __syncwarp();
                 x += s.n;
             }
-            if (issued) {   // all issued MMAs finish before TMEM is freed
-                volatile int never = 0;
-                if (tc::elect_one()) tc::commit(&bar.teardown);
-                __syncwarp();
-                tc::mbar_wait(&bar.teardown, 0, &never, 200000000ull);
-                __syncwarp();
-            }
+            volatile int never = 0;   // all issued MMAs finish before TMEM is freed
+            if (tc::elect_one()) tc::commit(&bar.teardown);
+            __syncwarp();
+            tc::mbar_wait(&bar.teardown, 0, &never, 200000000ull);
+            __syncwarp();
         }
     } else {
         // ---------------- softmax ----------------
@@ -363,13 +356,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
         const float c = fabsf(a.scale) * kLog2e;
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale: -q
         uint32_t s_uses = 0, seg = 0;
-        bool ok = true;
         auto wait = [&](uint64_t* b, uint32_t parity) {
-            ok = tc::mbar_wait_warp(b, parity, abort);
+            tc::mbar_pass(b, parity, abort);
+            __syncwarp();
             tc::fence_after_sync();
-            return ok;
         };
-        for (uint64_t x = lo; x < hi && ok; ++seg) {
+        auto arrive = [&](uint64_t* b) {   // one for the warp: arrivals on a barrier are taken one by one
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(b);
+        };
+        for (uint64_t x = lo; x < hi; ++seg) {
             const Segment s = segment_at(p, x, hi);
             const uint32_t tile = 2 * s.job.pair + (s.keys ? 0 : t), n = s.active(t, p.blocks);
             // the tile's query rows, swizzled as the MMA reads them: eight
@@ -402,11 +399,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            tc::fence_before_sync();
-            tc::mbar_arrive(&bar.q_ready[t]);
+            arrive(&bar.q_ready[t]);
             float m = -INFINITY, l = 0.0f;
             for (uint32_t i = 0; i < n; ++i) {
-                if (!wait(&bar.s_full[t], s_uses++ & 1u)) break;
+                wait(&bar.s_full[t], s_uses++ & 1u);
                 uint32_t v[128];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) tc::tmem_ld32(scores_at + 32 * j, v + 32 * j);
@@ -462,19 +458,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                     tc::tmem_st16(scores_at + 16 * q4, w);
                     if (q4 % 2) {   // 64 keys for the product
                         tc::tmem_wait_st();
-                        tc::fence_before_sync();
-                        tc::mbar_arrive(&bar.p_ready[t][q4 / 2]);
+                        arrive(&bar.p_ready[t][q4 / 2]);
                     }
                 }
                 float s0, s1;
                 split_pair(add2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
             }
-            if (!ok) break;
             // the segment's part
             const size_t part = (static_cast<size_t>(blockIdx.x) * p.max_seg + seg) * 2 + t;
             parts.ml[part * kTile + row] = make_float2(m, l);
-            if (!wait(&bar.o_done[t], seg & 1u)) break;
+            wait(&bar.o_done[t], seg & 1u);
             if (n) {
                 float* dst = parts.o + (part * kTile + row) * value;
 #pragma unroll

@@ -88,9 +88,21 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 
-// mbar_wait for a whole warp; the same answer in every lane.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+// mbar_wait on a critical path, without an answer: after the limit it sets
+// *abort and returns like any later wait, so that control flow stays the
+// same in every lane (a vote per wait cost 100 cycles on an MMA issue
+// path). The clock and the flag are looked at once in 64 polls.
+__device__ __forceinline__ void mbar_pass(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                          uint64_t limit_ns = 2000000000ull) {
+    if (mbar_try_wait(bar, parity)) return;
+    uint64_t t0 = 0;
+    for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+        if (i % 64) continue;
+        if (*abort) return;
+        const uint64_t now = globaltimer_ns();
+        if (!t0) t0 = now;
+        if (now - t0 > limit_ns) *abort = 1;
+    }
 }
 
 // ---- TMA / bulk copies (no multicast) -------------------------------------------
