@@ -8,6 +8,7 @@
 // sums here are float sums in an order of their own, so results agree with
 // k3xb_kda_tree to float tolerance, not bit for bit.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <atomic>
 
@@ -169,6 +170,455 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
                 make_float4(S[i][g][0], S[i][g][1], S[i][g][2], S[i][g][3]);
 }
 
+// ---- chunks of 16 tokens ------------------------------------------------------
+//
+// Within a chunk, with p_i the decay from the chunk's start to token i, e_j
+// the decay from token j to its end and D_ij the decay from j to i:
+//
+//   A_ij = k_i . (D_ij k_j)  (j < i),   P_ij = q_i . (D_ij k_j)  (j <= i)
+//   T = (1 + diag(b) A)^-1 diag(b)
+//   U = T (V - (p K) S0^T),   O = (p Q) S0^T + P U
+//   S = S0 diag(p_15) + U^T (e K)
+//
+// which is the rule's own sums in another order. Decays are products of the
+// tokens' own, never quotients, so any decay from 0 to 1 is as exact as in
+// the token form.
+//
+// Producer warps (one thread per key channel) make a chunk's operands: A and P
+// on the CUDA cores (120 pairs; a factored form would divide by decays), T by
+// substitution. Consumer warps own 16 value rows each and keep S in
+// registers, in the accumulator layout of mma.m16n8k16, which is also the
+// layout its left operand is read in: S, R = V - .. and U go from accumulators
+// straight into the next product, without shared memory.
+//
+// Every operand is carried as two f16 terms of a power-of-two multiple (hi +
+// lo, 22 bits of the largest element of its tile or row), and a product as hi
+// hi + hi lo + lo hi in f32 accumulators, the small products summed apart
+// (a tensor core truncates each sum): float accuracy at three times the MMA
+// work, where plain f16 or bf16 operands would leave the f32 state with 3
+// digits and TF32 in two terms would take twice the MMAs.
+
+constexpr int kChunk = 16, kStages = 3;
+
+template <int D>
+struct __align__(16) ChunkStage {
+    // [tok][channel] rows of D + 8 values: ldmatrix reads 8 of them without a
+    // bank conflict; 16 + 8 likewise
+    __half k[2][kChunk][D + 8], q[2][kChunk][D + 8], ke[2][kChunk][D + 8];   // p K, p Q, e K: hi, lo
+    __half t[2][kChunk][kChunk + 8], p[2][kChunk][kChunk + 8];
+    float total[D];     // p_15
+    int exps[5];        // the powers of two of k, q, ke, t, p
+};
+
+template <int D>
+struct __align__(16) ChunkScratch {
+    float a[kChunk][D], k[kChunk][D], q[kChunk][D];
+    float red[D / 32][32][36];        // a warp's pair sums by lane
+    float A[kChunk][kChunk], P[kChunk][kChunk];
+    float beta[kChunk];
+    float top[3][D / 32];
+};
+
+template <int D>
+constexpr size_t chunk_smem() { return kStages * sizeof(ChunkStage<D>) + sizeof(ChunkScratch<D>); }
+
+__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void named_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+// The power of two that takes a maximum to [2^14, 2^15) (f16 ends at 2^16);
+// zero, infinity and NaN keep theirs.
+__device__ __forceinline__ int scale_exp(float top) {
+    const int e = static_cast<int>(__float_as_uint(top) >> 23);
+    return top == 0.0f || e == 255 ? 0 : min(126, 14 + 127 - e);
+}
+
+__device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
+    hi = __float2half_rn(x);
+    lo = __float2half_rn(x - __half2float(hi));
+}
+// Two neighbours as packed hi and lo.
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 b = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - b.x, y - b.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* row) {
+    const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(row));
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+
+// The sum over a warp's lanes of 32 values per lane, value l to lane l.
+__device__ __forceinline__ float sum_rows(float (*red)[36], uint32_t lane) {
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(&red[lane][4 * i]);
+        s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+template <int D, typename E>
+__device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uint32_t t0, uint32_t t1, ChunkStage<D>* stages,
+                                               ChunkScratch<D>& sc, int threads) {
+    constexpr int NP = D / 32, CH = D / 32;   // producer warps; channels per lane in the pair sums
+    const uint32_t c = threadIdx.x, lane = c % 32, warp = c / 32, P = a.heads * D;
+    const E* q = static_cast<const E*>(a.q) + h * D + c;
+    const E* k = static_cast<const E*>(a.k) + h * D + c;
+    const float* ld = a.log_decay + h * D + c;
+    // this thread's channel of the next chunk's tokens; past the end k = q =
+    // beta = 0 and a decay of 1 leave everything as it is
+    float kk[kChunk], qq[kChunk], ll[kChunk], bb = 0.0f;
+    auto fetch = [&](uint32_t first) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            const bool in = first + i < t1;
+            const size_t t = first + i;
+            kk[i] = in ? to_f(k[t * a.row_stride]) : 0.0f;
+            qq[i] = in ? to_f(q[t * a.row_stride]) : 0.0f;
+            ll[i] = in ? ld[t * P] : 0.0f;
+        }
+        if (c < kChunk) bb = first + c < t1 ? a.beta[static_cast<size_t>(first + c) * a.heads + h] : 0.0f;
+    };
+    fetch(t0);
+    uint32_t n = 0;
+    for (uint32_t first = t0; first < t1; first += kChunk, ++n) {
+        ChunkStage<D>& st = stages[n % kStages];
+        float kp[kChunk], qp[kChunk], ke[kChunk];
+        {
+            float run = 1.0f;
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                ll[i] = expf(ll[i]);
+                sc.a[i][c] = ll[i];
+                sc.k[i][c] = kk[i];
+                sc.q[i][c] = qq[i];
+                run *= ll[i];
+                kp[i] = kk[i] * run;
+                qp[i] = qq[i] * run;
+            }
+            const float total = run;
+            run = 1.0f;
+#pragma unroll
+            for (int i = kChunk - 1; i >= 0; --i) {
+                ke[i] = kk[i] * run;
+                run *= ll[i];
+            }
+            if (c < kChunk) sc.beta[c] = bb;
+            float top[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                top[0] = fmaxf(top[0], fabsf(kp[i]));
+                top[1] = fmaxf(top[1], fabsf(qp[i]));
+                top[2] = fmaxf(top[2], fabsf(ke[i]));
+            }
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                top[e] = warp_max(top[e]);
+                if (lane == 0) sc.top[e][warp] = top[e];
+            }
+            if (n >= kStages) named_sync(2 + kStages + n % kStages, threads);   // the stage is read
+            st.total[c] = total;
+        }
+        named_sync(1, D);
+        if (first + kChunk < t1) fetch(first + kChunk);
+        {
+            int ex[3];
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                float top = sc.top[e][0];
+#pragma unroll
+                for (int w = 1; w < NP; ++w) top = fmaxf(top, sc.top[e][w]);
+                ex[e] = scale_exp(top);
+                if (c == 0) st.exps[e] = ex[e];
+            }
+            const float sk = exp2i(ex[0]), sq = exp2i(ex[1]), se = exp2i(ex[2]);
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                split_half(kp[i] * sk, st.k[0][i][c], st.k[1][i][c]);
+                split_half(qp[i] * sq, st.q[0][i][c], st.q[1][i][c]);
+                split_half(ke[i] * se, st.ke[0][i][c], st.ke[1][i][c]);
+            }
+        }
+        // pairs: the columns j of this warp, in twos of equal work
+        auto load = [&](const float* row, float (&x)[CH]) {
+            if constexpr (CH == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(row + lane * 4);
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else if constexpr (CH == 2) {
+                const float2 v = *reinterpret_cast<const float2*>(row + lane * 2);
+                x[0] = v.x; x[1] = v.y;
+            } else {
+                x[0] = row[lane];
+            }
+        };
+        float (*red)[36] = sc.red[warp];
+        for (int g = 0; g < kChunk / NP; ++g) {
+            const int j = g / 2 * 2 * NP + (g % 2 ? 2 * NP - 1 - static_cast<int>(warp) : static_cast<int>(warp));
+            float e[CH], x[CH], y[CH], z[CH];
+            load(sc.k[j], e);
+            load(sc.q[j], y);
+            float sp = 0.0f, sa;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) sp = fmaf(y[i], e[i], sp);
+            red[16 + j][lane] = sp;
+#pragma unroll 3
+            for (int i = j + 1; i < kChunk; ++i) {
+                load(sc.a[i], x);
+                load(sc.q[i], y);
+                load(sc.k[i], z);
+                sp = sa = 0.0f;
+#pragma unroll
+                for (int m = 0; m < CH; ++m) {
+                    e[m] *= x[m];
+                    sa = fmaf(z[m], e[m], sa);
+                    sp = fmaf(y[m], e[m], sp);
+                }
+                red[i][lane] = sa;
+                red[16 + i][lane] = sp;
+            }
+            __syncwarp();
+            const float s = sum_rows(red, lane);
+            const int i = lane % 16;
+            if (lane < 16) sc.A[i][j] = i > j ? s : 0.0f;
+            else sc.P[i][j] = i >= j ? s : 0.0f;
+            __syncwarp();
+        }
+        named_sync(1, D);
+        if (warp == 0) {   // T, a lane per column
+            const uint32_t j = lane % 16;
+            float x[kChunk], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                float s = 0.0f;
+#pragma unroll
+                for (int m = 0; m < i; ++m) s = fmaf(sc.A[i][m], x[m], s);
+                x[i] = (i == static_cast<int>(j) ? 1.0f : 0.0f) - sc.beta[i] * s;
+            }
+            const float b = sc.beta[j];
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                x[i] *= b;
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            const int ex = scale_exp(warp_max(top));
+            if (lane == 0) st.exps[3] = ex;
+            const float f = exp2i(ex);
+            if (lane < 16)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) split_half(x[i] * f, st.t[0][i][j], st.t[1][i][j]);
+        }
+        if (warp == NP - 1) {
+            float x[8], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = sc.P[2 * i + lane / 16][lane % 16];
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            const int ex = scale_exp(warp_max(top));
+            if (lane == 0) st.exps[4] = ex;
+            const float f = exp2i(ex);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) split_half(x[i] * f, st.p[0][2 * i + lane / 16][lane % 16], st.p[1][2 * i + lane / 16][lane % 16]);
+        }
+        named_arrive(2 + n % kStages, threads);
+    }
+}
+
+// Row maxima of two rows over a quad's lanes as scale exponents.
+__device__ __forceinline__ void row_exps(float m0, float m1, int (&ex)[2]) {
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+    }
+    ex[0] = scale_exp(m0);
+    ex[1] = scale_exp(m1);
+}
+
+// [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
+__device__ __forceinline__ void split_rows(const float (&x)[2][4], const float (&f)[2], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    split_pair(x[0][0] * f[0], x[0][1] * f[0], hi[0], lo[0]);
+    split_pair(x[0][2] * f[1], x[0][3] * f[1], hi[1], lo[1]);
+    split_pair(x[1][0] * f[0], x[1][1] * f[0], hi[2], lo[2]);
+    split_pair(x[1][2] * f[1], x[1][3] * f[1], hi[3], lo[3]);
+}
+
+// big += x hi * y hi, small += the cross products, for two n-tiles.
+__device__ __forceinline__ void mma_terms(float (&big)[2][4], float (&small)[2][4], const uint32_t (&xh)[4], const uint32_t (&xl)[4],
+                                          const uint32_t (&yh)[4], const uint32_t (&yl)[4]) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(big[n], xh, yh[2 * n], yh[2 * n + 1]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(small[n], xl, yh[2 * n], yh[2 * n + 1]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(small[n], xh, yl[2 * n], yl[2 * n + 1]);
+}
+
+template <int D, typename E>
+__device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uint32_t h, uint32_t row0, uint32_t t0, uint32_t t1,
+                                               const ChunkStage<D>* stages, int threads) {
+    const uint32_t lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, P = a.heads * D;
+    const size_t state_at = (static_cast<size_t>(s) * a.heads + h) * D * D + static_cast<size_t>(row0 + g) * D + 2 * t;
+    const E* v = static_cast<const E*>(a.v) + h * D + row0 + g;
+    float S[D / 8][4];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+        float2 x = make_float2(0.0f, 0.0f), y = x;
+        if (a.state) {
+            x = *reinterpret_cast<const float2*>(a.state + state_at + 8 * j);
+            y = *reinterpret_cast<const float2*>(a.state + state_at + 8 * D + 8 * j);
+        }
+        S[j][0] = x.x; S[j][1] = x.y; S[j][2] = y.x; S[j][3] = y.y;
+    }
+    // v of tokens 2t, 2t+1, 2t+8, 2t+9 and rows g, g + 8, in accumulator order
+    float vv[2][4];
+    auto fetch = [&](uint32_t first) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const size_t tok = first + 8 * n + 2 * t + e % 2;
+                vv[n][e] = tok < t1 ? to_f(v[tok * a.row_stride + 8 * (e / 2)]) : 0.0f;
+            }
+    };
+    fetch(t0);
+    // ldmatrix rows: n-major operands (lanes 0-7: tile 0, k 0-7; 8-15: k 8-15; 16-31: tile 1)
+    const uint32_t mrow = lane % 8 + lane / 16 * 8, mcol = lane / 8 % 2 * 8;
+    // k-major ones, transposed (lanes 0-7: tile 0, k 0-7; 8-15: k 8-15; 16-31: tile 1)
+    const uint32_t krow = lane % 16, kcol = lane / 16 * 8;
+    uint32_t n = 0;
+    for (uint32_t first = t0; first < t1; first += kChunk, ++n) {
+        const ChunkStage<D>& st = stages[n % kStages];
+        int ex[2];
+        {
+            float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+                m0 = fmaxf(m0, fmaxf(fabsf(S[j][0]), fabsf(S[j][1])));
+                m1 = fmaxf(m1, fmaxf(fabsf(S[j][2]), fabsf(S[j][3])));
+            }
+            row_exps(m0, m1, ex);
+        }
+        const float up[2] = {exp2i(ex[0]), exp2i(ex[1])}, down[2] = {exp2i(-ex[0]), exp2i(-ex[1])};
+        named_sync(2 + n % kStages, threads);
+        float kb[2][4] = {}, ks[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+            uint32_t xh[4], xl[4], yh[4], yl[4];
+            const float x[2][4] = {{S[2 * j][0], S[2 * j][1], S[2 * j][2], S[2 * j][3]},
+                                   {S[2 * j + 1][0], S[2 * j + 1][1], S[2 * j + 1][2], S[2 * j + 1][3]}};
+            split_rows(x, up, xh, xl);
+            ldmatrix4<false>(yh, &st.k[0][mrow][16 * j + mcol]);
+            ldmatrix4<false>(yl, &st.k[1][mrow][16 * j + mcol]);
+            mma_terms(kb, ks, xh, xl, yh, yl);
+            ldmatrix4<false>(yh, &st.q[0][mrow][16 * j + mcol]);
+            ldmatrix4<false>(yl, &st.q[1][mrow][16 * j + mcol]);
+            mma_terms(ob, os, xh, xl, yh, yl);
+        }
+        uint32_t xh[4], xl[4], yh[4], yl[4];
+        float r[2][4], ub[2][4] = {}, us[2][4] = {};
+        int rx[2], ux[2];
+        {
+            const float f = exp2i(-st.exps[0]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[i][e] = fmaf((kb[i][e] + ks[i][e]) * f, -down[e / 2], vv[i][e]);
+            row_exps(fmaxf(fmaxf(fabsf(r[0][0]), fabsf(r[0][1])), fmaxf(fabsf(r[1][0]), fabsf(r[1][1]))),
+                     fmaxf(fmaxf(fabsf(r[0][2]), fabsf(r[0][3])), fmaxf(fabsf(r[1][2]), fabsf(r[1][3]))), rx);
+            if (first + kChunk < t1) fetch(first + kChunk);
+            const float fr[2] = {exp2i(rx[0]), exp2i(rx[1])};
+            split_rows(r, fr, xh, xl);
+            ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
+            ldmatrix4<false>(yl, &st.t[1][mrow][mcol]);
+            mma_terms(ub, us, xh, xl, yh, yl);
+        }
+        float u[2][4];
+        {
+            const float f = exp2i(-st.exps[3]), fd[2] = {exp2i(-rx[0]), exp2i(-rx[1])};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[i][e] = (ub[i][e] + us[i][e]) * f * fd[e / 2];
+            row_exps(fmaxf(fmaxf(fabsf(u[0][0]), fabsf(u[0][1])), fmaxf(fabsf(u[1][0]), fabsf(u[1][1]))),
+                     fmaxf(fmaxf(fabsf(u[0][2]), fabsf(u[0][3])), fmaxf(fabsf(u[1][2]), fabsf(u[1][3]))), ux);
+            const float fu[2] = {exp2i(ux[0]), exp2i(ux[1])};
+            split_rows(u, fu, xh, xl);
+        }
+        const float ud[2] = {exp2i(-ux[0]), exp2i(-ux[1])};
+        {   // S = S diag(total) + U^T (e K)
+            const float f = exp2i(-st.exps[2]);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                float b[2][4] = {}, x[2][4] = {};
+                uint32_t wh[4], wl[4];
+                ldmatrix4<true>(wh, &st.ke[0][krow][16 * j + kcol]);
+                ldmatrix4<true>(wl, &st.ke[1][krow][16 * j + kcol]);
+                mma_terms(b, x, xh, xl, wh, wl);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 tot = *reinterpret_cast<const float2*>(&st.total[16 * j + 8 * i + 2 * t]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        S[2 * j + i][e] = fmaf((b[i][e] + x[i][e]) * f, ud[e / 2], S[2 * j + i][e] * (e % 2 ? tot.y : tot.x));
+                }
+            }
+        }
+        {   // O = (p Q) S0^T + P U
+            float pb[2][4] = {}, px[2][4] = {};
+            ldmatrix4<false>(yh, &st.p[0][mrow][mcol]);
+            ldmatrix4<false>(yl, &st.p[1][mrow][mcol]);
+            mma_terms(pb, px, xh, xl, yh, yl);
+            const float fq = exp2i(-st.exps[1]), fp = exp2i(-st.exps[4]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t tok = first + 8 * i + 2 * t + e % 2;
+                    const float o = fmaf((ob[i][e] + os[i][e]) * fq, down[e / 2], (pb[i][e] + px[i][e]) * fp * ud[e / 2]);
+                    if (tok < t1) store1<E>(a.out, static_cast<size_t>(tok) * P + h * D + row0 + g + 8 * (e / 2), o);
+                }
+        }
+        if (first + kStages * kChunk < t1) named_arrive(2 + kStages + n % kStages, threads);
+    }
+    if (!a.state_out) return;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+        *reinterpret_cast<float2*>(a.state_out + state_at + 8 * j) = make_float2(S[j][0], S[j][1]);
+        *reinterpret_cast<float2*>(a.state_out + state_at + 8 * D + 8 * j) = make_float2(S[j][2], S[j][3]);
+    }
+}
+
+// A CTA: D / 32 producer warps and NW consumer warps (16 NW value rows of a
+// head). Named barriers: 1 among the producers, 2.. a stage is full, 5.. read.
+template <int D, int NW, typename E>
+__global__ void __launch_bounds__(D + 32 * NW) kda_chunk_kernel(const SeqArgs a) {
+    extern __shared__ __align__(16) unsigned char chunk_mem[];
+    ChunkStage<D>* stages = reinterpret_cast<ChunkStage<D>*>(chunk_mem);
+    ChunkScratch<D>& scratch = *reinterpret_cast<ChunkScratch<D>*>(chunk_mem + kStages * sizeof(ChunkStage<D>));
+    constexpr uint32_t slices = D / (16 * NW);
+    const uint32_t s = blockIdx.y, h = blockIdx.x / slices, r0 = blockIdx.x % slices * (16 * NW);
+    uint32_t t0, t1;
+    if (!token_range(a, s, t0, t1)) return;
+    if (threadIdx.x < D) chunk_producer<D, E>(a, h, t0, t1, stages, scratch, D + 32 * NW);
+    else chunk_consumer<D, E>(a, s, h, r0 + (threadIdx.x - D) / 32 * 16, t0, t1, stages, D + 32 * NW);
+}
+
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 template <int D, typename E>
@@ -181,6 +631,30 @@ int launch_recurrent(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     else kda_recurrent_kernel<D, E, false><<<grid, kSeqThreads, 0, ctx->stream>>>(a);
     K3XB_LAUNCHED(ctx);
     return K3XB_OK;
+}
+
+template <int D, int NW, typename E>
+int launch_chunk(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
+    static std::atomic<uint64_t> configured{0};   // per template instance
+    const int cst = configure_once(ctx, configured, [&]() -> int {
+        K3XB_CUDA(ctx, cudaFuncSetAttribute(kda_chunk_kernel<D, NW, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            static_cast<int>(chunk_smem<D>())));
+        return K3XB_OK;
+    });
+    if (cst) return cst;
+    const dim3 grid(a.heads * (D / (16 * NW)), sequences);
+    kda_chunk_kernel<D, NW, E><<<grid, D + 32 * NW, chunk_smem<D>(), ctx->stream>>>(a);
+    K3XB_LAUNCHED(ctx);
+    return K3XB_OK;
+}
+
+template <typename E>
+int launch_prefill(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences, uint32_t d) {
+    switch (d) {
+        case 32: return launch_chunk<32, 2, E>(ctx, a, sequences);
+        case 64: return launch_chunk<64, 4, E>(ctx, a, sequences);
+        default: return launch_chunk<128, 4, E>(ctx, a, sequences);
+    }
 }
 
 template <typename E>
@@ -230,8 +704,8 @@ int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
     if (const int st = check_seq(ctx, "kda_prefill", type, sequences, heads, head_dim, a)) return st;
     PhaseScope ph(ctx, K3XB_PHASE_KDA_RECURRENCE);
     ++ctx->stats.kda_calls;
-    return type == K3XB_TYPE_F32 ? launch_seq<float>(ctx, a, sequences, head_dim)
-                                 : launch_seq<__nv_bfloat16>(ctx, a, sequences, head_dim);
+    return type == K3XB_TYPE_F32 ? launch_prefill<float>(ctx, a, sequences, head_dim)
+                                 : launch_prefill<__nv_bfloat16>(ctx, a, sequences, head_dim);
 }
 
 int k3xb_kda_step(k3xb_ctx* ctx, const void* q, const void* k, const void* v, uint64_t row_stride, int32_t type,
