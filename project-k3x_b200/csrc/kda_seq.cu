@@ -176,20 +176,21 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // the decay from token j to its end and D_ij the decay from j to i:
 //
 //   A_ij = k_i . (D_ij k_j)  (j < i),   P_ij = q_i . (D_ij k_j)  (j <= i)
-//   T = (1 + diag(b) A)^-1 diag(b)
-//   U = T (V - (p K) S0^T),   O = (p Q) S0^T + P U
+//   T = (1 + diag(b) A)^-1 diag(b),   W = T (p K)
+//   U = T V - W S0^T,   O = (p Q) S0^T + P U
 //   S = S0 diag(p_15) + U^T (e K)
 //
 // which is the rule's own sums in another order. Decays are products of the
-// tokens' own, never quotients, so any decay from 0 to 1 is as exact as in
-// the token form.
+// tokens' own, never quotients, so any decay from 0 on is as exact as in the
+// token form: for a pair (i, j) D_ij is split where the halves of the
+// smallest aligned block that holds both meet, D_ij = (decay from there to i)
+// (decay from j to there). Four block sizes (16, 8, 4, 2) make four products
+// of 8 upper by 8 lower rows, of which a token is in one side each.
 //
-// Producer warps (one thread per key channel) make a chunk's operands: A and P
-// on the CUDA cores (120 pairs; a factored form would divide by decays), T by
-// substitution. Consumer warps own 16 value rows each and keep S in
-// registers, in the accumulator layout of mma.m16n8k16, which is also the
-// layout its left operand is read in: S, R = V - .. and U go from accumulators
-// straight into the next product, without shared memory.
+// Producer warps make a chunk's operands; consumer warps own 16 value rows
+// each and keep S in registers, in the accumulator layout of mma.m16n8k16,
+// which is also the layout its left operand is read in: S, V and U go from
+// accumulators straight into the next product, without shared memory.
 //
 // Every operand is carried as two f16 terms of a power-of-two multiple (hi +
 // lo, 22 bits of the largest element of its tile or row), and a product as hi
@@ -202,21 +203,24 @@ constexpr int kChunk = 16, kStages = 3;
 
 template <int D>
 struct __align__(16) ChunkStage {
-    // [tok][channel] rows of D + 8 values: ldmatrix reads 8 of them without a
-    // bank conflict; 16 + 8 likewise
-    __half k[2][kChunk][D + 8], q[2][kChunk][D + 8], ke[2][kChunk][D + 8];   // p K, p Q, e K: hi, lo
+    // hi, lo; [tok][channel] rows of D + 8 values: ldmatrix reads 8 of them
+    // without a bank conflict; 16 + 8 likewise
+    __half w[2][kChunk][D + 8], q[2][kChunk][D + 8], ke[2][kChunk][D + 8];   // W, p Q, e K
     __half t[2][kChunk][kChunk + 8], p[2][kChunk][kChunk + 8];
     float total[D];     // p_15
-    int exps[5];        // the powers of two of k, q, ke, t, p
+    int exps[8];        // the powers of two of w, q, ke, t, p
 };
 
 template <int D>
 struct __align__(16) ChunkScratch {
-    float a[kChunk][D], k[kChunk][D], q[kChunk][D];
-    float red[D / 32][32][36];        // a warp's pair sums by lane
-    float A[kChunk][kChunk], P[kChunk][kChunk];
+    __half k[2][kChunk][D + 8];           // p K
+    // per block size: 8 upper rows of k, 8 of q, 8 lower rows of k
+    __half level[4][2][24][D + 8];
+    float At[kChunk][kChunk];             // At[j][i] = A_ij
+    float P[kChunk][kChunk];
+    float diag[D / 32][kChunk];           // q_i . k_i by producer warp
     float beta[kChunk];
-    float top[3][D / 32];
+    uint32_t top[6][D / 32];
 };
 
 template <int D>
@@ -231,6 +235,8 @@ __device__ __forceinline__ int scale_exp(float top) {
     const int e = static_cast<int>(__float_as_uint(top) >> 23);
     return top == 0.0f || e == 255 ? 0 : min(126, 14 + 127 - e);
 }
+// 2^e, e clamped to what a float holds normalised
+__device__ __forceinline__ float pow2(int e) { return exp2i(max(-126, min(127, e))); }
 
 __device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
     hi = __float2half_rn(x);
@@ -243,6 +249,13 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
     const __half2 l = __floats2half2_rn(x - b.x, y - b.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+template <int ROWS, int W>
+__device__ __forceinline__ void store_pair(__half (&dst)[2][ROWS][W], int row, int col, float x, float y) {
+    uint32_t hi, lo;
+    split_pair(x, y, hi, lo);
+    *reinterpret_cast<uint32_t*>(&dst[0][row][col]) = hi;
+    *reinterpret_cast<uint32_t*>(&dst[1][row][col]) = lo;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
@@ -261,153 +274,229 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* row) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 
-// The sum over a warp's lanes of 32 values per lane, value l to lane l.
-__device__ __forceinline__ float sum_rows(float (*red)[36], uint32_t lane) {
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+// big += x hi * y hi, small += the cross products, for two n-tiles.
+__device__ __forceinline__ void mma_terms(float (&big)[2][4], float (&small)[2][4], const uint32_t (&xh)[4], const uint32_t (&xl)[4],
+                                          const uint32_t (&yh)[4], const uint32_t (&yl)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(&red[lane][4 * i]);
-        s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
-    }
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    for (int n = 0; n < 2; ++n) mma_f16(big[n], xh, yh[2 * n], yh[2 * n + 1]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(small[n], xl, yh[2 * n], yh[2 * n + 1]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(small[n], xh, yl[2 * n], yl[2 * n + 1]);
 }
 
-template <int D, typename E>
+// Two neighbouring values as floats; VEC: at a multiple of two elements.
+template <typename E, bool VEC>
+__device__ __forceinline__ float2 load2(const E* p) {
+    if constexpr (!VEC) {
+        return make_float2(to_f(p[0]), to_f(p[1]));
+    } else if constexpr (sizeof(E) == 4) {
+        return *reinterpret_cast<const float2*>(p);
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+}
+
+// Largest |x| of 8 tokens' pairs over a warp, as bits (NaN above all).
+__device__ __forceinline__ uint32_t warp_top(const float2 (&x)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
+    return __reduce_max_sync(0xffffffffu, m);
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) { return make_float2(x.x * y.x, x.y * y.y); }
+__device__ __forceinline__ float2 mul1(float2 x, float y) { return make_float2(x.x * y, x.y * y); }
+
+// A producer thread: two neighbouring channels of eight tokens, lanes 0-15
+// the chunk's first half, 16-31 the same channels' second half.
+template <int D, typename E, bool VEC>
 __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uint32_t t0, uint32_t t1, ChunkStage<D>* stages,
                                                ChunkScratch<D>& sc, int threads) {
-    constexpr int NP = D / 32, CH = D / 32;   // producer warps; channels per lane in the pair sums
-    const uint32_t c = threadIdx.x, lane = c % 32, warp = c / 32, P = a.heads * D;
+    constexpr int NP = D / 32;   // producer warps
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, th = lane / 16, P = a.heads * D;
+    const uint32_t c = warp * 32 + lane % 16 * 2;
     const E* q = static_cast<const E*>(a.q) + h * D + c;
     const E* k = static_cast<const E*>(a.k) + h * D + c;
     const float* ld = a.log_decay + h * D + c;
-    // this thread's channel of the next chunk's tokens; past the end k = q =
-    // beta = 0 and a decay of 1 leave everything as it is
-    float kk[kChunk], qq[kChunk], ll[kChunk], bb = 0.0f;
+    // the next chunk's values; past the end k = q = beta = 0 and a decay of 1
+    // leave everything as it is
+    float2 kk[8], qq[8], al[8];
+    float bb = 0.0f;
     auto fetch = [&](uint32_t first) {
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            const bool in = first + i < t1;
-            const size_t t = first + i;
-            kk[i] = in ? to_f(k[t * a.row_stride]) : 0.0f;
-            qq[i] = in ? to_f(q[t * a.row_stride]) : 0.0f;
-            ll[i] = in ? ld[t * P] : 0.0f;
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t tok = first + 8 * th + i;
+            const float2 zero = make_float2(0.0f, 0.0f);
+            const size_t t = tok;
+            kk[i] = tok < t1 ? load2<E, VEC>(k + t * a.row_stride) : zero;
+            qq[i] = tok < t1 ? load2<E, VEC>(q + t * a.row_stride) : zero;
+            al[i] = tok < t1 ? load2<float, VEC>(ld + t * P) : zero;
         }
-        if (c < kChunk) bb = first + c < t1 ? a.beta[static_cast<size_t>(first + c) * a.heads + h] : 0.0f;
+        if (threadIdx.x < kChunk)
+            bb = first + threadIdx.x < t1 ? a.beta[static_cast<size_t>(first + threadIdx.x) * a.heads + h] : 0.0f;
     };
+    const uint32_t arow = lane % 16, acol = lane / 16 * 8;         // ldmatrix: left operands, and k-major ones transposed
     fetch(t0);
     uint32_t n = 0;
     for (uint32_t first = t0; first < t1; first += kChunk, ++n) {
         ChunkStage<D>& st = stages[n % kStages];
-        float kp[kChunk], qp[kChunk], ke[kChunk];
+        // decays within blocks of 8 (f[0]), 8's halves (f[1]), 4's (f[2])
+        // and 2's (f[3]): upper tokens from the middle, lower ones to it
+        float2 f1[8], f2[8], pre[8], suf[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) al[i] = make_float2(expf(al[i].x), expf(al[i].y));
+        const float2 one = make_float2(1.0f, 1.0f);
+#pragma unroll
+        for (int b = 0; b < 8; b += 4) {
+            f2[b] = al[b + 1];
+            f2[b + 1] = one;
+            f2[b + 2] = al[b + 2];
+            f2[b + 3] = mul2(al[b + 2], al[b + 3]);
+        }
+        f1[3] = one;
+        f1[2] = al[3];
+        f1[1] = f2[3];
+        f1[0] = mul2(al[1], f2[3]);
+        f1[4] = al[4];
+        f1[5] = mul2(al[4], al[5]);
+        f1[6] = mul2(f1[5], al[6]);
+        f1[7] = mul2(f1[5], f2[7]);
+        pre[0] = al[0];
+        pre[1] = mul2(al[0], al[1]);
+        pre[2] = mul2(pre[1], al[2]);
+        pre[3] = mul2(pre[1], f2[3]);
+        suf[7] = one;
+        suf[6] = al[7];
+        suf[5] = f2[7];
+        suf[4] = mul2(al[5], f2[7]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            pre[4 + i] = mul2(pre[3], f1[4 + i]);
+            suf[i] = mul2(f1[i], f1[7]);
+        }
+        // the other half's whole decay
+        const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, pre[7].x, 16), __shfl_xor_sync(0xffffffffu, pre[7].y, 16));
+        float2 kp[8], qp[8], ke[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 from = th ? mul2(pre[i], other) : pre[i], to = th ? suf[i] : mul2(suf[i], other);
+            kp[i] = mul2(kk[i], from);
+            qp[i] = mul2(qq[i], from);
+            ke[i] = mul2(kk[i], to);
+        }
         {
-            float run = 1.0f;
+            uint32_t top[6] = {warp_top(kp), warp_top(qp), warp_top(ke), warp_top(kk), warp_top(qq), warp_top(al)};
+            if (lane == 0)
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                ll[i] = expf(ll[i]);
-                sc.a[i][c] = ll[i];
-                sc.k[i][c] = kk[i];
-                sc.q[i][c] = qq[i];
-                run *= ll[i];
-                kp[i] = kk[i] * run;
-                qp[i] = qq[i] * run;
-            }
-            const float total = run;
-            run = 1.0f;
+                for (int e = 0; e < 6; ++e) sc.top[e][warp] = top[e];
+            // q_i . k_i over the warp's channels: each exchange halves the
+            // values that a lane still sums; lane l ends with token l / 2 % 8
+            float d[8];
 #pragma unroll
-            for (int i = kChunk - 1; i >= 0; --i) {
-                ke[i] = kk[i] * run;
-                run *= ll[i];
-            }
-            if (c < kChunk) sc.beta[c] = bb;
-            float top[3] = {0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 8; ++i) d[i] = fmaf(qq[i].x, kk[i].x, qq[i].y * kk[i].y);
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                top[0] = fmaxf(top[0], fabsf(kp[i]));
-                top[1] = fmaxf(top[1], fabsf(qp[i]));
-                top[2] = fmaxf(top[2], fabsf(ke[i]));
+            for (int w = 8; w > 1; w >>= 1)
+#pragma unroll
+                for (int i = 0; i < w / 2; ++i) {
+                    const bool up = lane & w;
+                    const float give = up ? d[i] : d[i + w / 2], keep = up ? d[i + w / 2] : d[i];
+                    d[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+                }
+            d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+            if (lane % 2 == 0) sc.diag[warp][8 * th + lane % 16 / 2] = d[0];
+        }
+        if (threadIdx.x < kChunk) sc.beta[threadIdx.x] = bb;
+        if (n >= kStages) named_sync(2 + kStages + n % kStages, threads);   // the stage is read
+        if (th) *reinterpret_cast<float2*>(&st.total[c]) = mul2(pre[7], other);
+        named_sync(1, D);
+        int ex[6];
+#pragma unroll
+        for (int e = 0; e < 6; ++e) {
+            uint32_t top = sc.top[e][0];
+#pragma unroll
+            for (int w = 1; w < NP; ++w) top = max(top, sc.top[e][w]);
+            ex[e] = e < 5 ? scale_exp(__uint_as_float(top))
+                          // a block's decays pass 1 only where a token's do: by its 8th power at most
+                          : top > 0x3f800000u ? 8 * (static_cast<int>(top >> 23) - 126) : 0;
+        }
+        const int lk = max(-126, ex[3] - ex[5]), lq = max(-126, ex[4] - ex[5]);   // the level operands' powers
+        {
+            const float sk = exp2i(ex[0]), sq = exp2i(ex[1]), se = exp2i(ex[2]), xk = exp2i(lk), xq = exp2i(lq);
+            if (threadIdx.x == 0) {
+                st.exps[1] = ex[1];
+                st.exps[2] = ex[2];
             }
 #pragma unroll
-            for (int e = 0; e < 3; ++e) {
-                top[e] = warp_max(top[e]);
-                if (lane == 0) sc.top[e][warp] = top[e];
+            for (int i = 0; i < 8; ++i) {
+                const int tok = 8 * th + i;
+                store_pair(sc.k, tok, c, kp[i].x * sk, kp[i].y * sk);
+                store_pair(st.q, tok, c, qp[i].x * sq, qp[i].y * sq);
+                store_pair(st.ke, tok, c, ke[i].x * se, ke[i].y * se);
+                const float2 ks = mul1(kk[i], xk), qs = mul1(qq[i], xq);
+                // blocks of 16: the second half is upper
+                const float2 g = th ? pre[i] : suf[i], k0 = mul2(ks, g);
+                store_pair(sc.level[0], th ? i : 16 + i, c, k0.x, k0.y);
+                if (th) {
+                    const float2 q0 = mul2(qs, g);
+                    store_pair(sc.level[0], 8 + i, c, q0.x, q0.y);
+                }
+#pragma unroll
+                for (int l = 1; l < 4; ++l) {
+                    const int half = 8 >> l;
+                    const int row = 4 * th + i / (2 * half) * half + i % half;   // of its side's 8
+                    const float2 f = l == 1 ? f1[i] : l == 2 ? f2[i] : i % 2 ? al[i] : one;
+                    const float2 kl = mul2(ks, f);
+                    if (i & half) {
+                        const float2 ql = mul2(qs, f);
+                        store_pair(sc.level[l], row, c, kl.x, kl.y);
+                        store_pair(sc.level[l], 8 + row, c, ql.x, ql.y);
+                    } else {
+                        store_pair(sc.level[l], 16 + row, c, kl.x, kl.y);
+                    }
+                }
             }
-            if (n >= kStages) named_sync(2 + kStages + n % kStages, threads);   // the stage is read
-            st.total[c] = total;
         }
         named_sync(1, D);
         if (first + kChunk < t1) fetch(first + kChunk);
-        {
-            int ex[3];
+        for (int l = warp; l < 4; l += NP) {
+            float b[4] = {}, x[4] = {};
 #pragma unroll
-            for (int e = 0; e < 3; ++e) {
-                float top = sc.top[e][0];
+            for (int j = 0; j < D / 32; ++j) {
+                uint32_t yh[4], yl[4];
+                ldmatrix4<false>(yh, &sc.level[l][0][16 + lane % 8][32 * j + lane / 8 * 8]);
+                ldmatrix4<false>(yl, &sc.level[l][1][16 + lane % 8][32 * j + lane / 8 * 8]);
 #pragma unroll
-                for (int w = 1; w < NP; ++w) top = fmaxf(top, sc.top[e][w]);
-                ex[e] = scale_exp(top);
-                if (c == 0) st.exps[e] = ex[e];
-            }
-            const float sk = exp2i(ex[0]), sq = exp2i(ex[1]), se = exp2i(ex[2]);
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                split_half(kp[i] * sk, st.k[0][i][c], st.k[1][i][c]);
-                split_half(qp[i] * sq, st.q[0][i][c], st.q[1][i][c]);
-                split_half(ke[i] * se, st.ke[0][i][c], st.ke[1][i][c]);
-            }
-        }
-        // pairs: the columns j of this warp, in twos of equal work
-        auto load = [&](const float* row, float (&x)[CH]) {
-            if constexpr (CH == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(row + lane * 4);
-                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-            } else if constexpr (CH == 2) {
-                const float2 v = *reinterpret_cast<const float2*>(row + lane * 2);
-                x[0] = v.x; x[1] = v.y;
-            } else {
-                x[0] = row[lane];
-            }
-        };
-        float (*red)[36] = sc.red[warp];
-        for (int g = 0; g < kChunk / NP; ++g) {
-            const int j = g / 2 * 2 * NP + (g % 2 ? 2 * NP - 1 - static_cast<int>(warp) : static_cast<int>(warp));
-            float e[CH], x[CH], y[CH], z[CH];
-            load(sc.k[j], e);
-            load(sc.q[j], y);
-            float sp = 0.0f, sa;
-#pragma unroll
-            for (int i = 0; i < CH; ++i) sp = fmaf(y[i], e[i], sp);
-            red[16 + j][lane] = sp;
-#pragma unroll 3
-            for (int i = j + 1; i < kChunk; ++i) {
-                load(sc.a[i], x);
-                load(sc.q[i], y);
-                load(sc.k[i], z);
-                sp = sa = 0.0f;
-#pragma unroll
-                for (int m = 0; m < CH; ++m) {
-                    e[m] *= x[m];
-                    sa = fmaf(z[m], e[m], sa);
-                    sp = fmaf(y[m], e[m], sp);
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t xh[4], xl[4];
+                    ldmatrix4<false>(xh, &sc.level[l][0][arow][32 * j + 16 * e + acol]);
+                    ldmatrix4<false>(xl, &sc.level[l][1][arow][32 * j + 16 * e + acol]);
+                    mma_f16(b, xh, yh[2 * e], yh[2 * e + 1]);
+                    mma_f16(x, xl, yh[2 * e], yh[2 * e + 1]);
+                    mma_f16(x, xh, yl[2 * e], yl[2 * e + 1]);
                 }
-                red[i][lane] = sa;
-                red[16 + i][lane] = sp;
             }
-            __syncwarp();
-            const float s = sum_rows(red, lane);
-            const int i = lane % 16;
-            if (lane < 16) sc.A[i][j] = i > j ? s : 0.0f;
-            else sc.P[i][j] = i >= j ? s : 0.0f;
-            __syncwarp();
+            const int half = 8 >> l, u = lane / 4, i = u / half * 2 * half + half + u % half;
+            const float fk = pow2(-lk), fq = pow2(-lq);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int w = lane % 4 * 2 + e, j = w / half * 2 * half + w % half;
+                if (u / half != w / half) continue;
+                sc.At[j][i] = (b[e] + x[e]) * fk * fk;
+                sc.P[i][j] = (b[2 + e] + x[2 + e]) * fk * fq;
+            }
         }
         named_sync(1, D);
-        if (warp == 0) {   // T, a lane per column
+        if (warp == n % NP) {   // T, a lane per column, one row's multiple after the other
             const uint32_t j = lane % 16;
             float x[kChunk], top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                float s = 0.0f;
+            for (int i = 0; i < kChunk; ++i) x[i] = 0.0f;
 #pragma unroll
-                for (int m = 0; m < i; ++m) s = fmaf(sc.A[i][m], x[m], s);
-                x[i] = (i == static_cast<int>(j) ? 1.0f : 0.0f) - sc.beta[i] * s;
+            for (int m = 0; m < kChunk; ++m) {
+                x[m] = fmaf(-sc.beta[m], x[m], m == static_cast<int>(j) ? 1.0f : 0.0f);
+#pragma unroll
+                for (int i = m + 1; i < kChunk; ++i) x[i] = fmaf(sc.At[m][i], x[m], x[i]);
             }
             const float b = sc.beta[j];
 #pragma unroll
@@ -415,25 +504,54 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
                 x[i] *= b;
                 top = fmaxf(top, fabsf(x[i]));
             }
-            const int ex = scale_exp(warp_max(top));
-            if (lane == 0) st.exps[3] = ex;
-            const float f = exp2i(ex);
+            const int e = scale_exp(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+            if (lane == 0) {
+                st.exps[3] = e;
+                st.exps[0] = e + ex[0] - 20;
+            }
+            const float f = exp2i(e);
             if (lane < 16)
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) split_half(x[i] * f, st.t[0][i][j], st.t[1][i][j]);
         }
-        if (warp == NP - 1) {
+        if (warp == (n + 1) % NP) {   // P
             float x[8], top = 0.0f;
+            const int j = lane % 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = sc.P[2 * i + lane / 16][lane % 16];
-                top = fmaxf(top, fabsf(x[i]));
+            for (int m = 0; m < 8; ++m) {
+                const int i = 2 * m + lane / 16;
+                x[m] = i > j ? sc.P[i][j] : 0.0f;
+                if (i == j)
+#pragma unroll
+                    for (int w = 0; w < NP; ++w) x[m] += sc.diag[w][i];
+                top = fmaxf(top, fabsf(x[m]));
             }
-            const int ex = scale_exp(warp_max(top));
-            if (lane == 0) st.exps[4] = ex;
-            const float f = exp2i(ex);
+            const int e = scale_exp(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
+            if (lane == 0) st.exps[4] = e;
+            const float f = exp2i(e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) split_half(x[i] * f, st.p[0][2 * i + lane / 16][lane % 16], st.p[1][2 * i + lane / 16][lane % 16]);
+            for (int m = 0; m < 8; ++m) split_half(x[m] * f, st.p[0][2 * m + lane / 16][j], st.p[1][2 * m + lane / 16][j]);
+        }
+        named_sync(1, D);
+        {   // W = T (p K): 16 sums of products below 2^30, kept as multiples of 2^20
+            uint32_t xh[4], xl[4];
+            ldmatrix4<false>(xh, &st.t[0][arow][acol]);
+            ldmatrix4<false>(xl, &st.t[1][arow][acol]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int col = warp * 32 + 16 * j;
+                float b[2][4] = {}, x[2][4] = {};
+                uint32_t yh[4], yl[4];
+                ldmatrix4<true>(yh, &sc.k[0][arow][col + acol]);
+                ldmatrix4<true>(yl, &sc.k[1][arow][col + acol]);
+                mma_terms(b, x, xh, xl, yh, yl);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        store_pair(st.w, lane / 4 + 8 * r, col + 8 * e + lane % 4 * 2, (b[e][2 * r] + x[e][2 * r]) * 0x1p-20f,
+                                   (b[e][2 * r + 1] + x[e][2 * r + 1]) * 0x1p-20f);
+            }
         }
         named_arrive(2 + n % kStages, threads);
     }
@@ -449,24 +567,18 @@ __device__ __forceinline__ void row_exps(float m0, float m1, int (&ex)[2]) {
     ex[0] = scale_exp(m0);
     ex[1] = scale_exp(m1);
 }
-
-// [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
-__device__ __forceinline__ void split_rows(const float (&x)[2][4], const float (&f)[2], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-    split_pair(x[0][0] * f[0], x[0][1] * f[0], hi[0], lo[0]);
-    split_pair(x[0][2] * f[1], x[0][3] * f[1], hi[1], lo[1]);
-    split_pair(x[1][0] * f[0], x[1][1] * f[0], hi[2], lo[2]);
-    split_pair(x[1][2] * f[1], x[1][3] * f[1], hi[3], lo[3]);
+__device__ __forceinline__ void row_exps(const float (&x)[2][4], int (&ex)[2]) {
+    row_exps(fmaxf(fmaxf(fabsf(x[0][0]), fabsf(x[0][1])), fmaxf(fabsf(x[1][0]), fabsf(x[1][1]))),
+             fmaxf(fmaxf(fabsf(x[0][2]), fabsf(x[0][3])), fmaxf(fabsf(x[1][2]), fabsf(x[1][3]))), ex);
 }
 
-// big += x hi * y hi, small += the cross products, for two n-tiles.
-__device__ __forceinline__ void mma_terms(float (&big)[2][4], float (&small)[2][4], const uint32_t (&xh)[4], const uint32_t (&xl)[4],
-                                          const uint32_t (&yh)[4], const uint32_t (&yl)[4]) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n) mma_f16(big[n], xh, yh[2 * n], yh[2 * n + 1]);
-#pragma unroll
-    for (int n = 0; n < 2; ++n) mma_f16(small[n], xl, yh[2 * n], yh[2 * n + 1]);
-#pragma unroll
-    for (int n = 0; n < 2; ++n) mma_f16(small[n], xh, yl[2 * n], yl[2 * n + 1]);
+// [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
+__device__ __forceinline__ void split_rows(const float (&x)[2][4], const int (&ex)[2], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    const float f0 = exp2i(ex[0]), f1 = exp2i(ex[1]);
+    split_pair(x[0][0] * f0, x[0][1] * f0, hi[0], lo[0]);
+    split_pair(x[0][2] * f1, x[0][3] * f1, hi[1], lo[1]);
+    split_pair(x[1][0] * f0, x[1][1] * f0, hi[2], lo[2]);
+    split_pair(x[1][2] * f1, x[1][3] * f1, hi[3], lo[3]);
 }
 
 template <int D, typename E>
@@ -492,8 +604,8 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const size_t tok = first + 8 * n + 2 * t + e % 2;
-                vv[n][e] = tok < t1 ? to_f(v[tok * a.row_stride + 8 * (e / 2)]) : 0.0f;
+                const uint32_t tok = first + 8 * n + 2 * t + e % 2;
+                vv[n][e] = tok < t1 ? to_f(v[static_cast<size_t>(tok) * a.row_stride + 8 * (e / 2)]) : 0.0f;
             }
     };
     fetch(t0);
@@ -504,7 +616,7 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
     uint32_t n = 0;
     for (uint32_t first = t0; first < t1; first += kChunk, ++n) {
         const ChunkStage<D>& st = stages[n % kStages];
-        int ex[2];
+        int sx[2], vx[2], ux[2];
         {
             float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
@@ -512,53 +624,41 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
                 m0 = fmaxf(m0, fmaxf(fabsf(S[j][0]), fabsf(S[j][1])));
                 m1 = fmaxf(m1, fmaxf(fabsf(S[j][2]), fabsf(S[j][3])));
             }
-            row_exps(m0, m1, ex);
+            row_exps(m0, m1, sx);
         }
-        const float up[2] = {exp2i(ex[0]), exp2i(ex[1])}, down[2] = {exp2i(-ex[0]), exp2i(-ex[1])};
+        row_exps(vv, vx);
+        uint32_t xh[4], xl[4], yh[4], yl[4];
+        split_rows(vv, vx, xh, xl);
+        if (first + kChunk < t1) fetch(first + kChunk);
+        const float sd[2] = {exp2i(-sx[0]), exp2i(-sx[1])};
         named_sync(2 + n % kStages, threads);
-        float kb[2][4] = {}, ks[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
+        // T V, W S0^T, (p Q) S0^T
+        float ub[2][4] = {}, us[2][4] = {}, wb[2][4] = {}, ws[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
+        ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
+        ldmatrix4<false>(yl, &st.t[1][mrow][mcol]);
+        mma_terms(ub, us, xh, xl, yh, yl);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
-            uint32_t xh[4], xl[4], yh[4], yl[4];
             const float x[2][4] = {{S[2 * j][0], S[2 * j][1], S[2 * j][2], S[2 * j][3]},
                                    {S[2 * j + 1][0], S[2 * j + 1][1], S[2 * j + 1][2], S[2 * j + 1][3]}};
-            split_rows(x, up, xh, xl);
-            ldmatrix4<false>(yh, &st.k[0][mrow][16 * j + mcol]);
-            ldmatrix4<false>(yl, &st.k[1][mrow][16 * j + mcol]);
-            mma_terms(kb, ks, xh, xl, yh, yl);
+            split_rows(x, sx, xh, xl);
+            ldmatrix4<false>(yh, &st.w[0][mrow][16 * j + mcol]);
+            ldmatrix4<false>(yl, &st.w[1][mrow][16 * j + mcol]);
+            mma_terms(wb, ws, xh, xl, yh, yl);
             ldmatrix4<false>(yh, &st.q[0][mrow][16 * j + mcol]);
             ldmatrix4<false>(yl, &st.q[1][mrow][16 * j + mcol]);
             mma_terms(ob, os, xh, xl, yh, yl);
         }
-        uint32_t xh[4], xl[4], yh[4], yl[4];
-        float r[2][4], ub[2][4] = {}, us[2][4] = {};
-        int rx[2], ux[2];
         {
-            const float f = exp2i(-st.exps[0]);
+            const float fw = pow2(-st.exps[0]), ft = pow2(-st.exps[3]), vd[2] = {exp2i(-vx[0]), exp2i(-vx[1])};
+            float u[2][4];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[i][e] = fmaf((kb[i][e] + ks[i][e]) * f, -down[e / 2], vv[i][e]);
-            row_exps(fmaxf(fmaxf(fabsf(r[0][0]), fabsf(r[0][1])), fmaxf(fabsf(r[1][0]), fabsf(r[1][1]))),
-                     fmaxf(fmaxf(fabsf(r[0][2]), fabsf(r[0][3])), fmaxf(fabsf(r[1][2]), fabsf(r[1][3]))), rx);
-            if (first + kChunk < t1) fetch(first + kChunk);
-            const float fr[2] = {exp2i(rx[0]), exp2i(rx[1])};
-            split_rows(r, fr, xh, xl);
-            ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
-            ldmatrix4<false>(yl, &st.t[1][mrow][mcol]);
-            mma_terms(ub, us, xh, xl, yh, yl);
-        }
-        float u[2][4];
-        {
-            const float f = exp2i(-st.exps[3]), fd[2] = {exp2i(-rx[0]), exp2i(-rx[1])};
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[i][e] = (ub[i][e] + us[i][e]) * f * fd[e / 2];
-            row_exps(fmaxf(fmaxf(fabsf(u[0][0]), fabsf(u[0][1])), fmaxf(fabsf(u[1][0]), fabsf(u[1][1]))),
-                     fmaxf(fmaxf(fabsf(u[0][2]), fabsf(u[0][3])), fmaxf(fabsf(u[1][2]), fabsf(u[1][3]))), ux);
-            const float fu[2] = {exp2i(ux[0]), exp2i(ux[1])};
-            split_rows(u, fu, xh, xl);
+                for (int e = 0; e < 4; ++e)
+                    u[i][e] = fmaf((ub[i][e] + us[i][e]) * ft, vd[e / 2], -((wb[i][e] + ws[i][e]) * fw * sd[e / 2]));
+            row_exps(u, ux);
+            split_rows(u, ux, xh, xl);
         }
         const float ud[2] = {exp2i(-ux[0]), exp2i(-ux[1])};
         {   // S = S diag(total) + U^T (e K)
@@ -566,10 +666,10 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
                 float b[2][4] = {}, x[2][4] = {};
-                uint32_t wh[4], wl[4];
-                ldmatrix4<true>(wh, &st.ke[0][krow][16 * j + kcol]);
-                ldmatrix4<true>(wl, &st.ke[1][krow][16 * j + kcol]);
-                mma_terms(b, x, xh, xl, wh, wl);
+                uint32_t zh[4], zl[4];
+                ldmatrix4<true>(zh, &st.ke[0][krow][16 * j + kcol]);
+                ldmatrix4<true>(zl, &st.ke[1][krow][16 * j + kcol]);
+                mma_terms(b, x, xh, xl, zh, zl);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 tot = *reinterpret_cast<const float2*>(&st.total[16 * j + 8 * i + 2 * t]);
@@ -590,7 +690,7 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t tok = first + 8 * i + 2 * t + e % 2;
-                    const float o = fmaf((ob[i][e] + os[i][e]) * fq, down[e / 2], (pb[i][e] + px[i][e]) * fp * ud[e / 2]);
+                    const float o = fmaf((ob[i][e] + os[i][e]) * fq, sd[e / 2], (pb[i][e] + px[i][e]) * fp * ud[e / 2]);
                     if (tok < t1) store1<E>(a.out, static_cast<size_t>(tok) * P + h * D + row0 + g + 8 * (e / 2), o);
                 }
         }
@@ -606,7 +706,7 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
 
 // A CTA: D / 32 producer warps and NW consumer warps (16 NW value rows of a
 // head). Named barriers: 1 among the producers, 2.. a stage is full, 5.. read.
-template <int D, int NW, typename E>
+template <int D, int NW, typename E, bool VEC>
 __global__ void __launch_bounds__(D + 32 * NW) kda_chunk_kernel(const SeqArgs a) {
     extern __shared__ __align__(16) unsigned char chunk_mem[];
     ChunkStage<D>* stages = reinterpret_cast<ChunkStage<D>*>(chunk_mem);
@@ -615,7 +715,7 @@ __global__ void __launch_bounds__(D + 32 * NW) kda_chunk_kernel(const SeqArgs a)
     const uint32_t s = blockIdx.y, h = blockIdx.x / slices, r0 = blockIdx.x % slices * (16 * NW);
     uint32_t t0, t1;
     if (!token_range(a, s, t0, t1)) return;
-    if (threadIdx.x < D) chunk_producer<D, E>(a, h, t0, t1, stages, scratch, D + 32 * NW);
+    if (threadIdx.x < D) chunk_producer<D, E, VEC>(a, h, t0, t1, stages, scratch, D + 32 * NW);
     else chunk_consumer<D, E>(a, s, h, r0 + (threadIdx.x - D) / 32 * 16, t0, t1, stages, D + 32 * NW);
 }
 
@@ -633,19 +733,26 @@ int launch_recurrent(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     return K3XB_OK;
 }
 
-template <int D, int NW, typename E>
-int launch_chunk(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
+template <int D, int NW, typename E, bool VEC>
+int launch_chunk_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     static std::atomic<uint64_t> configured{0};   // per template instance
     const int cst = configure_once(ctx, configured, [&]() -> int {
-        K3XB_CUDA(ctx, cudaFuncSetAttribute(kda_chunk_kernel<D, NW, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        K3XB_CUDA(ctx, cudaFuncSetAttribute(kda_chunk_kernel<D, NW, E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             static_cast<int>(chunk_smem<D>())));
         return K3XB_OK;
     });
     if (cst) return cst;
     const dim3 grid(a.heads * (D / (16 * NW)), sequences);
-    kda_chunk_kernel<D, NW, E><<<grid, D + 32 * NW, chunk_smem<D>(), ctx->stream>>>(a);
+    kda_chunk_kernel<D, NW, E, VEC><<<grid, D + 32 * NW, chunk_smem<D>(), ctx->stream>>>(a);
     K3XB_LAUNCHED(ctx);
     return K3XB_OK;
+}
+
+template <int D, int NW, typename E>
+int launch_chunk(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
+    // two channels a load where every row starts at one
+    const bool vec = aligned(a.q, 2 * sizeof(E)) && aligned(a.k, 2 * sizeof(E)) && a.row_stride % 2 == 0 && aligned(a.log_decay, 8);
+    return vec ? launch_chunk_as<D, NW, E, true>(ctx, a, sequences) : launch_chunk_as<D, NW, E, false>(ctx, a, sequences);
 }
 
 template <typename E>
