@@ -10,11 +10,13 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
 #include "kernels.cuh"
 #include "profile.cuh"
+#include "tc.cuh"
 
 namespace k3xb {
 
@@ -187,10 +189,16 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // (decay from j to there). Four block sizes (16, 8, 4, 2) make four products
 // of 8 upper by 8 lower rows, of which a token is in one side each.
 //
-// Producer warps make a chunk's operands; consumer warps own 16 value rows
-// each and keep S in registers, in the accumulator layout of mma.m16n8k16,
-// which is also the layout its left operand is read in: S, V and U go from
-// accumulators straight into the next product, without shared memory.
+// Two kernels. chunk_operands_kernel makes every chunk's operands, all chunks
+// and heads side by side. chunk_scan_kernel goes along the sequences: a warp
+// owns 16 value rows and keeps S in registers, in the accumulator layout of
+// mma.m16n8k16, which is also the layout its left operand is read in: S, V
+// and U go from accumulators straight into the next product, without shared
+// memory. (Both in one kernel, with producer warps beside the scan's, took
+// 7900 cycles a chunk for the operands where the scan needs 2000, and kept
+// half the GPU idle at one sequence.) A chunk's operands cross memory once,
+// about as many bytes as its inputs, as an image of the shared memory that
+// the scan copies them to.
 //
 // Every operand is carried as two f16 terms of a power-of-two multiple (hi +
 // lo, 22 bits of the largest element of its tile or row), and a product as hi
@@ -200,9 +208,11 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // digits and TF32 in two terms would take twice the MMAs.
 
 constexpr int kChunk = 16, kStages = 3;
+// Operands held at a time: longer batches go in segments of chunks.
+constexpr size_t kOperandBytes = size_t(1) << 30;
 
 template <int D>
-struct __align__(16) ChunkStage {
+struct __align__(128) ChunkStage {
     // hi, lo; [tok][channel] rows of D + 8 values: ldmatrix reads 8 of them
     // without a bank conflict; 16 + 8 likewise
     __half w[2][kChunk][D + 8], q[2][kChunk][D + 8], ke[2][kChunk][D + 8];   // W, p Q, e K
@@ -216,18 +226,32 @@ struct __align__(16) ChunkScratch {
     __half k[2][kChunk][D + 8];           // p K
     // per block size: 8 upper rows of k, 8 of q, 8 lower rows of k
     __half level[4][2][24][D + 8];
+    __half t[2][kChunk][kChunk + 8];
     float At[kChunk][kChunk];             // At[j][i] = A_ij
     float P[kChunk][kChunk];
-    float diag[D / 32][kChunk];           // q_i . k_i by producer warp
+    float diag[D / 32][kChunk];           // q_i . k_i by warp
     float beta[kChunk];
     uint32_t top[6][D / 32];
 };
 
-template <int D>
-constexpr size_t chunk_smem() { return kStages * sizeof(ChunkStage<D>) + sizeof(ChunkScratch<D>); }
-
-__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-__device__ __forceinline__ void named_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+// The chunks of a call lie in slots: sequence s from offsets[s] / 16 + s on
+// (a sequence of n tokens ends before the next one's: n / 16 rounded up is at
+// most the distance). A segment is a range of slots.
+struct ChunkPlan {
+    uint32_t slot0, slots;     // this segment
+    uint32_t stride;           // chunks that a CTA of the first kernel steps over
+    void* stages;              // [slots][heads] ChunkStage
+    const float* carry_in;     // states at the segment's start of sequences that began before it
+    float* carry_out;          // states at its end
+};
+// The chunks [first, last) of a sequence that lie in the segment.
+__device__ __forceinline__ void segment_chunks(const ChunkPlan& p, uint32_t s, uint32_t t0, uint32_t t1, uint32_t& first,
+                                               uint32_t& last, uint32_t& base) {
+    base = t0 / kChunk + s;
+    const uint32_t n = (t1 - t0 + kChunk - 1) / kChunk;
+    first = min(n, p.slot0 > base ? p.slot0 - base : 0u);
+    last = min(n, p.slot0 + p.slots > base ? p.slot0 + p.slots - base : 0u);
+}
 
 // The power of two that takes a maximum to [2^14, 2^15) (f16 ends at 2^16);
 // zero, infinity and NaN keep theirs.
@@ -259,7 +283,7 @@ __device__ __forceinline__ void store_pair(__half (&dst)[2][ROWS][W], int row, i
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
 }
@@ -308,12 +332,19 @@ __device__ __forceinline__ uint32_t warp_top(const float2 (&x)[8]) {
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return make_float2(x.x * y.x, x.y * y.y); }
 __device__ __forceinline__ float2 mul1(float2 x, float y) { return make_float2(x.x * y, x.y * y); }
 
-// A producer thread: two neighbouring channels of eight tokens, lanes 0-15
-// the chunk's first half, 16-31 the same channels' second half.
+// D threads: each two neighbouring channels of eight tokens, lanes 0-15 the
+// chunk's first half, 16-31 the same channels' second half.
 template <int D, typename E, bool VEC>
-__device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uint32_t t0, uint32_t t1, ChunkStage<D>* stages,
-                                               ChunkScratch<D>& sc, int threads) {
-    constexpr int NP = D / 32;   // producer warps
+__global__ void __launch_bounds__(D) chunk_operands_kernel(const SeqArgs a, const ChunkPlan plan) {
+    extern __shared__ __align__(16) unsigned char chunk_mem[];
+    ChunkScratch<D>& sc = *reinterpret_cast<ChunkScratch<D>*>(chunk_mem);
+    constexpr int NP = D / 32;   // warps
+    const uint32_t s = blockIdx.y, h = blockIdx.x % a.heads;
+    uint32_t t0, t1, chunk, chunk_end, base;
+    if (!token_range(a, s, t0, t1)) return;
+    segment_chunks(plan, s, t0, t1, chunk, chunk_end, base);
+    chunk += blockIdx.x / a.heads;
+    if (chunk >= chunk_end) return;
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, th = lane / 16, P = a.heads * D;
     const uint32_t c = warp * 32 + lane % 16 * 2;
     const E* q = static_cast<const E*>(a.q) + h * D + c;
@@ -337,10 +368,9 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
             bb = first + threadIdx.x < t1 ? a.beta[static_cast<size_t>(first + threadIdx.x) * a.heads + h] : 0.0f;
     };
     const uint32_t arow = lane % 16, acol = lane / 16 * 8;         // ldmatrix: left operands, and k-major ones transposed
-    fetch(t0);
-    uint32_t n = 0;
-    for (uint32_t first = t0; first < t1; first += kChunk, ++n) {
-        ChunkStage<D>& st = stages[n % kStages];
+    fetch(t0 + chunk * kChunk);
+    for (; chunk < chunk_end; chunk += plan.stride) {
+        ChunkStage<D>& st = static_cast<ChunkStage<D>*>(plan.stages)[static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h];
         // decays within blocks of 8 (f[0]), 8's halves (f[1]), 4's (f[2])
         // and 2's (f[3]): upper tokens from the middle, lower ones to it
         float2 f1[8], f2[8], pre[8], suf[8];
@@ -407,9 +437,8 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
             if (lane % 2 == 0) sc.diag[warp][8 * th + lane % 16 / 2] = d[0];
         }
         if (threadIdx.x < kChunk) sc.beta[threadIdx.x] = bb;
-        if (n >= kStages) named_sync(2 + kStages + n % kStages, threads);   // the stage is read
         if (th) *reinterpret_cast<float2*>(&st.total[c]) = mul2(pre[7], other);
-        named_sync(1, D);
+        __syncthreads();
         int ex[6];
 #pragma unroll
         for (int e = 0; e < 6; ++e) {
@@ -457,8 +486,8 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
                 }
             }
         }
-        named_sync(1, D);
-        if (first + kChunk < t1) fetch(first + kChunk);
+        __syncthreads();
+        if (chunk + plan.stride < chunk_end) fetch(t0 + (chunk + plan.stride) * kChunk);
         for (int l = warp; l < 4; l += NP) {
             float b[4] = {}, x[4] = {};
 #pragma unroll
@@ -486,8 +515,8 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
                 sc.P[i][j] = (b[2 + e] + x[2 + e]) * fk * fq;
             }
         }
-        named_sync(1, D);
-        if (warp == n % NP) {   // T, a lane per column, one row's multiple after the other
+        __syncthreads();
+        if (warp == 0) {   // T, a lane per column, one row's multiple after the other
             const uint32_t j = lane % 16;
             float x[kChunk], top = 0.0f;
 #pragma unroll
@@ -512,9 +541,13 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
             const float f = exp2i(e);
             if (lane < 16)
 #pragma unroll
-                for (int i = 0; i < kChunk; ++i) split_half(x[i] * f, st.t[0][i][j], st.t[1][i][j]);
+                for (int i = 0; i < kChunk; ++i) {
+                    split_half(x[i] * f, sc.t[0][i][j], sc.t[1][i][j]);
+                    st.t[0][i][j] = sc.t[0][i][j];
+                    st.t[1][i][j] = sc.t[1][i][j];
+                }
         }
-        if (warp == (n + 1) % NP) {   // P
+        if (warp == NP - 1) {   // P
             float x[8], top = 0.0f;
             const int j = lane % 16;
 #pragma unroll
@@ -532,11 +565,11 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
 #pragma unroll
             for (int m = 0; m < 8; ++m) split_half(x[m] * f, st.p[0][2 * m + lane / 16][j], st.p[1][2 * m + lane / 16][j]);
         }
-        named_sync(1, D);
+        __syncthreads();
         {   // W = T (p K): 16 sums of products below 2^30, kept as multiples of 2^20
             uint32_t xh[4], xl[4];
-            ldmatrix4<false>(xh, &st.t[0][arow][acol]);
-            ldmatrix4<false>(xl, &st.t[1][arow][acol]);
+            ldmatrix4<false>(xh, &sc.t[0][arow][acol]);
+            ldmatrix4<false>(xl, &sc.t[1][arow][acol]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int col = warp * 32 + 16 * j;
@@ -553,7 +586,7 @@ __device__ __forceinline__ void chunk_producer(const SeqArgs& a, uint32_t h, uin
                                    (b[e][2 * r + 1] + x[e][2 * r + 1]) * 0x1p-20f);
             }
         }
-        named_arrive(2 + n % kStages, threads);
+        __syncthreads();
     }
 }
 
@@ -581,19 +614,65 @@ __device__ __forceinline__ void split_rows(const float (&x)[2][4], const int (&e
     split_pair(x[1][2] * f1, x[1][3] * f1, hi[3], lo[3]);
 }
 
-template <int D, typename E>
-__device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uint32_t h, uint32_t row0, uint32_t t0, uint32_t t1,
-                                               const ChunkStage<D>* stages, int threads) {
-    const uint32_t lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, P = a.heads * D;
+struct ScanBars {
+    uint64_t full[kStages], empty[kStages];
+    int abort;
+};
+template <int D>
+constexpr size_t scan_smem() { return kStages * sizeof(ChunkStage<D>) + sizeof(ScanBars); }
+
+// NW warps of 16 value rows of one head, and a warp that copies the operands.
+template <int D, int NW, typename E>
+__global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs a, const ChunkPlan plan) {
+    extern __shared__ __align__(128) unsigned char scan_mem[];
+    ChunkStage<D>* stages = reinterpret_cast<ChunkStage<D>*>(scan_mem);
+    ScanBars& bar = *reinterpret_cast<ScanBars*>(scan_mem + kStages * sizeof(ChunkStage<D>));
+    volatile int* abort = &bar.abort;
+    constexpr uint32_t slices = D / (16 * NW);
+    const uint32_t s = blockIdx.y, h = blockIdx.x / slices, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint32_t t0, t1, chunk, chunk_end, base;
+    if (!token_range(a, s, t0, t1)) return;
+    segment_chunks(plan, s, t0, t1, chunk, chunk_end, base);
+    // a sequence without tokens passes its state on in the first segment
+    if (chunk >= chunk_end && (t0 < t1 || plan.slot0)) return;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tc::mbar_init(&bar.full[i], 1);
+            tc::mbar_init(&bar.empty[i], NW);
+        }
+        bar.abort = 0;
+        tc::fence_barrier_init();
+    }
+    __syncthreads();
+    if (warp == NW) {
+        if (lane == 0) {
+            const ChunkStage<D>* src = static_cast<const ChunkStage<D>*>(plan.stages) + static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h;
+            uint32_t n = 0;
+            for (; chunk + n < chunk_end; ++n, src += a.heads) {
+                if (!tc::mbar_wait(&bar.empty[n % kStages], n / kStages & 1u ^ 1u, abort)) break;
+                tc::mbar_arrive_expect_tx(&bar.full[n % kStages], sizeof(ChunkStage<D>));
+                tc::bulk_load(&stages[n % kStages], src, sizeof(ChunkStage<D>), &bar.full[n % kStages]);
+            }
+            volatile int never = 0;   // copies in flight end before the CTA does
+            for (uint32_t i = 0; i < kStages && i < n; ++i)
+                tc::mbar_wait(&bar.full[(n - 1 - i) % kStages], (n - 1 - i) / kStages & 1u, &never, 200000000ull);
+            if (*abort) atomicExch(a.status, K3XB_BACKEND_UNAVAILABLE);
+        }
+        return;
+    }
+    const uint32_t row0 = blockIdx.x % slices * (16 * NW) + warp * 16;
+    const uint32_t g = lane / 4, t = lane % 4, P = a.heads * D;
     const size_t state_at = (static_cast<size_t>(s) * a.heads + h) * D * D + static_cast<size_t>(row0 + g) * D + 2 * t;
     const E* v = static_cast<const E*>(a.v) + h * D + row0 + g;
+    const float* state = chunk ? plan.carry_in : a.state;
+    float* state_out = chunk_end * kChunk < t1 - t0 ? plan.carry_out : a.state_out;
     float S[D / 8][4];
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
         float2 x = make_float2(0.0f, 0.0f), y = x;
-        if (a.state) {
-            x = *reinterpret_cast<const float2*>(a.state + state_at + 8 * j);
-            y = *reinterpret_cast<const float2*>(a.state + state_at + 8 * D + 8 * j);
+        if (state) {
+            x = *reinterpret_cast<const float2*>(state + state_at + 8 * j);
+            y = *reinterpret_cast<const float2*>(state + state_at + 8 * D + 8 * j);
         }
         S[j][0] = x.x; S[j][1] = x.y; S[j][2] = y.x; S[j][3] = y.y;
     }
@@ -608,13 +687,13 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
                 vv[n][e] = tok < t1 ? to_f(v[static_cast<size_t>(tok) * a.row_stride + 8 * (e / 2)]) : 0.0f;
             }
     };
-    fetch(t0);
+    fetch(t0 + chunk * kChunk);
     // ldmatrix rows: n-major operands (lanes 0-7: tile 0, k 0-7; 8-15: k 8-15; 16-31: tile 1)
     const uint32_t mrow = lane % 8 + lane / 16 * 8, mcol = lane / 8 % 2 * 8;
     // k-major ones, transposed (lanes 0-7: tile 0, k 0-7; 8-15: k 8-15; 16-31: tile 1)
     const uint32_t krow = lane % 16, kcol = lane / 16 * 8;
-    uint32_t n = 0;
-    for (uint32_t first = t0; first < t1; first += kChunk, ++n) {
+    for (uint32_t n = 0; chunk + n < chunk_end; ++n) {
+        const uint32_t first = t0 + (chunk + n) * kChunk;
         const ChunkStage<D>& st = stages[n % kStages];
         int sx[2], vx[2], ux[2];
         {
@@ -629,9 +708,10 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
         row_exps(vv, vx);
         uint32_t xh[4], xl[4], yh[4], yl[4];
         split_rows(vv, vx, xh, xl);
-        if (first + kChunk < t1) fetch(first + kChunk);
+        if (chunk + n + 1 < chunk_end) fetch(first + kChunk);
         const float sd[2] = {exp2i(-sx[0]), exp2i(-sx[1])};
-        named_sync(2 + n % kStages, threads);
+        tc::mbar_pass(&bar.full[n % kStages], n / kStages & 1u, abort);
+        __syncwarp();
         // T V, W S0^T, (p Q) S0^T
         float ub[2][4] = {}, us[2][4] = {}, wb[2][4] = {}, ws[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
         ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
@@ -694,29 +774,15 @@ __device__ __forceinline__ void chunk_consumer(const SeqArgs& a, uint32_t s, uin
                     if (tok < t1) store1<E>(a.out, static_cast<size_t>(tok) * P + h * D + row0 + g + 8 * (e / 2), o);
                 }
         }
-        if (first + kStages * kChunk < t1) named_arrive(2 + kStages + n % kStages, threads);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bar.empty[n % kStages]);
     }
-    if (!a.state_out) return;
+    if (!state_out) return;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
-        *reinterpret_cast<float2*>(a.state_out + state_at + 8 * j) = make_float2(S[j][0], S[j][1]);
-        *reinterpret_cast<float2*>(a.state_out + state_at + 8 * D + 8 * j) = make_float2(S[j][2], S[j][3]);
+        *reinterpret_cast<float2*>(state_out + state_at + 8 * j) = make_float2(S[j][0], S[j][1]);
+        *reinterpret_cast<float2*>(state_out + state_at + 8 * D + 8 * j) = make_float2(S[j][2], S[j][3]);
     }
-}
-
-// A CTA: D / 32 producer warps and NW consumer warps (16 NW value rows of a
-// head). Named barriers: 1 among the producers, 2.. a stage is full, 5.. read.
-template <int D, int NW, typename E, bool VEC>
-__global__ void __launch_bounds__(D + 32 * NW) kda_chunk_kernel(const SeqArgs a) {
-    extern __shared__ __align__(16) unsigned char chunk_mem[];
-    ChunkStage<D>* stages = reinterpret_cast<ChunkStage<D>*>(chunk_mem);
-    ChunkScratch<D>& scratch = *reinterpret_cast<ChunkScratch<D>*>(chunk_mem + kStages * sizeof(ChunkStage<D>));
-    constexpr uint32_t slices = D / (16 * NW);
-    const uint32_t s = blockIdx.y, h = blockIdx.x / slices, r0 = blockIdx.x % slices * (16 * NW);
-    uint32_t t0, t1;
-    if (!token_range(a, s, t0, t1)) return;
-    if (threadIdx.x < D) chunk_producer<D, E, VEC>(a, h, t0, t1, stages, scratch, D + 32 * NW);
-    else chunk_consumer<D, E>(a, s, h, r0 + (threadIdx.x - D) / 32 * 16, t0, t1, stages, D + 32 * NW);
 }
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -734,17 +800,42 @@ int launch_recurrent(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
 }
 
 template <int D, int NW, typename E, bool VEC>
-int launch_chunk_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
+int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     static std::atomic<uint64_t> configured{0};   // per template instance
     const int cst = configure_once(ctx, configured, [&]() -> int {
-        K3XB_CUDA(ctx, cudaFuncSetAttribute(kda_chunk_kernel<D, NW, E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            static_cast<int>(chunk_smem<D>())));
+        K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_operands_kernel<D, E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            static_cast<int>(sizeof(ChunkScratch<D>))));
+        K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_scan_kernel<D, NW, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            static_cast<int>(scan_smem<D>())));
         return K3XB_OK;
     });
     if (cst) return cst;
-    const dim3 grid(a.heads * (D / (16 * NW)), sequences);
-    kda_chunk_kernel<D, NW, E, VEC><<<grid, D + 32 * NW, chunk_smem<D>(), ctx->stream>>>(a);
-    K3XB_LAUNCHED(ctx);
+    const uint32_t slots = a.tokens / kChunk + sequences;
+    const size_t per_slot = a.heads * sizeof(ChunkStage<D>);
+    const uint32_t step = static_cast<uint32_t>(std::min<size_t>(slots, std::max<size_t>(1, kOperandBytes / per_slot)));
+    // states between segments: in state_out, or in scratch where that is not wanted
+    const size_t carry = step < slots && !a.state_out ? static_cast<size_t>(sequences) * a.heads * D * D : 0;
+    Sizer sz;
+    sz.take<unsigned char>(step * per_slot);
+    sz.take<float>(carry);
+    void* mem;
+    if (const int st = ensure_scratch(ctx, sz.used, &mem)) return st;
+    Carver cv(mem);
+    ChunkPlan p{};
+    p.stages = cv.take<unsigned char>(step * per_slot);
+    float* between = cv.take<float>(carry);
+    if (!carry) between = a.state_out;
+    p.carry_in = p.carry_out = between;
+    for (uint32_t x = 0; x < slots; x += step) {
+        p.slot0 = x;
+        p.slots = std::min(step, slots - x);
+        // one CTA per chunk of an average sequence; longer ones loop
+        p.stride = std::min((p.slots + sequences - 1) / sequences, 0x7fffffffu / a.heads);
+        chunk_operands_kernel<D, E, VEC><<<dim3(p.stride * a.heads, sequences), D, sizeof(ChunkScratch<D>), ctx->stream>>>(a, p);
+        K3XB_LAUNCHED(ctx);
+        chunk_scan_kernel<D, NW, E><<<dim3(a.heads * (D / (16 * NW)), sequences), 32 * NW + 32, scan_smem<D>(), ctx->stream>>>(a, p);
+        K3XB_LAUNCHED(ctx);
+    }
     return K3XB_OK;
 }
 
@@ -752,7 +843,7 @@ template <int D, int NW, typename E>
 int launch_chunk(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     // two channels a load where every row starts at one
     const bool vec = aligned(a.q, 2 * sizeof(E)) && aligned(a.k, 2 * sizeof(E)) && a.row_stride % 2 == 0 && aligned(a.log_decay, 8);
-    return vec ? launch_chunk_as<D, NW, E, true>(ctx, a, sequences) : launch_chunk_as<D, NW, E, false>(ctx, a, sequences);
+    return vec ? launch_chunks_as<D, NW, E, true>(ctx, a, sequences) : launch_chunks_as<D, NW, E, false>(ctx, a, sequences);
 }
 
 template <typename E>
