@@ -266,18 +266,22 @@ __device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
     hi = __float2half_rn(x);
     lo = __float2half_rn(x - __half2float(hi));
 }
+
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) { return make_float2(x.x * y.x, x.y * y.y); }
+__device__ __forceinline__ float2 mul1(float2 x, float y) { return make_float2(x.x * y, x.y * y); }
+
 // Two neighbours as packed hi and lo.
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
+__device__ __forceinline__ void split_pair(float2 x, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __float22half2_rn(x);
     const float2 b = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - b.x, y - b.y);
+    const __half2 l = __floats2half2_rn(x.x - b.x, x.y - b.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 template <int ROWS, int W>
-__device__ __forceinline__ void store_pair(__half (&dst)[2][ROWS][W], int row, int col, float x, float y) {
+__device__ __forceinline__ void store_pair(__half (&dst)[2][ROWS][W], int row, int col, float2 x) {
     uint32_t hi, lo;
-    split_pair(x, y, hi, lo);
+    split_pair(x, hi, lo);
     *reinterpret_cast<uint32_t*>(&dst[0][row][col]) = hi;
     *reinterpret_cast<uint32_t*>(&dst[1][row][col]) = lo;
 }
@@ -309,6 +313,18 @@ __device__ __forceinline__ void mma_terms(float (&big)[2][4], float (&small)[2][
     for (int n = 0; n < 2; ++n) mma_f16(small[n], xh, yl[2 * n], yl[2 * n + 1]);
 }
 
+// The same for a contraction of one step, in one accumulator: the small
+// products first, so that the sum is truncated once at its full size.
+__device__ __forceinline__ void mma_terms1(float (&c)[2][4], const uint32_t (&xh)[4], const uint32_t (&xl)[4], const uint32_t (&yh)[4],
+                                           const uint32_t (&yl)[4]) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(c[n], xl, yh[2 * n], yh[2 * n + 1]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(c[n], xh, yl[2 * n], yl[2 * n + 1]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) mma_f16(c[n], xh, yh[2 * n], yh[2 * n + 1]);
+}
+
 // Two neighbouring values as floats; VEC: at a multiple of two elements.
 template <typename E, bool VEC>
 __device__ __forceinline__ float2 load2(const E* p) {
@@ -329,13 +345,11 @@ __device__ __forceinline__ uint32_t warp_top(const float2 (&x)[8]) {
     for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
     return __reduce_max_sync(0xffffffffu, m);
 }
-__device__ __forceinline__ float2 mul2(float2 x, float2 y) { return make_float2(x.x * y.x, x.y * y.y); }
-__device__ __forceinline__ float2 mul1(float2 x, float y) { return make_float2(x.x * y, x.y * y); }
 
 // D threads: each two neighbouring channels of eight tokens, lanes 0-15 the
 // chunk's first half, 16-31 the same channels' second half.
 template <int D, typename E, bool VEC>
-__global__ void __launch_bounds__(D) chunk_operands_kernel(const SeqArgs a, const ChunkPlan plan) {
+__global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(const SeqArgs a, const ChunkPlan plan) {
     extern __shared__ __align__(16) unsigned char chunk_mem[];
     ChunkScratch<D>& sc = *reinterpret_cast<ChunkScratch<D>*>(chunk_mem);
     constexpr int NP = D / 32;   // warps
@@ -459,16 +473,16 @@ __global__ void __launch_bounds__(D) chunk_operands_kernel(const SeqArgs a, cons
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int tok = 8 * th + i;
-                store_pair(sc.k, tok, c, kp[i].x * sk, kp[i].y * sk);
-                store_pair(st.q, tok, c, qp[i].x * sq, qp[i].y * sq);
-                store_pair(st.ke, tok, c, ke[i].x * se, ke[i].y * se);
+                store_pair(sc.k, tok, c, mul1(kp[i], sk));
+                store_pair(st.q, tok, c, mul1(qp[i], sq));
+                store_pair(st.ke, tok, c, mul1(ke[i], se));
                 const float2 ks = mul1(kk[i], xk), qs = mul1(qq[i], xq);
                 // blocks of 16: the second half is upper
                 const float2 g = th ? pre[i] : suf[i], k0 = mul2(ks, g);
-                store_pair(sc.level[0], th ? i : 16 + i, c, k0.x, k0.y);
+                store_pair(sc.level[0], th ? i : 16 + i, c, k0);
                 if (th) {
                     const float2 q0 = mul2(qs, g);
-                    store_pair(sc.level[0], 8 + i, c, q0.x, q0.y);
+                    store_pair(sc.level[0], 8 + i, c, q0);
                 }
 #pragma unroll
                 for (int l = 1; l < 4; ++l) {
@@ -478,10 +492,10 @@ __global__ void __launch_bounds__(D) chunk_operands_kernel(const SeqArgs a, cons
                     const float2 kl = mul2(ks, f);
                     if (i & half) {
                         const float2 ql = mul2(qs, f);
-                        store_pair(sc.level[l], row, c, kl.x, kl.y);
-                        store_pair(sc.level[l], 8 + row, c, ql.x, ql.y);
+                        store_pair(sc.level[l], row, c, kl);
+                        store_pair(sc.level[l], 8 + row, c, ql);
                     } else {
-                        store_pair(sc.level[l], 16 + row, c, kl.x, kl.y);
+                        store_pair(sc.level[l], 16 + row, c, kl);
                     }
                 }
             }
@@ -573,17 +587,17 @@ __global__ void __launch_bounds__(D) chunk_operands_kernel(const SeqArgs a, cons
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int col = warp * 32 + 16 * j;
-                float b[2][4] = {}, x[2][4] = {};
+                float w[2][4] = {};
                 uint32_t yh[4], yl[4];
                 ldmatrix4<true>(yh, &sc.k[0][arow][col + acol]);
                 ldmatrix4<true>(yl, &sc.k[1][arow][col + acol]);
-                mma_terms(b, x, xh, xl, yh, yl);
+                mma_terms1(w, xh, xl, yh, yl);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        store_pair(st.w, lane / 4 + 8 * r, col + 8 * e + lane % 4 * 2, (b[e][2 * r] + x[e][2 * r]) * 0x1p-20f,
-                                   (b[e][2 * r + 1] + x[e][2 * r + 1]) * 0x1p-20f);
+                        store_pair(st.w, lane / 4 + 8 * r, col + 8 * e + lane % 4 * 2,
+                                   mul1(make_float2(w[e][2 * r], w[e][2 * r + 1]), 0x1p-20f));
             }
         }
         __syncthreads();
@@ -606,14 +620,12 @@ __device__ __forceinline__ void row_exps(const float (&x)[2][4], int (&ex)[2]) {
 }
 
 // [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
-__device__ __forceinline__ void split_rows(const float (&x)[2][4], const int (&ex)[2], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-    const float f0 = exp2i(ex[0]), f1 = exp2i(ex[1]);
-    split_pair(x[0][0] * f0, x[0][1] * f0, hi[0], lo[0]);
-    split_pair(x[0][2] * f1, x[0][3] * f1, hi[1], lo[1]);
-    split_pair(x[1][0] * f0, x[1][1] * f0, hi[2], lo[2]);
-    split_pair(x[1][2] * f1, x[1][3] * f1, hi[3], lo[3]);
+__device__ __forceinline__ void split_rows(const float (&x)[4], const float (&y)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    split_pair(make_float2(x[0], x[1]), hi[0], lo[0]);
+    split_pair(make_float2(x[2], x[3]), hi[1], lo[1]);
+    split_pair(make_float2(y[0], y[1]), hi[2], lo[2]);
+    split_pair(make_float2(y[2], y[3]), hi[3], lo[3]);
 }
-
 struct ScanBars {
     uint64_t full[kStages], empty[kStages];
     int abort;
@@ -622,8 +634,8 @@ template <int D>
 constexpr size_t scan_smem() { return kStages * sizeof(ChunkStage<D>) + sizeof(ScanBars); }
 
 // NW warps of 16 value rows of one head, and a warp that copies the operands.
-template <int D, int NW, typename E>
-__global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs a, const ChunkPlan plan) {
+template <int D, int NW, int PER_SM, typename E>
+__global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const SeqArgs a, const ChunkPlan plan) {
     extern __shared__ __align__(128) unsigned char scan_mem[];
     ChunkStage<D>* stages = reinterpret_cast<ChunkStage<D>*>(scan_mem);
     ScanBars& bar = *reinterpret_cast<ScanBars*>(scan_mem + kStages * sizeof(ChunkStage<D>));
@@ -645,14 +657,28 @@ __global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs 
     }
     __syncthreads();
     if (warp == NW) {
-        if (lane == 0) {
-            const ChunkStage<D>* src = static_cast<const ChunkStage<D>*>(plan.stages) + static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h;
-            uint32_t n = 0;
-            for (; chunk + n < chunk_end; ++n, src += a.heads) {
-                if (!tc::mbar_wait(&bar.empty[n % kStages], n / kStages & 1u ^ 1u, abort)) break;
-                tc::mbar_arrive_expect_tx(&bar.full[n % kStages], sizeof(ChunkStage<D>));
-                tc::bulk_load(&stages[n % kStages], src, sizeof(ChunkStage<D>), &bar.full[n % kStages]);
+        const ChunkStage<D>* src = static_cast<const ChunkStage<D>*>(plan.stages) + static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h;
+        const E* v = static_cast<const E*>(a.v) + h * D + blockIdx.x % slices * (16 * NW);
+        uint32_t n = 0;
+        bool ok = true;
+        for (; ok && chunk + n < chunk_end; ++n, src += a.heads) {
+            // this CTA's columns of v, for the warps to find in L2
+            const uint32_t tok = t0 + (chunk + n) * kChunk + lane / 2;
+            if (tok < t1) {
+                const E* at = v + static_cast<size_t>(tok) * a.row_stride + lane % 2 * (8 * NW);
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
             }
+            if (lane == 0) {
+                ok = tc::mbar_wait(&bar.empty[n % kStages], n / kStages & 1u ^ 1u, abort);
+                if (ok) {
+                    tc::mbar_arrive_expect_tx(&bar.full[n % kStages], sizeof(ChunkStage<D>));
+                    tc::bulk_load(&stages[n % kStages], src, sizeof(ChunkStage<D>), &bar.full[n % kStages]);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        if (!ok) --n;   // the last one was not copied
+        if (lane == 0) {
             volatile int never = 0;   // copies in flight end before the CTA does
             for (uint32_t i = 0; i < kStages && i < n; ++i)
                 tc::mbar_wait(&bar.full[(n - 1 - i) % kStages], (n - 1 - i) / kStages & 1u, &never, 200000000ull);
@@ -692,10 +718,11 @@ __global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs 
     const uint32_t mrow = lane % 8 + lane / 16 * 8, mcol = lane / 8 % 2 * 8;
     // k-major ones, transposed (lanes 0-7: tile 0, k 0-7; 8-15: k 8-15; 16-31: tile 1)
     const uint32_t krow = lane % 16, kcol = lane / 16 * 8;
+    int sx[2] = {0, 0};   // S holds the state's rows times 2^sx
     for (uint32_t n = 0; chunk + n < chunk_end; ++n) {
         const uint32_t first = t0 + (chunk + n) * kChunk;
         const ChunkStage<D>& st = stages[n % kStages];
-        int sx[2], vx[2], ux[2];
+        int vx[2], ux[2];
         {
             float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
@@ -703,25 +730,53 @@ __global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs 
                 m0 = fmaxf(m0, fmaxf(fabsf(S[j][0]), fabsf(S[j][1])));
                 m1 = fmaxf(m1, fmaxf(fabsf(S[j][2]), fabsf(S[j][3])));
             }
-            row_exps(m0, m1, sx);
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+            }
+            // a row's multiple changes when its largest element leaves
+            // [2^8, 2^15]: f16 holds it then, with 32 bits below it
+            const bool off0 = m0 > 0x1p15f || (m0 < 0x1p8f && m0 != 0.0f && sx[0] < 100);
+            const bool off1 = m1 > 0x1p15f || (m1 < 0x1p8f && m1 != 0.0f && sx[1] < 100);
+            if (__any_sync(0xffffffffu, off0 || off1)) {
+                const int d0 = off0 ? min(scale_exp(m0) - 2, 100 - sx[0]) : 0, d1 = off1 ? min(scale_exp(m1) - 2, 100 - sx[1]) : 0;
+                const float f0 = exp2i(d0), f1 = exp2i(d1);
+                sx[0] += d0;
+                sx[1] += d1;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) {
+                    S[j][0] *= f0;
+                    S[j][1] *= f0;
+                    S[j][2] *= f1;
+                    S[j][3] *= f1;
+                }
+            }
         }
-        row_exps(vv, vx);
         uint32_t xh[4], xl[4], yh[4], yl[4];
-        split_rows(vv, vx, xh, xl);
+        row_exps(vv, vx);
+        {
+            const float f0 = exp2i(vx[0]), f1 = exp2i(vx[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                vv[i][0] *= f0;
+                vv[i][1] *= f0;
+                vv[i][2] *= f1;
+                vv[i][3] *= f1;
+            }
+            split_rows(vv[0], vv[1], xh, xl);
+        }
         if (chunk + n + 1 < chunk_end) fetch(first + kChunk);
-        const float sd[2] = {exp2i(-sx[0]), exp2i(-sx[1])};
         tc::mbar_pass(&bar.full[n % kStages], n / kStages & 1u, abort);
         __syncwarp();
         // T V, W S0^T, (p Q) S0^T
-        float ub[2][4] = {}, us[2][4] = {}, wb[2][4] = {}, ws[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
+        float u[2][4] = {}, wb[2][4] = {}, ws[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
         ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
         ldmatrix4<false>(yl, &st.t[1][mrow][mcol]);
-        mma_terms(ub, us, xh, xl, yh, yl);
+        mma_terms1(u, xh, xl, yh, yl);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
-            const float x[2][4] = {{S[2 * j][0], S[2 * j][1], S[2 * j][2], S[2 * j][3]},
-                                   {S[2 * j + 1][0], S[2 * j + 1][1], S[2 * j + 1][2], S[2 * j + 1][3]}};
-            split_rows(x, sx, xh, xl);
+            split_rows(S[2 * j], S[2 * j + 1], xh, xl);
             ldmatrix4<false>(yh, &st.w[0][mrow][16 * j + mcol]);
             ldmatrix4<false>(yl, &st.w[1][mrow][16 * j + mcol]);
             mma_terms(wb, ws, xh, xl, yh, yl);
@@ -730,47 +785,59 @@ __global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs 
             mma_terms(ob, os, xh, xl, yh, yl);
         }
         {
-            const float fw = pow2(-st.exps[0]), ft = pow2(-st.exps[3]), vd[2] = {exp2i(-vx[0]), exp2i(-vx[1])};
-            float u[2][4];
+            const float fw[2] = {pow2(-st.exps[0] - sx[0]), pow2(-st.exps[0] - sx[1])};
+            const float fv[2] = {pow2(-st.exps[3] - vx[0]), pow2(-st.exps[3] - vx[1])};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    u[i][e] = fmaf((ub[i][e] + us[i][e]) * ft, vd[e / 2], -((wb[i][e] + ws[i][e]) * fw * sd[e / 2]));
+                for (int e = 0; e < 4; ++e) u[i][e] = fmaf(wb[i][e] + ws[i][e], -fw[e / 2], u[i][e] * fv[e / 2]);
             row_exps(u, ux);
-            split_rows(u, ux, xh, xl);
+            // a product's two powers together stay within a float's
+            ux[0] = min(ux[0], 126 - max(st.exps[2], st.exps[4]));
+            ux[1] = min(ux[1], 126 - max(st.exps[2], st.exps[4]));
+            const float f0 = pow2(ux[0]), f1 = pow2(ux[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u[i][0] *= f0;
+                u[i][1] *= f0;
+                u[i][2] *= f1;
+                u[i][3] *= f1;
+            }
+            split_rows(u[0], u[1], xh, xl);
         }
-        const float ud[2] = {exp2i(-ux[0]), exp2i(-ux[1])};
+        const float fq[2] = {pow2(-st.exps[1] - sx[0]), pow2(-st.exps[1] - sx[1])};
         {   // S = S diag(total) + U^T (e K)
-            const float f = exp2i(-st.exps[2]);
+            const float f0 = pow2(sx[0] - ux[0] - st.exps[2]), f1 = pow2(sx[1] - ux[1] - st.exps[2]);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
-                float b[2][4] = {}, x[2][4] = {};
+                float c[2][4] = {};
                 uint32_t zh[4], zl[4];
                 ldmatrix4<true>(zh, &st.ke[0][krow][16 * j + kcol]);
                 ldmatrix4<true>(zl, &st.ke[1][krow][16 * j + kcol]);
-                mma_terms(b, x, xh, xl, zh, zl);
+                mma_terms1(c, xh, xl, zh, zl);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 tot = *reinterpret_cast<const float2*>(&st.total[16 * j + 8 * i + 2 * t]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        S[2 * j + i][e] = fmaf((b[i][e] + x[i][e]) * f, ud[e / 2], S[2 * j + i][e] * (e % 2 ? tot.y : tot.x));
+                    float (&x)[4] = S[2 * j + i];
+                    x[0] = fmaf(c[i][0], f0, x[0] * tot.x);
+                    x[1] = fmaf(c[i][1], f0, x[1] * tot.y);
+                    x[2] = fmaf(c[i][2], f1, x[2] * tot.x);
+                    x[3] = fmaf(c[i][3], f1, x[3] * tot.y);
                 }
             }
         }
         {   // O = (p Q) S0^T + P U
-            float pb[2][4] = {}, px[2][4] = {};
+            float c[2][4] = {};
             ldmatrix4<false>(yh, &st.p[0][mrow][mcol]);
             ldmatrix4<false>(yl, &st.p[1][mrow][mcol]);
-            mma_terms(pb, px, xh, xl, yh, yl);
-            const float fq = exp2i(-st.exps[1]), fp = exp2i(-st.exps[4]);
+            mma_terms1(c, xh, xl, yh, yl);
+            const float fp[2] = {pow2(-ux[0] - st.exps[4]), pow2(-ux[1] - st.exps[4])};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t tok = first + 8 * i + 2 * t + e % 2;
-                    const float o = fmaf((ob[i][e] + os[i][e]) * fq, sd[e / 2], (pb[i][e] + px[i][e]) * fp * ud[e / 2]);
+                    const float o = fmaf(ob[i][e] + os[i][e], fq[e / 2], c[i][e] * fp[e / 2]);
                     if (tok < t1) store1<E>(a.out, static_cast<size_t>(tok) * P + h * D + row0 + g + 8 * (e / 2), o);
                 }
         }
@@ -778,10 +845,11 @@ __global__ void __launch_bounds__(32 * NW + 32) chunk_scan_kernel(const SeqArgs 
         if (lane == 0) tc::mbar_arrive(&bar.empty[n % kStages]);
     }
     if (!state_out) return;
+    const float f0 = pow2(-sx[0]), f1 = pow2(-sx[1]);
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
-        *reinterpret_cast<float2*>(state_out + state_at + 8 * j) = make_float2(S[j][0], S[j][1]);
-        *reinterpret_cast<float2*>(state_out + state_at + 8 * D + 8 * j) = make_float2(S[j][2], S[j][3]);
+        *reinterpret_cast<float2*>(state_out + state_at + 8 * j) = make_float2(S[j][0] * f0, S[j][1] * f0);
+        *reinterpret_cast<float2*>(state_out + state_at + 8 * D + 8 * j) = make_float2(S[j][2] * f1, S[j][3] * f1);
     }
 }
 
@@ -805,8 +873,9 @@ int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     const int cst = configure_once(ctx, configured, [&]() -> int {
         K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_operands_kernel<D, E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             static_cast<int>(sizeof(ChunkScratch<D>))));
-        K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_scan_kernel<D, NW, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            static_cast<int>(scan_smem<D>())));
+        for (auto* scan : {chunk_scan_kernel<D, NW, 1, E>, chunk_scan_kernel<D, NW, 2, E>})
+            K3XB_CUDA(ctx, cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                static_cast<int>(scan_smem<D>())));
         return K3XB_OK;
     });
     if (cst) return cst;
@@ -829,11 +898,17 @@ int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     for (uint32_t x = 0; x < slots; x += step) {
         p.slot0 = x;
         p.slots = std::min(step, slots - x);
-        // one CTA per chunk of an average sequence; longer ones loop
-        p.stride = std::min((p.slots + sequences - 1) / sequences, 0x7fffffffu / a.heads);
+        // sixteen CTAs for each that the GPU holds at a time (three per SM), so
+        // that sequences of unlike lengths even out and a CTA has chunks to
+        // load ahead; no more than an average sequence's chunks
+        const uint64_t wanted = (48ull * ctx->sm_count + static_cast<uint64_t>(a.heads) * sequences - 1) / (static_cast<uint64_t>(a.heads) * sequences);
+        p.stride = static_cast<uint32_t>(std::min<uint64_t>(wanted, (p.slots + sequences - 1) / sequences));
         chunk_operands_kernel<D, E, VEC><<<dim3(p.stride * a.heads, sequences), D, sizeof(ChunkScratch<D>), ctx->stream>>>(a, p);
         K3XB_LAUNCHED(ctx);
-        chunk_scan_kernel<D, NW, E><<<dim3(a.heads * (D / (16 * NW)), sequences), 32 * NW + 32, scan_smem<D>(), ctx->stream>>>(a, p);
+        const dim3 grid(a.heads * (D / (16 * NW)), sequences);
+        const bool crowd = static_cast<uint64_t>(grid.x) * grid.y > static_cast<uint64_t>(ctx->sm_count);
+        if (crowd) chunk_scan_kernel<D, NW, 2, E><<<grid, 32 * NW + 32, scan_smem<D>(), ctx->stream>>>(a, p);
+        else chunk_scan_kernel<D, NW, 1, E><<<grid, 32 * NW + 32, scan_smem<D>(), ctx->stream>>>(a, p);
         K3XB_LAUNCHED(ctx);
     }
     return K3XB_OK;
