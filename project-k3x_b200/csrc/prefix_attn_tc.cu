@@ -90,25 +90,20 @@ struct PrefixPlan {
     uint32_t blocks;           // 128-key blocks of the prefix
     uint32_t pairs, odd;       // row tile pairs; 1: a last single tile
     uint32_t steps_per_head;
-    uint32_t ctas, max_seg;    // parts a CTA may leave
-    uint64_t total;            // steps in all; 0: no prefix
+    uint32_t range, max_seg;   // steps of a CTA; parts it may leave
+    uint32_t total;            // steps in all; 0: no prefix
 };
-
-__host__ __device__ __forceinline__ uint64_t first_step(const PrefixPlan& p, uint32_t cta) { return cta * p.total / p.ctas; }
 
 // A (kv head, row tile pair) and where its steps lie in the flat list.
 struct Job {
-    uint32_t head, pair, index;
-    uint64_t begin;
-    uint32_t steps;
+    uint32_t head, pair, index, begin, steps;
 };
-__device__ __forceinline__ Job job_of(const PrefixPlan& p, uint64_t step) {
+__device__ __forceinline__ Job job_of(const PrefixPlan& p, uint32_t step) {
     Job j;
-    j.head = static_cast<uint32_t>(step / p.steps_per_head);
-    const uint32_t off = static_cast<uint32_t>(step % p.steps_per_head);
-    j.pair = min(off / p.blocks, p.pairs);
+    j.head = step / p.steps_per_head;
+    j.pair = min((step - j.head * p.steps_per_head) / p.blocks, p.pairs);
     j.index = j.head * (p.pairs + p.odd) + j.pair;
-    j.begin = static_cast<uint64_t>(j.head) * p.steps_per_head + static_cast<uint64_t>(j.pair) * p.blocks;
+    j.begin = j.head * p.steps_per_head + j.pair * p.blocks;
     j.steps = j.pair < p.pairs ? p.blocks : (p.blocks + 1) / 2;
     return j;
 }
@@ -142,11 +137,11 @@ struct Segment {
     }
     __device__ __forceinline__ uint32_t block(uint32_t t, uint32_t i) const { return keys ? 2 * (first + i) + t : first + i; }
 };
-__device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint64_t x, uint64_t end) {
+__device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint32_t x, uint32_t end) {
     Segment s;
     s.job = job_of(p, x);
-    s.first = static_cast<uint32_t>(x - s.job.begin);
-    s.n = static_cast<uint32_t>(min(end, s.job.begin + s.job.steps) - x);
+    s.first = x - s.job.begin;
+    s.n = min(end, s.job.begin + s.job.steps) - x;
     s.keys = s.job.pair == p.pairs;
     return s;
 }
@@ -201,7 +196,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = bar.tmem_base;
-    const uint64_t lo = first_step(p, blockIdx.x), hi = first_step(p, blockIdx.x + 1);
+    const uint32_t lo = blockIdx.x * p.range, hi = min(p.total, lo + p.range);
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -237,7 +232,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                         tc::tma_load_3d(ring + pos % slots * kAtom + e * (kAtom / 2), &map_v, full, NV == 2 ? e * 128 : 0, head,
                                         block * kTile + (NV == 2 ? i : e) * 64);
             };
-            for (uint64_t x = lo; x < hi && ok;) {
+            for (uint32_t x = lo; x < hi && ok;) {
                 const Segment s = segment_at(p, x, hi);
                 const uint32_t h = s.job.head, n1 = s.active(1, p.blocks);
                 load_k(h, s.block(0, 0));
@@ -312,7 +307,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 }
                 p_phase ^= 1u << t;
             };
-            for (uint64_t x = lo; x < hi; ++seg) {
+            for (uint32_t x = lo; x < hi; ++seg) {
                 const Segment s = segment_at(p, x, hi);
                 const uint32_t n1 = s.active(1, p.blocks);
                 for (uint32_t t = 0; t < 2; ++t) tc::mbar_pass(&bar.q_ready[t], seg & 1u, abort);
@@ -366,7 +361,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(b);
         };
-        for (uint64_t x = lo; x < hi; ++seg) {
+        for (uint32_t x = lo; x < hi; ++seg) {
             const Segment s = segment_at(p, x, hi);
             const uint32_t tile = 2 * s.job.pair + (s.keys ? 0 : t), n = s.active(t, p.blocks);
             // the tile's query rows, swizzled as the MMA reads them: eight
@@ -509,12 +504,14 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&x)[4], uin
 
 struct OwnPlan {
     uint32_t row_tiles;   // 16-row tiles of a sequence's rows per kv head
-    uint32_t splits;      // CTAs along a sequence's keys
+    uint32_t splits;      // tasks along a sequence's keys
+    uint32_t tasks;       // [kv head][row tile][split] of a sequence
+    uint32_t prefix;      // 1: the tasks read the prefix too
     float* o;             // [seq][kv head][row tile][split][16][value] where splits > 1
     float2* ml;           // [seq][kv head][row tile][split][16]
 };
 
-// A running join of parts for one row and `C` of its columns.
+// A running join of parts for one row and C of its columns.
 template <int C>
 struct Join {
     float m = -INFINITY, l = 0.0f, o[C];
@@ -522,57 +519,74 @@ struct Join {
 #pragma unroll
         for (int i = 0; i < C; ++i) o[i] = 0.0f;
     }
-    __device__ __forceinline__ void add(float2 ml, const float* src) {
+    __device__ __forceinline__ void add(float2 ml, const float (&x)[C]) {
         if (ml.x == -INFINITY && ml.y == 0.0f) return;   // no visible key: o was never written
         const float mn = fmaxf(m, ml.x), at = mn == -INFINITY ? 0.0f : mn;
         const float w0 = ex2(m - at), w1 = ex2(ml.x - at);
         l = fmaf(l, w0, ml.y * w1);
         m = mn;
 #pragma unroll
-        for (int i = 0; i < C; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(src + i);
-            o[i] = fmaf(o[i], w0, x.x * w1);
-            o[i + 1] = fmaf(o[i + 1], w0, x.y * w1);
-            o[i + 2] = fmaf(o[i + 2], w0, x.z * w1);
-            o[i + 3] = fmaf(o[i + 3], w0, x.w * w1);
-        }
+        for (int i = 0; i < C; ++i) o[i] = fmaf(o[i], w0, x[i] * w1);
+    }
+};
+template <int C>
+__device__ __forceinline__ void load_cols(const float* src, float (&x)[C]) {
+    if constexpr (C == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        x[0] = v.x; x[1] = v.y;
+    }
+}
+
+// The prefix's parts of one row of a kv head.
+struct RowParts {
+    size_t at, step;      // the first part's row; from one CTA's to the next one's
+    uint32_t n, halves, seg0;
+    __device__ __forceinline__ RowParts(const PrefixPlan& p, uint32_t h, uint32_t r) {
+        const uint32_t tile = r / kTile, pair = min(tile / 2, p.pairs), jobs = p.pairs + p.odd;
+        const bool keys = pair == p.pairs;
+        const uint32_t begin = h * p.steps_per_head + pair * p.blocks;
+        const uint32_t end = begin + (keys ? (p.blocks + 1) / 2 : p.blocks);
+        const uint32_t c0 = begin / p.range, c1 = (end - 1) / p.range;
+        // the job is one of the segments of CTA c0 and the first one of the CTAs behind it
+        seg0 = h * jobs + pair - job_of(p, c0 * p.range).index;
+        halves = keys ? 2 : 1;
+        n = (c1 - c0 + 1) * halves;
+        step = static_cast<size_t>(p.max_seg) * 2 * kTile;
+        at = c0 * step + (keys ? 0 : tile % 2) * kTile + r % kTile;
+    }
+    __device__ __forceinline__ size_t part(uint32_t i) const {
+        const uint32_t c = i / halves;
+        return at + c * step + (c ? 0 : seg0 * 2 * kTile) + (i - c * halves) * kTile;
     }
 };
 
-// Adds the prefix's parts of row r (of kv head h), columns col .. col + C,
-// four parts' loads at a time in flight.
+// Joins the prefix's parts to two rows' sums, a lane C columns, up to eight
+// loads in flight.
 template <int C>
-__device__ __forceinline__ void join_prefix(Join<C>& j, const PrefixPlan& p, const Parts& parts, uint32_t h, uint32_t r,
-                                            uint32_t col, uint32_t value) {
-    if (!p.total) return;
-    const uint32_t tile = r / kTile, pair = min(tile / 2, p.pairs), jobs = p.pairs + p.odd;
-    const bool keys = pair == p.pairs;
-    const uint64_t begin = static_cast<uint64_t>(h) * p.steps_per_head + static_cast<uint64_t>(pair) * p.blocks;
-    const uint64_t end = begin + (keys ? (p.blocks + 1) / 2 : p.blocks);
-    const uint32_t c0 = static_cast<uint32_t>(((begin + 1) * p.ctas - 1) / p.total);
-    const uint32_t c1 = static_cast<uint32_t>((end * p.ctas - 1) / p.total);
-    // the job is the last one that CTA c0 begins, or its only one, and the
-    // first one of the CTAs behind it
-    const uint32_t seg0 = h * jobs + pair - job_of(p, first_step(p, c0)).index;
-    const uint32_t halves = keys ? 2 : 1, n = (c1 - c0 + 1) * halves;
-    for (uint32_t i0 = 0; i0 < n; i0 += 4) {
-        size_t at[4];
-        float2 ml[4];
+__device__ __forceinline__ void join_prefix(Join<C> (&j)[2], const PrefixPlan& p, const Parts& parts, uint32_t h, const uint32_t (&r)[2],
+                                            const bool (&there)[2], uint32_t col, uint32_t value) {
+    const RowParts rows[2] = {RowParts(p, h, r[0]), RowParts(p, h, r[1])};
+    const uint32_t n[2] = {there[0] ? rows[0].n : 0, there[1] ? rows[1].n : 0}, most = max(n[0], n[1]);
+    for (uint32_t i0 = 0; i0 < most; i0 += 4) {
+        float x[2][4][C];
+        float2 ml[2][4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t k = min(i0 + i, n - 1), c = k / halves;
-            at[i] = ((static_cast<size_t>(c0 + c) * p.max_seg + (c ? 0 : seg0)) * 2 + (keys ? k % 2 : tile % 2)) * kTile + r % kTile;
-            ml[i] = parts.ml[at[i]];
-        }
-        float4 x[4][C / 4];
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
+            for (uint32_t i = 0; i < 4; ++i)
+                if (i0 + i < n[k]) {
+                    const size_t at = rows[k].part(i0 + i);
+                    ml[k][i] = parts.ml[at];
+                    load_cols<C>(parts.o + at * value + col, x[k][i]);
+                }
 #pragma unroll
-            for (int e = 0; e < C / 4; ++e)
-                x[i][e] = reinterpret_cast<const float4*>(parts.o + at[i] * value + col)[e];
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-            if (i0 + i < n) j.add(ml[i], reinterpret_cast<const float*>(x[i]));
+            for (uint32_t i = 0; i < 4; ++i)
+                if (i0 + i < n[k]) j[k].add(ml[k][i], x[k][i]);
     }
 }
 
@@ -581,12 +595,9 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, const Join<C>& j, u
                                           uint32_t col) {
     const size_t row = (static_cast<size_t>(s) * a.N + node) * a.heads + head;
     const float inv = j.l == 0.0f ? 0.0f : 1.0f / j.l;   // nothing visible: a zero row
-    uint32_t w[C / 2];
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + row * a.value + col);
 #pragma unroll
-    for (int i = 0; i < C; i += 2) w[i / 2] = pack2<BF16>(j.o[i] * inv, j.o[i + 1] * inv);
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.value + col);
-#pragma unroll
-    for (int i = 0; i < C / 8; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    for (int i = 0; i < C / 2; ++i) dst[i] = pack2<BF16>(j.o[2 * i] * inv, j.o[2 * i + 1] * inv);
     if (a.lse && col == 0) a.lse[row] = j.l == 0.0f ? -INFINITY : (j.m + __log2f(j.l)) * kLn2;
 }
 
@@ -608,36 +619,113 @@ __device__ __forceinline__ float half_of(uint16_t w) {
 
 constexpr uint32_t kOwnThreads = 128;
 
-// A CTA takes 16 rows of one sequence and kv head; its four warps take 16
-// keys at a time in turn. Key and value rows go straight from global memory
-// to MMA fragments, 16 bytes a lane: the contraction over key dimensions may
-// run in any order, so lane t of a quad reads 8 neighbouring dimensions and
-// feeds them to two steps of 16 (the queries are read alike), and value
-// column g of an output tile j stands for dimension 8 g + j.
+// A task is 16 rows of one sequence and kv head (and a split of its keys), 16
+// keys at a time: one warp's where there are many tasks, four warps' that
+// take tiles in turn where there are few. Key and value rows go straight from
+// global memory to MMA fragments, 16 bytes a lane: the contraction over key
+// dimensions may run in any order, so lane t of a quad reads 8 neighbouring
+// dimensions and feeds them to two steps of 16 (the queries are read alike),
+// and value column g of an output tile j stands for dimension 8 g + j.
 //
 // Draft rows are masked by the node's ancestors. A masked key's probability
 // is zero, but zero times a value that is infinite or NaN is not, so the
 // product takes such values of draft rows as zeros, and the rows that do see
 // them add them one by one.
-template <int DQ, int DV, bool BF16>
-__global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
+template <int DQ, int DV, bool BF16, uint32_t W>
+__global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
                                                           const Parts parts, const OwnPlan own) {
     constexpr int SEG = DQ / 32, H = DV / 64, LD = DV + 4;
-    __shared__ float sm_o[4][16][LD];
+    // a warp's output rows; before, a task's queries as each lane's fragments
+    // need them ([SEG][2][32] of 16 bytes, at its first warp's rows)
+    constexpr int WARP = 16 * LD > SEG * 256 ? 16 * LD : SEG * 256;
+    __shared__ __align__(16) float buf[4][WARP];
     __shared__ float2 sm_ml[4][16];
-    __shared__ uint4 sm_q[SEG][2][32];   // the queries, as each lane's fragments need them
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    const uint32_t split = blockIdx.x % own.splits, rt = blockIdx.x / own.splits % own.row_tiles;
-    const uint32_t h = blockIdx.x / own.splits / own.row_tiles, s = blockIdx.y;
+    const uint32_t all = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    float (*sm_o)[LD] = reinterpret_cast<float (*)[LD]>(buf[all]);
+    uint4 (*sm_q)[2][32] = reinterpret_cast<uint4 (*)[2][32]>(buf[all / W * W]);
+    const uint32_t warp = all % W, mine = all / W, task = blockIdx.x * (4 / W) + mine;   // warp of a task; task of the CTA
+    if (task >= own.tasks) return;   // a whole warp (W = 1); with W = 4 there is a CTA per task
+    auto sync = [&] {
+        if constexpr (W == 1) __syncwarp();
+        else __syncthreads();
+    };
+    const uint32_t split = task % own.splits, rt = task / own.splits % own.row_tiles;
+    const uint32_t h = task / own.splits / own.row_tiles, s = blockIdx.y;
     const uint32_t group = a.heads / a.kv_heads, rows = a.N * group;
     const int32_t len = own_rows(a, s);
-    const uint32_t keys = len < 0 ? 0u : static_cast<uint32_t>(len) + a.N;
     const float c = fabsf(a.scale) * kLog2e;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-    // this split's keys, in tiles of 16
-    const uint32_t tiles = (keys + 15) / 16;
-    const uint32_t k_end = min(keys, (split + 1) * ((tiles + own.splits - 1) / own.splits) * 16);
+    // this task's tiles of 16 keys: first the prefix's, where they are read
+    // here, then the sequence's own
+    const uint32_t pre = own.prefix && len >= 0 ? (a.prefix_len + 15) / 16 : 0;
+    const uint32_t tiles = len < 0 ? 0 : pre + (static_cast<uint32_t>(len) + a.N + 15) / 16;
+    const uint32_t per_split = (tiles + own.splits - 1) / own.splits, end = min(tiles, (split + 1) * per_split);
+    uint32_t tile = split * per_split + warp;
 
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4 kr[2][SEG], vr[4][H];
+    // this lane's pieces of the tile to load, taken along by pointers (an
+    // address from 64-bit strides costs a dozen instructions a load)
+    const uint32_t main_seg = a.main / 32;
+    const uint16_t *kp[2], *ep[2], *vp[4];
+    uint64_t k_step, e_step, v_step;
+    auto aim = [&](uint32_t i) {   // at tile i of its source
+        const KvSource& x = i < pre ? a.prefix : a.suffix;
+        const uint64_t seq = i < pre ? 0 : s, k0 = (i < pre ? i : i - pre) * 16ull;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint64_t key = k0 + 8 * e + g;
+            kp[e] = static_cast<const uint16_t*>(x.k) + seq * x.k_seq + h * x.k_head + key * x.k_row + t * 8;
+            ep[e] = static_cast<const uint16_t*>(x.extra) + seq * x.extra_seq + key * x.extra_row + t * 8 - a.main;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            vp[e] = static_cast<const uint16_t*>(x.v) + seq * x.v_seq + h * x.v_head + (k0 + 2 * t + (e & 1) + 8 * (e >> 1)) * x.v_row + g * 8;
+        k_step = 16 * W * x.k_row;
+        e_step = 16 * W * x.extra_row;
+        v_step = 16 * W * x.v_row;
+    };
+    // keys of tile i's source from its first one on
+    auto left = [&](uint32_t i) { return i < pre ? a.prefix_len - i * 16 : static_cast<uint32_t>(len) + a.N - (i - pre) * 16; };
+    auto load_k = [&](uint32_t n) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const bool in = 8 * x + g < n;
+#pragma unroll
+            for (int j = 0; j < SEG; ++j) {
+                const uint16_t* src = j < 2 || static_cast<uint32_t>(j) < main_seg ? kp[x] : ep[x];   // main_dim is 64 at least
+                kr[x][j] = in ? __ldg(reinterpret_cast<const uint4*>(src + j * 32)) : zero;
+            }
+        }
+    };
+    auto load_v = [&](uint32_t n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const bool in = 2 * t + (x & 1) + 8 * (x >> 1) < n;
+#pragma unroll
+            for (int j = 0; j < H; ++j) vr[x][j] = in ? __ldg(reinterpret_cast<const uint4*>(vp[x] + j * 64)) : zero;
+        }
+    };
+    auto advance = [&](uint32_t i) {   // from tile i - W to tile i
+        if (i >= pre && i - W < pre) {
+            aim(i);
+            return;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            kp[x] += k_step;
+            ep[x] += e_step;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vp[x] += v_step;
+    };
+    // the first tile's rows come while the queries do, a later one's while
+    // the tile before is worked on
+    if (tile < end) {
+        aim(tile);
+        load_k(left(tile));
+        load_v(left(tile));
+    }
     uint64_t seen[2];   // draft rows that rows g and g + 8 see
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -647,17 +735,13 @@ __global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_consta
         seen[i] = there ? a.ancestors[node] : 0;
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + (static_cast<size_t>(s) * a.N + node) * a.q_row +
                               static_cast<size_t>(h * group + r % group) * DQ + t * 8;
-        for (uint32_t j = warp; j < SEG; j += 4) {
-            uint4 w = make_uint4(0, 0, 0, 0);
+        for (uint32_t j = warp; j < SEG; j += W) {
+            uint4 w = zero;
             if (there) w = __ldg(reinterpret_cast<const uint4*>(src + j * 32));
             sm_q[j][i][lane] = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
         }
     }
-    __syncthreads();
-    const uint16_t* kp = static_cast<const uint16_t*>(a.suffix.k) + s * a.suffix.k_seq + h * a.suffix.k_head + t * 8;
-    const uint16_t* ep = static_cast<const uint16_t*>(a.suffix.extra) + s * a.suffix.extra_seq + t * 8;
-    const uint16_t* vp = static_cast<const uint16_t*>(a.suffix.v) + s * a.suffix.v_seq + h * a.suffix.v_head + g * 8;
-    const uint32_t main_seg = a.main / 32;
+    sync();
     float o[H][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int x = 0; x < H; ++x)
@@ -666,26 +750,9 @@ __global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_consta
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[x][j][e] = 0.0f;
 
-    for (uint32_t k0 = split * ((tiles + own.splits - 1) / own.splits) * 16 + 16 * warp; k0 < k_end; k0 += 64) {
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        uint4 kr[2][SEG], vr[4][H];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint64_t key = k0 + 8 * x + g;
-#pragma unroll
-            for (int j = 0; j < SEG; ++j) {
-                const uint16_t* src = static_cast<uint32_t>(j) < main_seg ? kp + key * a.suffix.k_row + j * 32
-                                                                        : ep + key * a.suffix.extra_row + (j - main_seg) * 32;
-                kr[x][j] = key < keys ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const uint64_t key = k0 + 2 * t + (x & 1) + 8 * (x >> 1);
-#pragma unroll
-            for (int j = 0; j < H; ++j)
-                vr[x][j] = key < keys ? __ldg(reinterpret_cast<const uint4*>(vp + key * a.suffix.v_row + j * 64)) : zero;
-        }
+    for (; tile < end; tile += W) {
+        const bool own_tile = tile >= pre, more = tile + W < end;
+        const uint32_t n = left(tile), k0 = own_tile ? (tile - pre) * 16 : 0;
         float sc[2][4] = {};
 #pragma unroll
         for (int j = 0; j < SEG; ++j) {
@@ -697,7 +764,12 @@ __global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_consta
                 mma16(sc[x], a1, kr[x][j].z, kr[x][j].w, BF16);
             }
         }
-        const bool drafts = k0 + 16 > static_cast<uint32_t>(len);
+        // the next tile's keys; its values when this one's are used
+        if (more) {
+            advance(tile + W);
+            load_k(left(tile + W));
+        }
+        const bool drafts = own_tile && k0 + 16 > static_cast<uint32_t>(len);
         uint32_t vis = 0xffu;   // bit 4 x + e: key of sc[x][e] is visible to its row
         if (drafts) {
             vis = 0;
@@ -705,11 +777,17 @@ __global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_consta
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t key = k0 + 8 * x + 2 * t + (e & 1);
-                    const bool see = key < static_cast<uint32_t>(len) || (key < keys && (seen[e >> 1] >> (key - len) & 1u));
+                    const uint32_t at = 8 * x + 2 * t + (e & 1), key = k0 + at;
+                    const bool see = key < static_cast<uint32_t>(len) || (at < n && (seen[e >> 1] >> (key - len) & 1u));
                     if (see) vis |= 1u << (4 * x + e);
                     else sc[x][e] = -INFINITY;
                 }
+        } else if (n < 16) {   // the prefix's last tile
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (8 * x + 2 * t + (e & 1) >= n) sc[x][e] = -INFINITY;
         }
         float top[2];
 #pragma unroll
@@ -754,7 +832,7 @@ __global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_consta
         if (drafts && __any_sync(0xffffffffu, odd_values)) {
             // one key at a time: its probabilities from the lane that has
             // them, its values from memory
-            for (uint32_t kk = 0; kk < 16 && k0 + kk < keys; ++kk) {
+            for (uint32_t kk = 0; kk < min(16u, n); ++kk) {
                 const uint32_t src = (lane & ~3u) | (kk % 8 / 2), bit = 4 * (kk / 8) + kk % 2;
                 const uint32_t sv = __shfl_sync(0xffffffffu, vis, src);
                 float pk[2];
@@ -790,63 +868,93 @@ __global__ void __launch_bounds__(kOwnThreads, 3) own_kernel(const __grid_consta
                 mma16(o[x][j], pa, __byte_perm(v0[j / 2], v1[j / 2], pick), __byte_perm(v2[j / 2], v3[j / 2], pick), BF16);
             }
         }
+        if (more) load_v(left(tile + W));
     }
-    // the four warps' results, then the row's parts
+    // the task's results to rows of lanes, then the rows' parts
+    sync();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t == 0) sm_ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+        if (t == 0) sm_ml[all][g + 8 * i] = make_float2(m[i], l[i]);
 #pragma unroll
         for (int x = 0; x < H; ++x)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int j = 0; j < 8; j += 4)
-                    *reinterpret_cast<float4*>(&sm_o[warp][g + 8 * i][x * 64 + (2 * t + e) * 8 + j]) =
+                    *reinterpret_cast<float4*>(&sm_o[g + 8 * i][x * 64 + (2 * t + e) * 8 + j]) =
                         make_float4(o[x][j][2 * i + e], o[x][j + 1][2 * i + e], o[x][j + 2][2 * i + e], o[x][j + 3][2 * i + e]);
     }
-    __syncthreads();
-    constexpr int C = DV / 8;
-    const uint32_t row = threadIdx.x / 8, col = threadIdx.x % 8 * C, r = rt * 16 + row;
-    Join<C> j;
-    for (int w = 0; w < 4; ++w) j.add(sm_ml[w][row], &sm_o[w][row][col]);
-    if (own.splits > 1) {
-        const size_t at = (((static_cast<size_t>(s) * a.kv_heads + h) * own.row_tiles + rt) * own.splits + split) * 16 + row;
-        if (col == 0) own.ml[at] = make_float2(j.m, j.l);
+    sync();
+    constexpr int C = DV / 32;
+    const uint32_t col = lane * C, here = min(16u, rows - rt * 16);
+    if (own.splits == 1 && p.total) asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t row = 2 * warp; row < here; row += 2 * W) {   // two rows at a time
+        Join<C> j[2];
+        const bool there[2] = {true, row + 1 < here};
 #pragma unroll
-        for (int i = 0; i < C; i += 4)
-            *reinterpret_cast<float4*>(own.o + at * DV + col + i) = make_float4(j.o[i], j.o[i + 1], j.o[i + 2], j.o[i + 3]);
-        return;
+        for (uint32_t i = 0; i < 2; ++i) {
+            if (!there[i]) continue;
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) {
+                float x[C];
+                load_cols<C>(&buf[mine * W + w][(row + i) * LD + col], x);
+                j[i].add(sm_ml[mine * W + w][row + i], x);
+            }
+            if (own.splits == 1) continue;
+            const size_t at = (static_cast<size_t>(s) * own.tasks + task) * 16 + row + i;
+            if (lane == 0) own.ml[at] = make_float2(j[i].m, j[i].l);
+#pragma unroll
+            for (int e = 0; e < C; ++e) own.o[at * DV + col + e] = j[i].o[e];
+        }
+        if (own.splits > 1) continue;
+        const uint32_t r[2] = {rt * 16 + row, rt * 16 + row + there[1]};
+        if (p.total && len >= 0) join_prefix<C>(j, p, parts, h, {s * rows + r[0], s * rows + r[1]}, there, col, DV);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i)
+            if (there[i]) write_row<BF16>(a, j[i], s, r[i] / group, h * group + r[i] % group, col);
     }
-    if (p.total) asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (r >= rows) return;
-    if (len >= 0) join_prefix(j, p, parts, h, (s * a.N) * group + r, col, DV);
-    write_row<BF16>(a, j, s, r / group, h * group + r % group, col);
 }
 
-// The join on its own, where own_kernel split the keys.
+// The join on its own, where own_kernel split the keys: a warp per two rows.
 template <int DV, bool BF16>
 __global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
                                                            const Parts parts, const OwnPlan own) {
-    constexpr int C = DV / 8;
+    constexpr int C = DV / 32;
     const uint32_t rt = blockIdx.x % own.row_tiles, h = blockIdx.x / own.row_tiles, s = blockIdx.y;
     const uint32_t group = a.heads / a.kv_heads, rows = a.N * group;
-    const uint32_t row = threadIdx.x / 8, col = threadIdx.x % 8 * C, r = rt * 16 + row;
-    if (r >= rows) return;
-    Join<C> j;
-    if (own_rows(a, s) >= 0) {
-        const size_t at = ((static_cast<size_t>(s) * a.kv_heads + h) * own.row_tiles + rt) * own.splits * 16 + row;
-        for (uint32_t i = 0; i < own.splits; ++i) j.add(own.ml[at + 16 * i], own.o + (at + 16 * i) * DV + col);
-        join_prefix(j, p, parts, h, (s * a.N) * group + r, col, DV);
+    const uint32_t col = threadIdx.x % 32 * C, here = min(16u, rows - rt * 16);
+    const int32_t len = own_rows(a, s);
+    for (uint32_t row = threadIdx.x / 32 * 2; row < here; row += 8) {
+        Join<C> j[2];
+        const bool there[2] = {true, row + 1 < here};
+        const uint32_t r[2] = {rt * 16 + row, rt * 16 + row + there[1]};
+        if (len >= 0) {
+            const size_t at = (static_cast<size_t>(s) * own.tasks + blockIdx.x * own.splits) * 16 + row;
+#pragma unroll 4
+            for (uint32_t k = 0; k < own.splits; ++k)
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i)
+                    if (there[i]) {
+                        float x[C];
+                        load_cols<C>(own.o + (at + 16 * k + i) * DV + col, x);
+                        j[i].add(own.ml[at + 16 * k + i], x);
+                    }
+            if (p.total) join_prefix<C>(j, p, parts, h, {s * rows + r[0], s * rows + r[1]}, there, col, DV);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i)
+            if (there[i]) write_row<BF16>(a, j[i], s, r[i] / group, h * group + r[i] % group, col);
     }
-    write_row<BF16>(a, j, s, r / group, h * group + r % group, col);
 }
 
 template <int DQ, int DV, bool BF16>
 int launch_own(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.kv_heads * own.row_tiles * own.splits, a.S);
+    // a warp per task from three rounds of the GPU's warps on
+    const bool many = static_cast<uint64_t>(own.tasks) * a.S >= 8ull * ctx->sm_count;
+    cfg.gridDim = dim3(many ? (own.tasks + 3) / 4 : own.tasks, a.S);
     cfg.blockDim = dim3(kOwnThreads);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr{};
@@ -856,7 +964,8 @@ int launch_own(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Part
     // beside the prefix kernel's tail (it waits there before it joins); a
     // split launch leaves the join, and the wait, to join_kernel
     cfg.numAttrs = p.total && own.splits == 1 ? 1 : 0;
-    K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16>, a, p, parts, own));
+    if (many) K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16, 1>, a, p, parts, own));
+    else K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16, 4>, a, p, parts, own));
     ++ctx->stats.kernel_launches;
     if (own.splits > 1) {
         join_kernel<DV, BF16><<<dim3(a.kv_heads * own.row_tiles, a.S), kOwnThreads, 0, ctx->stream>>>(a, p, parts, own);
@@ -883,7 +992,7 @@ int launch_both(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Par
         map_e = map_k;
         if (a.extra && (st = make_row_map(ctx, &map_e, x.extra, 2ull * a.extra, 1, a.prefix_len, 2 * x.extra_row, 2 * x.extra_row, kTile)))
             return st;
-        prefix_kernel<BF16, NK, NV><<<p.ctas, kPrefixThreads, prefix_smem(NK), ctx->stream>>>(map_k, map_e, map_v, a, p, parts);
+        prefix_kernel<BF16, NK, NV><<<(p.total + p.range - 1) / p.range, kPrefixThreads, prefix_smem(NK), ctx->stream>>>(map_k, map_e, map_v, a, p, parts);
         K3XB_LAUNCHED(ctx);
     }
     return launch_own<64 * NK, 64 * NV, BF16>(ctx, a, p, parts, own);
@@ -928,28 +1037,38 @@ int launch_attend_tc(k3xb_ctx* ctx, const AttnArgs& a, bool bf16) {
     p.rows = a.S * a.N * group;
     p.group = group;
     p.blocks = static_cast<uint32_t>((static_cast<uint64_t>(a.prefix_len) + kTile - 1) / kTile);
+    OwnPlan own{};
+    own.row_tiles = (a.N * group + 15) / 16;
+    // One sequence shares its prefix with nobody: its few rows read it with
+    // their own (32 heads, one token after 700: 25 -> 13 us; the first kernel
+    // alone takes 12).
+    own.prefix = a.S == 1 && own.row_tiles <= 4;
     const uint32_t tiles = (p.rows + kTile - 1) / kTile;
     p.pairs = tiles / 2;
     p.odd = tiles % 2;
     const uint64_t per_head = static_cast<uint64_t>(p.pairs) * p.blocks + p.odd * ((p.blocks + 1) / 2);
-    if (per_head >= (1ull << 31)) return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: rows times prefix too large");
+    if (per_head * a.kv_heads >= (1ull << 31)) return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: rows times prefix too large");
     p.steps_per_head = static_cast<uint32_t>(per_head);
-    p.total = per_head * a.kv_heads;
+    p.total = own.prefix ? 0 : p.steps_per_head * a.kv_heads;
+    uint32_t ctas = 0;
     if (p.total) {
-        p.ctas = static_cast<uint32_t>(std::min<uint64_t>(sms, p.total));
-        const uint64_t range = (p.total + p.ctas - 1) / p.ctas;
-        p.max_seg = static_cast<uint32_t>(range / (p.odd ? (p.blocks + 1) / 2 : p.blocks) + 2);
+        p.range = (p.total + sms - 1) / sms;
+        ctas = (p.total + p.range - 1) / p.range;
+        p.max_seg = p.range / (p.odd ? (p.blocks + 1) / 2 : p.blocks) + 2;
     }
-    OwnPlan own{};
-    own.row_tiles = (a.N * group + 15) / 16;
-    // Enough CTAs for two per SM; a split has 256 cache rows at least
-    // (by the capacity: lengths are on the device).
-    const uint64_t ctas = static_cast<uint64_t>(a.S) * a.kv_heads * own.row_tiles;
-    own.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((2 * sms + ctas - 1) / ctas, a.capacity / 256)));
+    // Tasks for the GPU's warps three times over (twelve per SM), since
+    // sequences are of unlike lengths; a split has 256 cache rows at least (by
+    // the capacity: lengths are on the device), or 64 where latency counts.
+    const uint64_t whole = static_cast<uint64_t>(a.S) * a.kv_heads * own.row_tiles;
+    const uint64_t rows_read = a.capacity + (own.prefix ? static_cast<uint64_t>(a.prefix_len) : 0), least = own.prefix ? 64 : 256;
+    own.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((36 * sms + whole - 1) / whole, rows_read / least)));
+    if (static_cast<uint64_t>(a.kv_heads) * own.row_tiles * own.splits >= (1ull << 31))
+        return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: too many rows per sequence");
+    own.tasks = a.kv_heads * own.row_tiles * own.splits;
     Parts parts{};
     auto carve = [&](auto& c) {
-        const size_t n = static_cast<size_t>(p.total ? p.ctas : 0) * p.max_seg * 2 * kTile;
-        const size_t k = own.splits > 1 ? static_cast<size_t>(ctas) * own.splits * 16 : 0;
+        const size_t n = static_cast<size_t>(ctas) * p.max_seg * 2 * kTile;
+        const size_t k = own.splits > 1 ? static_cast<size_t>(own.tasks) * a.S * 16 : 0;
         parts.o = c.template take<float>(n * a.value);
         parts.ml = c.template take<float2>(n);
         own.o = c.template take<float>(k * a.value);

@@ -6,8 +6,10 @@ library or a B200 is missing, every entry point raises K3xbError.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libk3xb.so")
@@ -194,7 +196,7 @@ def library() -> C.CDLL:
             "k3xb_kda_commit": [vp, vp, vp, u32, u32, u32, u32, vp, vp, vp, vp, vp, vp, vp],
             "k3xb_kda_prefill": [vp, vp, vp, vp, u64, C.c_int32, vp, vp, vp, u32, u32, u32, u32, vp, vp, vp],
             "k3xb_kda_step": [vp, vp, vp, vp, u64, C.c_int32, vp, vp, u32, u32, u32, vp, u32, vp, vp],
-            "k3xb_prefix_attention": [vp, C.POINTER(PrefixAttentionIO)],
+            "k3xb_prefix_attention": [vp, vp],
             "k3xb_accept_greedy": [vp, vp, vp, u32, u32, u32, vp, vp, vp, vp],
             "k3xb_accept_rejection": [vp, vp, vp, vp, u32, u32, u32, f32, u64, u64, vp, vp, vp],
             "k3xb_fill_normal_f32": [vp, vp, sz, u64, u64, f32, f32],
@@ -264,14 +266,14 @@ def _p(t):
     return C.c_void_p(t.data_ptr())
 
 
-def _a(t, dtype, shape, name):
-    """Address of a contiguous CUDA tensor of this type and shape (None ->
-    NULL)."""
+def _a(t, dtype, shape, device, name):
+    """Address of a contiguous tensor of this type and shape on this GPU
+    (None -> NULL)."""
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda:
-        raise K3xbError(INVALID_EXTENT, f"{name}: expected a contiguous CUDA tensor {dtype} {shape}, got {t.dtype} "
-                                        f"{tuple(t.shape)}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise K3xbError(INVALID_EXTENT, f"{name}: expected a contiguous tensor {dtype} {tuple(shape)} on GPU {device}, got "
+                                        f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -279,13 +281,19 @@ _TYPES = {}
 
 
 def _type(t, name):
-    """K3XB_TYPE_* of a CUDA tensor."""
+    """K3XB_TYPE_* of a tensor."""
     if not _TYPES:
         import torch
         _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16})
-    if t.dtype not in _TYPES or not t.is_cuda:
-        raise K3xbError(INVALID_EXTENT, f"{name}: expected a CUDA tensor of float32, bfloat16 or float16")
-    return _TYPES[t.dtype]
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise K3xbError(INVALID_EXTENT, f"{name}: expected float32, bfloat16 or float16")
+    return kind
+
+
+# PrefixAttentionIO as one packing: a call fills some forty fields
+_IO = struct.Struct("@7Iif4xQQQ" + "QQQ8QI4x" * 2 + "QQQ")
+_NO_ROWS = (0,) * 12
 
 
 class Context:
@@ -384,66 +392,76 @@ class Context:
                                              _p(log_decay), _p(beta), com, _p(state_out)), "kda_commit")
 
     def _kda_rows(self, q, k, v, log_decay, beta, out):
-        """Checks shared by kda_prefill and kda_step; returns (tokens, heads,
-        head_dim, row_stride, type)."""
-        import torch
-        if q.dim() != 2 or beta.dim() != 2 or not beta.shape[1] or q.shape[1] % beta.shape[1]:
+        """Checks shared by kda_prefill and kda_step; returns the call's
+        arguments up to beta, and out, tokens, heads and head_dim."""
+        if q.dim() != 2 or beta.dim() != 2:
             raise K3xbError(INVALID_EXTENT, "q must be [tokens][heads * head_dim] and beta [tokens][heads]")
-        (T, P), h = q.shape, beta.shape[1]
-        kind, stride = _type(q, "q"), q.stride(0) if T > 1 else P
-        for t in (q, k, v):
-            if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device or t.stride(1) != 1 or (
-                    T > 1 and t.stride(0) != stride):
+        shape, strides, dtype, device = q.shape, q.stride(), q.dtype, self.device
+        T, P = shape
+        h = beta.shape[1]
+        if not h or P % h or q.get_device() != device or strides[1] != 1:
+            raise K3xbError(INVALID_EXTENT, f"q must be [tokens][heads * head_dim] rows on GPU {device}")
+        for t in (k, v):
+            if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (t.stride() != strides and T > 1):
                 raise K3xbError(INVALID_EXTENT, "q, k and v must be rows of one shape, type and row stride")
-        f32 = torch.float32
-        return T, h, P // h, stride, kind, _a(log_decay, f32, (T, P), "log_decay"), _a(beta, f32, (T, h), "beta"), _a(
-            out, q.dtype, (T, P), "out")
+        f32 = beta.dtype
+        if _type(beta, "beta") != TYPE_F32:
+            raise K3xbError(INVALID_EXTENT, "beta must be float32")
+        return (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides[0] if T > 1 else P, _type(q, "q"),
+                _a(log_decay, f32, shape, device, "log_decay"), _a(beta, f32, (T, h), device, "beta")), _a(
+                    out, dtype, shape, device, "out"), T, h, P // h
 
     def kda_prefill(self, q, k, v, log_decay, beta, offsets, out, state=None, state_out=None):
         """The gated delta rule over packed prompts: q/k/v [tokens][h*d] (rows
         may be strided alike), log_decay [tokens][h*d], beta [tokens][h],
         offsets [S+1] int32 on the device, out [tokens][h*d]; state and
         state_out [S][h][d][d] (None: zeros / not kept; may be one tensor)."""
-        import torch
-        T, h, d, stride, kind, ld, be, o = self._kda_rows(q, k, v, log_decay, beta, out)
+        rows, o, T, h, d = self._kda_rows(q, k, v, log_decay, beta, out)
         S = offsets.shape[0] - 1
-        self._check(self.lib.k3xb_kda_prefill(
-            self.h, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride, kind, ld, be,
-            _a(offsets, torch.int32, (S + 1,), "offsets"), S, T, h, d,
-            _a(state, torch.float32, (S, h, d, d), "state"), _a(state_out, torch.float32, (S, h, d, d), "state_out"), o),
-            "kda_prefill")
+        if offsets.element_size() != 4 or offsets.is_floating_point():
+            raise K3xbError(INVALID_EXTENT, "offsets must be int32")
+        st = self.lib.k3xb_kda_prefill(
+            self.h, *rows, _a(offsets, offsets.dtype, (S + 1,), self.device, "offsets"), S, T, h, d,
+            _a(state, beta.dtype, (S, h, d, d), self.device, "state"),
+            _a(state_out, beta.dtype, (S, h, d, d), self.device, "state_out"), o)
+        if st:
+            self._check(st, "kda_prefill")
 
     def kda_step(self, q, k, v, log_decay, beta, state, out, slots=None):
         """One token of each sequence, its state advanced in place: q/k/v
         [S][h*d], state [states][h][d][d]; slots [S] int32 (None: state s;
         negative: idle)."""
-        import torch
-        S, h, d, stride, kind, ld, be, o = self._kda_rows(q, k, v, log_decay, beta, out)
+        rows, o, S, h, d = self._kda_rows(q, k, v, log_decay, beta, out)
         states = state.shape[0]
-        self._check(self.lib.k3xb_kda_step(
-            self.h, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride, kind, ld, be, S, h, d,
-            _a(slots, torch.int32, (S,), "slots"), states, _a(state, torch.float32, (states, h, d, d), "state"), o),
-            "kda_step")
+        if slots is not None and (slots.element_size() != 4 or slots.is_floating_point()):
+            raise K3xbError(INVALID_EXTENT, "slots must be int32")
+        st = self.lib.k3xb_kda_step(
+            self.h, *rows, S, h, d, None if slots is None else _a(slots, slots.dtype, (S,), self.device, "slots"), states,
+            _a(state, beta.dtype, (states, h, d, d), self.device, "state"), o)
+        if st:
+            self._check(st, "kda_step")
 
     @staticmethod
-    def _kv_rows(k, v, extra, sequences, kv_heads, main, value, extra_dim, dtype):
-        """KvRows of [rows][kv_heads][dim] tensors (sequences None) or of
-        [S][rows][kv_heads][dim] ones; any strides with a contiguous last
-        dimension."""
+    def _kv_rows(k, v, extra, lead, kv_heads, main, value, extra_dim, dtype, device):
+        """The fields of KvRows for [*lead][rows][kv_heads][dim] tensors (lead
+        (S,) or ()); any strides with a contiguous last dimension."""
         if k is None or not k.numel():
-            return KvRows()
-        lead = () if sequences is None else (sequences,)
+            return _NO_ROWS
         rows = k.shape[len(lead)]
-        for t, want, name in ((k, (*lead, rows, kv_heads, main), "k"), (v, (*lead, rows, kv_heads, value), "v"),
-                              (extra, (*lead, rows, extra_dim), "extra")):
-            if t is None and not extra_dim and name == "extra":
-                continue
-            if t is None or tuple(t.shape) != want or t.dtype != dtype or not t.is_cuda or t.stride(-1) != 1:
-                raise K3xbError(INVALID_EXTENT, f"cache {name}: expected {want} of {dtype} on the GPU with a contiguous "
-                                                "last dimension")
-        ks, vs, es = k.stride(), v.stride(), (0,) * (len(lead) + 2) if extra is None else extra.stride()
-        return KvRows(k.data_ptr(), v.data_ptr(), None if extra is None else extra.data_ptr(), ks[-3], ks[-2],
-                      ks[0] if lead else 0, vs[-3], vs[-2], vs[0] if lead else 0, es[-2], es[0] if lead else 0, rows)
+        ks, vs = k.stride(), v.stride()
+        bad = (k.shape != (*lead, rows, kv_heads, main) or v.shape != (*lead, rows, kv_heads, value) or k.dtype is not dtype or
+               v.dtype is not dtype or k.get_device() != device or v.get_device() != device or ks[-1] != 1 or vs[-1] != 1)
+        ep = er = eq = 0
+        if extra_dim:
+            bad = bad or extra is None
+            if not bad:
+                es = extra.stride()
+                bad = extra.shape != (*lead, rows, extra_dim) or extra.dtype is not dtype or extra.get_device() != device or es[-1] != 1
+                ep, er, eq = extra.data_ptr(), es[-2], es[0] if lead else 0
+        if bad:
+            raise K3xbError(INVALID_EXTENT, f"cache: expected rows of {kv_heads} heads of {main}, {value} and a part of {extra_dim} "
+                                            f"in {dtype} on GPU {device}, contiguous in the last dimension")
+        return (k.data_ptr(), v.data_ptr(), ep, ks[-3], ks[-2], ks[0] if lead else 0, vs[-3], vs[-2], vs[0] if lead else 0, er, eq, rows)
 
     def prefix_attention(self, q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_len, parent, out, prefix_extra=None,
                          suffix_extra=None, lse=None, scale=None):
@@ -452,23 +470,26 @@ class Context:
         [rows][kv_heads][dim] / [rows][extra] (None or empty: no prefix);
         suffix_k/_v/_extra [S][capacity][kv_heads][dim] / [S][capacity][extra];
         suffix_len [S] int32 on the device; parent [N] on the host; out
-        [S][N][heads][value]; lse [S][N][heads] or None; scale default
+        [S][N][heads][value]; lse [S][N][heads] float32 or None; scale default
         1 / sqrt(main + extra)."""
-        import torch
         S, N, heads, width = q.shape
-        kv_heads, main, value = suffix_k.shape[2], suffix_k.shape[3], suffix_v.shape[3]
-        extra = width - main
-        if not q.is_contiguous() or extra < 0 or len(parent) != N:
-            raise K3xbError(INVALID_EXTENT, "q must be contiguous, as wide as a key, with one parent per node")
-        par = (C.c_int32 * N)(*parent)
-        io = PrefixAttentionIO(
+        _, _, kv_heads, main = suffix_k.shape
+        value, extra, dtype, device = suffix_v.shape[3], width - main, q.dtype, self.device
+        if not q.is_contiguous() or q.get_device() != device or extra < 0 or len(parent) != N:
+            raise K3xbError(INVALID_EXTENT, f"q must be contiguous on GPU {device}, as wide as a key, with one parent per node")
+        if suffix_len.element_size() != 4 or suffix_len.is_floating_point() or (lse is not None and _type(lse, "lse") != TYPE_F32):
+            raise K3xbError(INVALID_EXTENT, "suffix_len must be int32 and lse float32")
+        par = array.array("i", parent)
+        io = _IO.pack(
             S, N, heads, kv_heads, main, extra, value, _type(q, "q"), width ** -0.5 if scale is None else scale,
-            C.addressof(par), q.data_ptr(), 0,
-            self._kv_rows(prefix_k, prefix_v, prefix_extra, None, kv_heads, main, value, extra, q.dtype),
-            self._kv_rows(suffix_k, suffix_v, suffix_extra, S, kv_heads, main, value, extra, q.dtype),
-            _a(suffix_len, torch.int32, (S,), "suffix_len"), _a(out, q.dtype, (S, N, heads, value), "out"),
-            _a(lse, torch.float32, (S, N, heads), "lse"))
-        self._check(self.lib.k3xb_prefix_attention(self.h, C.byref(io)), "prefix_attention")
+            par.buffer_info()[0], q.data_ptr(), 0,
+            *self._kv_rows(prefix_k, prefix_v, prefix_extra, (), kv_heads, main, value, extra, dtype, device),
+            *self._kv_rows(suffix_k, suffix_v, suffix_extra, (S,), kv_heads, main, value, extra, dtype, device),
+            _a(suffix_len, suffix_len.dtype, (S,), device, "suffix_len"), _a(out, dtype, (S, N, heads, value), device, "out"),
+            0 if lse is None else _a(lse, lse.dtype, (S, N, heads), device, "lse"))
+        st = self.lib.k3xb_prefix_attention(self.h, io)
+        if st:
+            self._check(st, "prefix_attention")
 
     def select_routing(self, scores, bias, natural_k, ids, weights, selected, escalated=None, stats=None,
                        mode=ROUTING_NATURAL, fixed_k=0, mass_target=0.9, minimum_gap=0.0, quality_floor_k=0):

@@ -5,6 +5,7 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+import types
 
 import pytest
 
@@ -31,6 +32,7 @@ def test_struct_layout_is_the_headers(tmp_path):
         want.append(C.sizeof(cls))
         want += [getattr(cls, f[0]).offset for f in cls._fields_]
     assert got == want
+    assert k3xb._IO.size == C.sizeof(k3xb.PrefixAttentionIO)
 
 
 def test_null_context_is_refused():
@@ -47,9 +49,9 @@ def test_host_tensors_are_refused():
     import k3xb
     q = torch.zeros(2, 64)
     with pytest.raises(k3xb.K3xbError) as e:
-        k3xb.Context._kda_rows(None, q, q, q, q, torch.zeros(2, 1), q)
+        k3xb.Context._kda_rows(types.SimpleNamespace(device=0), q, q, q, q, torch.zeros(2, 1), q)
     assert e.value.status == k3xb.INVALID_EXTENT
     k = torch.zeros(1, 4, 2, 64)
     with pytest.raises(k3xb.K3xbError) as e:
-        k3xb.Context._kv_rows(k, k, None, 1, 2, 64, 64, 0, torch.float32)
+        k3xb.Context._kv_rows(k, k, None, (1,), 2, 64, 64, 0, torch.float32, 0)
     assert e.value.status == k3xb.INVALID_EXTENT
