@@ -567,8 +567,9 @@ int k3xb_kda_step(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
  * kv_heads heads, a key k[s*k_seq + p*k_row + head*k_head ..+main_dim] and a
  * value v[..+value_dim], and one extra[s*extra_seq + p*extra_row ..+extra_dim]
  * that the heads share (the q_extra part of the gated MLA layer, model.cpp:
- * 755-811). Strides in elements; 0: packed [seq][rows][kv_heads][dim]. Any
- * order of rows and heads is allowed. */
+ * 755-811). Strides in elements, in any order of rows and heads, 0 where a
+ * row, head or sequence is broadcast; all eight 0: packed
+ * [seq][rows][kv_heads][dim]. */
 typedef struct {
     const void *k, *v, *extra;     /* extra: NULL when extra_dim is 0 */
     uint64_t k_row, k_head, k_seq, v_row, v_head, v_seq, extra_row, extra_seq;

@@ -119,18 +119,25 @@ int launch_rows(k3xb_ctx* ctx, const AttnArgs& a) {
     return K3XB_OK;
 }
 
-// A source's strides with the packed ones filled in ([seq][row][head][dim]);
-// a stride over a single row or head is never used.
-KvSource source_of(const k3xb_kv_rows& r, const AttnArgs& a) {
+// A source's strides; all zero: packed [seq][row][head][dim]. A stride over a
+// single row, head or sequence is never used, so it gets the packed value.
+KvSource source_of(const k3xb_kv_rows& r, const AttnArgs& a, uint32_t sequences) {
     KvSource s{r.k, r.v, r.extra, r.k_row, r.k_head, r.k_seq, r.v_row, r.v_head, r.v_seq, r.extra_row, r.extra_seq};
-    if (!s.k_head || a.kv_heads == 1) s.k_head = a.main;
-    if (!s.v_head || a.kv_heads == 1) s.v_head = a.value;
-    if (!s.k_row) s.k_row = static_cast<uint64_t>(a.kv_heads) * a.main;
-    if (!s.v_row) s.v_row = static_cast<uint64_t>(a.kv_heads) * a.value;
-    if (!s.extra_row) s.extra_row = a.extra;
-    if (!s.k_seq) s.k_seq = r.rows * s.k_row;
-    if (!s.v_seq) s.v_seq = r.rows * s.v_row;
-    if (!s.extra_seq) s.extra_seq = r.rows * s.extra_row;
+    const bool packed = !(r.k_row | r.k_head | r.k_seq | r.v_row | r.v_head | r.v_seq | r.extra_row | r.extra_seq);
+    if (packed || a.kv_heads == 1) {
+        s.k_head = a.main;
+        s.v_head = a.value;
+    }
+    if (packed || r.rows == 1) {
+        s.k_row = static_cast<uint64_t>(a.kv_heads) * a.main;
+        s.v_row = static_cast<uint64_t>(a.kv_heads) * a.value;
+        s.extra_row = a.extra;
+    }
+    if (packed || sequences == 1) {
+        s.k_seq = r.rows * s.k_row;
+        s.v_seq = r.rows * s.v_row;
+        s.extra_seq = r.rows * s.extra_row;
+    }
     return s;
 }
 
@@ -167,8 +174,8 @@ extern "C" int k3xb_prefix_attention(k3xb_ctx* ctx, const k3xb_prefix_attention_
     a.q_row = io->q_row ? io->q_row : static_cast<uint64_t>(a.heads) * (a.main + a.extra);
     a.prefix_len = io->prefix.rows;
     a.capacity = io->suffix.rows;
-    a.prefix = source_of(io->prefix, a);
-    a.suffix = source_of(io->suffix, a);
+    a.prefix = source_of(io->prefix, a, 1);
+    a.suffix = source_of(io->suffix, a, a.S);
     a.suffix_len = io->suffix_len;
     a.q = io->q;
     a.out = io->out;

@@ -1027,6 +1027,9 @@ bool attend_tc_takes(const AttnArgs& a, int32_t type) {
         ok = ok && whole16(x->k, {x->k_row, x->k_head, x->k_seq}) && whole16(x->v, {x->v_row, x->v_head, x->v_seq}) &&
              (!a.extra || whole16(x->extra, {x->extra_row, x->extra_seq}));
     }
+    // a tensor map steps over no zero stride (a broadcast prefix)
+    if (a.prefix_len)
+        ok = ok && a.prefix.k_row && a.prefix.k_head && a.prefix.v_row && a.prefix.v_head && (!a.extra || a.prefix.extra_row);
     // masked scores are -inf times the scale, and row indices of a kv head 32-bit
     return ok && a.scale != 0.0f && static_cast<uint64_t>(a.S) * a.N * (a.heads / a.kv_heads) < (1ull << 31);
 }

@@ -399,8 +399,8 @@ class Context:
         shape, strides, dtype, device = q.shape, q.stride(), q.dtype, self.device
         T, P = shape
         h = beta.shape[1]
-        if not h or P % h or q.get_device() != device or strides[1] != 1:
-            raise K3xbError(INVALID_EXTENT, f"q must be [tokens][heads * head_dim] rows on GPU {device}")
+        if not h or P % h or q.get_device() != device or strides[1] != 1 or (T > 1 and strides[0] < P):
+            raise K3xbError(INVALID_EXTENT, f"q must be [tokens][heads * head_dim] rows on GPU {device} that do not overlap")
         for t in (k, v):
             if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (t.stride() != strides and T > 1):
                 raise K3xbError(INVALID_EXTENT, "q, k and v must be rows of one shape, type and row stride")
@@ -458,6 +458,8 @@ class Context:
                 es = extra.stride()
                 bad = extra.shape != (*lead, rows, extra_dim) or extra.dtype is not dtype or extra.get_device() != device or es[-1] != 1
                 ep, er, eq = extra.data_ptr(), es[-2], es[0] if lead else 0
+        if not (any(ks[:-1]) or any(vs[:-1]) or er or eq):   # the C call reads all zeros as packed
+            bad = True
         if bad:
             raise K3xbError(INVALID_EXTENT, f"cache: expected rows of {kv_heads} heads of {main}, {value} and a part of {extra_dim} "
                                             f"in {dtype} on GPU {device}, contiguous in the last dimension")

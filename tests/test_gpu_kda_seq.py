@@ -309,6 +309,7 @@ def test_refusals(torch, ctx):
         lambda: ctx.kda_prefill(*x, off, out.bfloat16()),                                        # out of another type
         lambda: ctx.kda_prefill(*(t.half() for t in x[:3]), *x[3:], off, out.half()),             # f16
         lambda: ctx.kda_prefill(x[0], x[1][:3], *x[2:], off, out),
+        lambda: ctx.kda_prefill(*(t[:1].expand_as(t) for t in x[:3]), *x[3:], off, out),          # one row for all tokens
         lambda: ctx.kda_prefill(*x, off[:1], out),                                               # no sequence
         lambda: ctx.kda_step(*x, state[:2], out),                                                # fewer states than rows
         lambda: ctx.kda_step(*x, state.double(), out),

@@ -237,6 +237,30 @@ def test_cache_orders(torch, ctx, order):
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("S", [1, 5])
+def test_broadcast_caches(torch, ctx, S):
+    """One cache for all sequences, one head's rows for all heads, one row for
+    all positions: zero strides are taken as they are."""
+    N, heads = 2, 4
+    c = _case(torch, S, N, heads, heads, 128, 64, 128, 70, [9] * S, "bfloat16", 950)
+    for src in ("prefix", "suffix"):
+        lead = [] if src == "prefix" else [slice(None)]
+        for which in ("cache", "heads", "rows"):
+            d = dict(c)
+            for n in ("_k", "_v", "_extra"):
+                t = c[src + n]
+                if which == "cache":
+                    if src == "prefix":
+                        continue
+                    d[src + n] = t[:1].expand_as(t)
+                elif which == "heads":
+                    if n != "_extra":
+                        d[src + n] = t[..., :1, :].expand_as(t)
+                else:
+                    d[src + n] = t[tuple(lead + [slice(0, 1)])].expand_as(t)
+            _check(torch, ctx, d, _chain(N))
+
+
 def test_offsets_past_32_bits(torch, ctx):
     """A prefix of more than 2^31 key elements whose last rows decide."""
     rows, heads = 530000, 32
