@@ -626,22 +626,48 @@ __device__ __forceinline__ void split_rows(const float (&x)[4], const float (&y)
     split_pair(make_float2(y[0], y[1]), hi[2], lo[2]);
     split_pair(make_float2(y[2], y[3]), hi[3], lo[3]);
 }
-struct ScanBars {
+template <int D, int NW, int KS>
+struct __align__(128) ScanSmem {
+    ChunkStage<D> stage[kStages];
+    // odd and even chunks, row group, half, what (W S0^T, Q S0^T), token tile: a lane's sums
+    float4 part[2][KS > 1 ? NW : 1][KS][2][2][32];
     uint64_t full[kStages], empty[kStages];
     int abort;
 };
-template <int D>
-constexpr size_t scan_smem() { return kStages * sizeof(ChunkStage<D>) + sizeof(ScanBars); }
 
-// NW warps of 16 value rows of one head, and a warp that copies the operands.
-template <int D, int NW, int PER_SM, typename E>
-__global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const SeqArgs a, const ChunkPlan plan) {
+// The blockIdx.y-th sequence of the batch, the longest ones first (they then
+// start first, and the last round of CTAs is short: 13 ragged turns 580 -> 500
+// us); the given order from 512 on, where sorting would cost more.
+__device__ __forceinline__ uint32_t sequence_of(const SeqArgs& a, uint32_t y, uint32_t* found) {
+    const uint32_t n = gridDim.y;
+    if (n == 1 || n > 512) return y;
+    for (uint32_t s = threadIdx.x; s < n; s += blockDim.x) {
+        const uint32_t len = a.offsets[s + 1] - a.offsets[s];
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t other = a.offsets[i + 1] - a.offsets[i];
+            rank += other > len || (other == len && i < s);
+        }
+        if (rank == y) *found = s;
+    }
+    __syncthreads();
+    return *found;
+}
+
+// A row group is 16 value rows of one head, and KS warps of it take a part of
+// the key channels each: with one sequence there are SMs for all of them, and
+// a warp's MMAs per chunk halve (an MMA holds up its warp's issue for its 8
+// cycles); the parts of W S0^T and Q S0^T are added through shared memory. A
+// last warp copies the operands.
+template <int D, int NW, int KS, int PER_SM, typename E>
+__global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(const SeqArgs a, const ChunkPlan plan) {
     extern __shared__ __align__(128) unsigned char scan_mem[];
-    ChunkStage<D>* stages = reinterpret_cast<ChunkStage<D>*>(scan_mem);
-    ScanBars& bar = *reinterpret_cast<ScanBars*>(scan_mem + kStages * sizeof(ChunkStage<D>));
+    ScanSmem<D, NW, KS>& bar = *reinterpret_cast<ScanSmem<D, NW, KS>*>(scan_mem);
+    ChunkStage<D>* stages = bar.stage;
     volatile int* abort = &bar.abort;
+    __shared__ uint32_t found;
     constexpr uint32_t slices = D / (16 * NW);
-    const uint32_t s = blockIdx.y, h = blockIdx.x / slices, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t s = sequence_of(a, blockIdx.y, &found), h = blockIdx.x / slices, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint32_t t0, t1, chunk, chunk_end, base;
     if (!token_range(a, s, t0, t1)) return;
     segment_chunks(plan, s, t0, t1, chunk, chunk_end, base);
@@ -650,13 +676,13 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             tc::mbar_init(&bar.full[i], 1);
-            tc::mbar_init(&bar.empty[i], NW);
+            tc::mbar_init(&bar.empty[i], NW * KS);
         }
         bar.abort = 0;
         tc::fence_barrier_init();
     }
     __syncthreads();
-    if (warp == NW) {
+    if (warp == NW * KS) {
         const ChunkStage<D>* src = static_cast<const ChunkStage<D>*>(plan.stages) + static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h;
         const E* v = static_cast<const E*>(a.v) + h * D + blockIdx.x % slices * (16 * NW);
         uint32_t n = 0;
@@ -686,15 +712,17 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
         }
         return;
     }
-    const uint32_t row0 = blockIdx.x % slices * (16 * NW) + warp * 16;
+    constexpr int DK = D / KS;   // this warp's key channels, from k0 on
+    const uint32_t half = warp % KS, k0 = half * DK;
+    const uint32_t row0 = blockIdx.x % slices * (16 * NW) + warp / KS * 16;
     const uint32_t g = lane / 4, t = lane % 4, P = a.heads * D;
-    const size_t state_at = (static_cast<size_t>(s) * a.heads + h) * D * D + static_cast<size_t>(row0 + g) * D + 2 * t;
+    const size_t state_at = (static_cast<size_t>(s) * a.heads + h) * D * D + static_cast<size_t>(row0 + g) * D + k0 + 2 * t;
     const E* v = static_cast<const E*>(a.v) + h * D + row0 + g;
     const float* state = chunk ? plan.carry_in : a.state;
     float* state_out = chunk_end * kChunk < t1 - t0 ? plan.carry_out : a.state_out;
-    float S[D / 8][4];
+    float S[DK / 8][4];
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
+    for (int j = 0; j < DK / 8; ++j) {
         float2 x = make_float2(0.0f, 0.0f), y = x;
         if (state) {
             x = *reinterpret_cast<const float2*>(state + state_at + 8 * j);
@@ -726,7 +754,7 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
         {
             float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
+            for (int j = 0; j < DK / 8; ++j) {
                 m0 = fmaxf(m0, fmaxf(fabsf(S[j][0]), fabsf(S[j][1])));
                 m1 = fmaxf(m1, fmaxf(fabsf(S[j][2]), fabsf(S[j][3])));
             }
@@ -745,7 +773,7 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
                 sx[0] += d0;
                 sx[1] += d1;
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
+                for (int j = 0; j < DK / 8; ++j) {
                     S[j][0] *= f0;
                     S[j][1] *= f0;
                     S[j][2] *= f1;
@@ -769,28 +797,51 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
         if (chunk + n + 1 < chunk_end) fetch(first + kChunk);
         tc::mbar_pass(&bar.full[n % kStages], n / kStages & 1u, abort);
         __syncwarp();
-        // T V, W S0^T, (p Q) S0^T
+        // T V, W S0^T and (p Q) S0^T
         float u[2][4] = {}, wb[2][4] = {}, ws[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
         ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
         ldmatrix4<false>(yl, &st.t[1][mrow][mcol]);
         mma_terms1(u, xh, xl, yh, yl);
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
+        for (int j = 0; j < DK / 16; ++j) {
             split_rows(S[2 * j], S[2 * j + 1], xh, xl);
-            ldmatrix4<false>(yh, &st.w[0][mrow][16 * j + mcol]);
-            ldmatrix4<false>(yl, &st.w[1][mrow][16 * j + mcol]);
+            ldmatrix4<false>(yh, &st.w[0][mrow][k0 + 16 * j + mcol]);
+            ldmatrix4<false>(yl, &st.w[1][mrow][k0 + 16 * j + mcol]);
             mma_terms(wb, ws, xh, xl, yh, yl);
-            ldmatrix4<false>(yh, &st.q[0][mrow][16 * j + mcol]);
-            ldmatrix4<false>(yl, &st.q[1][mrow][16 * j + mcol]);
+            ldmatrix4<false>(yh, &st.q[0][mrow][k0 + 16 * j + mcol]);
+            ldmatrix4<false>(yl, &st.q[1][mrow][k0 + 16 * j + mcol]);
             mma_terms(ob, os, xh, xl, yh, yl);
         }
         {
             const float fw[2] = {pow2(-st.exps[0] - sx[0]), pow2(-st.exps[0] - sx[1])};
+            const float fq[2] = {pow2(-st.exps[1] - sx[0]), pow2(-st.exps[1] - sx[1])};
             const float fv[2] = {pow2(-st.exps[3] - vx[0]), pow2(-st.exps[3] - vx[1])};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[i][e] = fmaf(wb[i][e] + ws[i][e], -fw[e / 2], u[i][e] * fv[e / 2]);
+                for (int e = 0; e < 4; ++e) {
+                    wb[i][e] = (wb[i][e] + ws[i][e]) * fw[e / 2];
+                    ob[i][e] = (ob[i][e] + os[i][e]) * fq[e / 2];
+                }
+            if constexpr (KS > 1) {   // the halves' sums, in the same order in both warps
+                float4 (*part)[2][2][32] = bar.part[n % 2][warp / KS];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    part[half][0][i][lane] = make_float4(wb[i][0], wb[i][1], wb[i][2], wb[i][3]);
+                    part[half][1][i][lane] = make_float4(ob[i][0], ob[i][1], ob[i][2], ob[i][3]);
+                }
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(warp / KS)), "n"(32 * KS) : "memory");
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 x = part[0][0][i][lane], y = part[1][0][i][lane], z = part[half ^ 1][1][i][lane];
+                    wb[i][0] = x.x + y.x; wb[i][1] = x.y + y.y; wb[i][2] = x.z + y.z; wb[i][3] = x.w + y.w;
+                    ob[i][0] += z.x; ob[i][1] += z.y; ob[i][2] += z.z; ob[i][3] += z.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[i][e] = fmaf(u[i][e], fv[e / 2], -wb[i][e]);
             row_exps(u, ux);
             // a product's two powers together stay within a float's
             ux[0] = min(ux[0], 126 - max(st.exps[2], st.exps[4]));
@@ -805,19 +856,18 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
             }
             split_rows(u[0], u[1], xh, xl);
         }
-        const float fq[2] = {pow2(-st.exps[1] - sx[0]), pow2(-st.exps[1] - sx[1])};
         {   // S = S diag(total) + U^T (e K)
             const float f0 = pow2(sx[0] - ux[0] - st.exps[2]), f1 = pow2(sx[1] - ux[1] - st.exps[2]);
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
+            for (int j = 0; j < DK / 16; ++j) {
                 float c[2][4] = {};
                 uint32_t zh[4], zl[4];
-                ldmatrix4<true>(zh, &st.ke[0][krow][16 * j + kcol]);
-                ldmatrix4<true>(zl, &st.ke[1][krow][16 * j + kcol]);
+                ldmatrix4<true>(zh, &st.ke[0][krow][k0 + 16 * j + kcol]);
+                ldmatrix4<true>(zl, &st.ke[1][krow][k0 + 16 * j + kcol]);
                 mma_terms1(c, xh, xl, zh, zl);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float2 tot = *reinterpret_cast<const float2*>(&st.total[16 * j + 8 * i + 2 * t]);
+                    const float2 tot = *reinterpret_cast<const float2*>(&st.total[k0 + 16 * j + 8 * i + 2 * t]);
                     float (&x)[4] = S[2 * j + i];
                     x[0] = fmaf(c[i][0], f0, x[0] * tot.x);
                     x[1] = fmaf(c[i][1], f0, x[1] * tot.y);
@@ -833,13 +883,15 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
             mma_terms1(c, xh, xl, yh, yl);
             const float fp[2] = {pow2(-ux[0] - st.exps[4]), pow2(-ux[1] - st.exps[4])};
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
+                if (KS > 1 && i != static_cast<int>(half)) continue;   // a half writes one tile of tokens
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t tok = first + 8 * i + 2 * t + e % 2;
-                    const float o = fmaf(ob[i][e] + os[i][e], fq[e / 2], c[i][e] * fp[e / 2]);
+                    const float o = fmaf(c[i][e], fp[e / 2], ob[i][e]);
                     if (tok < t1) store1<E>(a.out, static_cast<size_t>(tok) * P + h * D + row0 + g + 8 * (e / 2), o);
                 }
+            }
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&bar.empty[n % kStages]);
@@ -847,7 +899,7 @@ __global__ void __launch_bounds__(32 * NW + 32, PER_SM) chunk_scan_kernel(const 
     if (!state_out) return;
     const float f0 = pow2(-sx[0]), f1 = pow2(-sx[1]);
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
+    for (int j = 0; j < DK / 8; ++j) {
         *reinterpret_cast<float2*>(state_out + state_at + 8 * j) = make_float2(S[j][0] * f0, S[j][1] * f0);
         *reinterpret_cast<float2*>(state_out + state_at + 8 * D + 8 * j) = make_float2(S[j][2] * f1, S[j][3] * f1);
     }
@@ -867,15 +919,28 @@ int launch_recurrent(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     return K3XB_OK;
 }
 
+template <int D, int NW, int KS, int PER_SM, typename E>
+int launch_scan(k3xb_ctx* ctx, const SeqArgs& a, const ChunkPlan& p, uint32_t sequences) {
+    static std::atomic<uint64_t> configured{0};   // per template instance
+    const size_t smem = sizeof(ScanSmem<D, NW, KS>);
+    const int cst = configure_once(ctx, configured, [&]() -> int {
+        K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_scan_kernel<D, NW, KS, PER_SM, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            static_cast<int>(smem)));
+        return K3XB_OK;
+    });
+    if (cst) return cst;
+    const dim3 grid(a.heads * (D / (16 * NW)), sequences);
+    chunk_scan_kernel<D, NW, KS, PER_SM, E><<<grid, 32 * NW * KS + 32, smem, ctx->stream>>>(a, p);
+    K3XB_LAUNCHED(ctx);
+    return K3XB_OK;
+}
+
 template <int D, int NW, typename E, bool VEC>
 int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     static std::atomic<uint64_t> configured{0};   // per template instance
     const int cst = configure_once(ctx, configured, [&]() -> int {
         K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_operands_kernel<D, E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             static_cast<int>(sizeof(ChunkScratch<D>))));
-        for (auto* scan : {chunk_scan_kernel<D, NW, 1, E>, chunk_scan_kernel<D, NW, 2, E>})
-            K3XB_CUDA(ctx, cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                static_cast<int>(scan_smem<D>())));
         return K3XB_OK;
     });
     if (cst) return cst;
@@ -895,6 +960,7 @@ int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
     float* between = cv.take<float>(carry);
     if (!carry) between = a.state_out;
     p.carry_in = p.carry_out = between;
+    const uint64_t scans = static_cast<uint64_t>(a.heads) * (D / 32) * sequences;
     for (uint32_t x = 0; x < slots; x += step) {
         p.slot0 = x;
         p.slots = std::min(step, slots - x);
@@ -905,11 +971,13 @@ int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
         p.stride = static_cast<uint32_t>(std::min<uint64_t>(wanted, (p.slots + sequences - 1) / sequences));
         chunk_operands_kernel<D, E, VEC><<<dim3(p.stride * a.heads, sequences), D, sizeof(ChunkScratch<D>), ctx->stream>>>(a, p);
         K3XB_LAUNCHED(ctx);
-        const dim3 grid(a.heads * (D / (16 * NW)), sequences);
-        const bool crowd = static_cast<uint64_t>(grid.x) * grid.y > static_cast<uint64_t>(ctx->sm_count);
-        if (crowd) chunk_scan_kernel<D, NW, 2, E><<<grid, 32 * NW + 32, scan_smem<D>(), ctx->stream>>>(a, p);
-        else chunk_scan_kernel<D, NW, 1, E><<<grid, 32 * NW + 32, scan_smem<D>(), ctx->stream>>>(a, p);
-        K3XB_LAUNCHED(ctx);
+        // few sequences: an SM for every 32 rows, with two warps to a row
+        // group; else two CTAs per SM where there are that many
+        int st;
+        if (D == 128 && scans <= static_cast<uint64_t>(ctx->sm_count)) st = launch_scan<D, 2, D == 128 ? 2 : 1, 1, E>(ctx, a, p, sequences);
+        else if (scans > 2ull * ctx->sm_count) st = launch_scan<D, NW, 1, 2, E>(ctx, a, p, sequences);
+        else st = launch_scan<D, NW, 1, 1, E>(ctx, a, p, sequences);
+        if (st) return st;
     }
     return K3XB_OK;
 }
