@@ -338,12 +338,12 @@ __device__ __forceinline__ float2 load2(const E* p) {
     }
 }
 
-// Largest |x| of 8 tokens' pairs over a warp, as bits (NaN above all).
+// Largest |x| of 8 tokens' pairs over a warp, as bits.
 __device__ __forceinline__ uint32_t warp_top(const float2 (&x)[8]) {
-    uint32_t m = 0;
+    float m[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
-    return __reduce_max_sync(0xffffffffu, m);
+    for (int i = 0; i < 8; ++i) m[i % 2] = fmaxf(m[i % 2], fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+    return __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m[0], m[1])));
 }
 
 // D threads: each two neighbouring channels of eight tokens, lanes 0-15 the

@@ -568,7 +568,9 @@ struct RowParts {
 template <int C>
 __device__ __forceinline__ void join_prefix(Join<C> (&j)[2], const PrefixPlan& p, const Parts& parts, uint32_t h, const uint32_t (&r)[2],
                                             const bool (&there)[2], uint32_t col, uint32_t value) {
-    const RowParts rows[2] = {RowParts(p, h, r[0]), RowParts(p, h, r[1])};
+    RowParts rows[2] = {RowParts(p, h, r[0]), RowParts(p, h, r[0])};
+    rows[1].at += r[1] - r[0];
+    if (r[1] / kTile != r[0] / kTile) rows[1] = RowParts(p, h, r[1]);
     const uint32_t n[2] = {there[0] ? rows[0].n : 0, there[1] ? rows[1].n : 0}, most = max(n[0], n[1]);
     for (uint32_t i0 = 0; i0 < most; i0 += 4) {
         float x[2][4][C];
@@ -601,14 +603,21 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, const Join<C>& j, u
     if (a.lse && col == 0) a.lse[row] = j.l == 0.0f ? -INFINITY : (j.m + __log2f(j.l)) * kLn2;
 }
 
-// Replaces the infinities and NaN of two values by zeros; whether there were.
+// Replaces the infinities and NaN of two values by zeros.
 template <bool BF16>
-__device__ __forceinline__ bool drop_nonfinite(uint32_t& w) {
+__device__ __forceinline__ void drop_nonfinite(uint32_t& w) {
     constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
-    if (lo) w &= 0xffff0000u;
-    if (hi) w &= 0x0000ffffu;
-    return lo || hi;
+    if ((w & e) == e) w &= 0xffff0000u;
+    if ((w >> 16 & e) == e) w &= 0x0000ffffu;
+}
+
+// acc + 0 * w in both halves: zeros as long as every w was finite.
+template <bool BF16>
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t w, uint32_t acc) {
+    uint32_t r;
+    if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(acc));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(acc));
+    return r;
 }
 
 template <bool BF16>
@@ -820,16 +829,28 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
                 pr[x][e] = ex2(fmaf(sc[x][e], c, -off[e >> 1]));
                 l[e >> 1] += pr[x][e];
             }
-        bool odd_values = false;
+        uint32_t finite = 0;   // stays zero (of either sign) unless a draft row has an infinity or NaN
         if (drafts) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
-                for (int j = 0; j < H; ++j)
-                    odd_values |= drop_nonfinite<BF16>(vr[x][j].x) | drop_nonfinite<BF16>(vr[x][j].y) |
-                                  drop_nonfinite<BF16>(vr[x][j].z) | drop_nonfinite<BF16>(vr[x][j].w);
+                for (int j = 0; j < H; ++j) {
+                    finite = add_zero_times<BF16>(vr[x][j].x, finite);
+                    finite = add_zero_times<BF16>(vr[x][j].y, finite);
+                    finite = add_zero_times<BF16>(vr[x][j].z, finite);
+                    finite = add_zero_times<BF16>(vr[x][j].w, finite);
+                }
         }
-        if (drafts && __any_sync(0xffffffffu, odd_values)) {
+        if (drafts && __any_sync(0xffffffffu, finite & 0x7fff7fffu)) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int j = 0; j < H; ++j) {
+                    drop_nonfinite<BF16>(vr[x][j].x);
+                    drop_nonfinite<BF16>(vr[x][j].y);
+                    drop_nonfinite<BF16>(vr[x][j].z);
+                    drop_nonfinite<BF16>(vr[x][j].w);
+                }
             // one key at a time: its probabilities from the lane that has
             // them, its values from memory
             for (uint32_t kk = 0; kk < min(16u, n); ++kk) {
@@ -932,15 +953,23 @@ __global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant
         const uint32_t r[2] = {rt * 16 + row, rt * 16 + row + there[1]};
         if (len >= 0) {
             const size_t at = (static_cast<size_t>(s) * own.tasks + blockIdx.x * own.splits) * 16 + row;
-#pragma unroll 4
-            for (uint32_t k = 0; k < own.splits; ++k)
+            for (uint32_t k0 = 0; k0 < own.splits; k0 += 6) {   // six splits' loads in flight
+                float x[2][6][C];
+                float2 ml[2][6];
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i)
-                    if (there[i]) {
-                        float x[C];
-                        load_cols<C>(own.o + (at + 16 * k + i) * DV + col, x);
-                        j[i].add(own.ml[at + 16 * k + i], x);
-                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < 6; ++k)
+                        if (there[i] && k0 + k < own.splits) {
+                            ml[i][k] = own.ml[at + 16 * (k0 + k) + i];
+                            load_cols<C>(own.o + (at + 16 * (k0 + k) + i) * DV + col, x[i][k]);
+                        }
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+                    for (uint32_t k = 0; k < 6; ++k)
+                        if (there[i] && k0 + k < own.splits) j[i].add(ml[i][k], x[i][k]);
+            }
             if (p.total) join_prefix<C>(j, p, parts, h, {s * rows + r[0], s * rows + r[1]}, there, col, DV);
         }
 #pragma unroll
