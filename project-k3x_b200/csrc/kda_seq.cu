@@ -33,6 +33,7 @@ struct SeqArgs {
     float* state_out;          // NULL: not kept; may be `state`
     void* out;
     int32_t* status;
+    uint32_t from, below;      // sequences that a kernel takes: from <= tokens < below
 };
 
 template <typename E>
@@ -62,8 +63,9 @@ __device__ __forceinline__ void store1(void* p, size_t i, float x) {
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
 
-// The token range of a sequence; false (and the status word set) where the
-// offsets are not a range within the tokens.
+// The token range of a sequence; false where the kernel does not take its
+// length, and (with the status word set) where the offsets are no range
+// within the tokens.
 __device__ __forceinline__ bool token_range(const SeqArgs& a, uint32_t s, uint32_t& t0, uint32_t& t1) {
     if (!a.offsets) {
         t0 = s;
@@ -72,7 +74,7 @@ __device__ __forceinline__ bool token_range(const SeqArgs& a, uint32_t s, uint32
     }
     t0 = a.offsets[s];
     t1 = a.offsets[s + 1];
-    if (t0 <= t1 && t1 <= a.tokens) return true;
+    if (t0 <= t1 && t1 <= a.tokens) return t1 - t0 >= a.from && t1 - t0 < a.below;
     if (threadIdx.x == 0) atomicExch(a.status, K3XB_INVALID_EXTENT);
     return false;
 }
@@ -81,6 +83,11 @@ __device__ __forceinline__ bool token_range(const SeqArgs& a, uint32_t s, uint32
 // sequence; eight lanes share a row (D / 8 keys each, in 16-byte pieces 128
 // bytes apart), so a row's two sums take three shuffles. Both are taken in
 // one pass over the row: o = (S diag(a)) q + delta (k . q).
+//
+// One token of each sequence is bound by its state, read and written once
+// (one B200, 32 heads of 128): 64 sequences 54 us = 5.0 TB/s, 312 of a pool of
+// 400 243 us = 5.4 TB/s, 0.77 and 0.82 of the measured copy rate; 32 rows a CTA
+// leave a thread 128 bytes in flight and 64 sequences 8192 CTAs.
 constexpr int kRows = 32, kSeqThreads = 128, kRowSets = kRows / (kSeqThreads / 8);
 
 template <int D, typename E, bool VEC>
@@ -194,11 +201,16 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // owns 16 value rows and keeps S in registers, in the accumulator layout of
 // mma.m16n8k16, which is also the layout its left operand is read in: S, V
 // and U go from accumulators straight into the next product, without shared
-// memory. (Both in one kernel, with producer warps beside the scan's, took
-// 7900 cycles a chunk for the operands where the scan needs 2000, and kept
-// half the GPU idle at one sequence.) A chunk's operands cross memory once,
-// about as many bytes as its inputs, as an image of the shared memory that
-// the scan copies them to.
+// memory. (Both in one kernel, with producer warps beside the scan's, the
+// producers took 7900 cycles a chunk and the scan 2700, and half the GPU was
+// idle at one sequence: 8192 tokens of 32 heads 2.48 ms, apart 1.23.) A
+// chunk's operands cross memory once, 1.2 times the bytes of its inputs, as an
+// image of the shared memory that the scan copies them to.
+//
+// Measured (one B200): 8192 tokens, 32 heads of 128, f32: operands 257 us (3.5
+// TB/s, the issue slots 53% busy: ~2150 instructions a warp and chunk, most
+// of them splits), scan 570 us, 1.1 us a chunk: a chain of products (84 MMAs a
+// warp), row maxima and splits from one chunk's state to the next's.
 //
 // Every operand is carried as two f16 terms of a power-of-two multiple (hi +
 // lo, 22 bits of the largest element of its tile or row), and a product as hi
@@ -636,11 +648,11 @@ struct __align__(128) ScanSmem {
 };
 
 // The blockIdx.y-th sequence of the batch, the longest ones first (they then
-// start first, and the last round of CTAs is short: 13 ragged turns 580 -> 500
-// us); the given order from 512 on, where sorting would cost more.
+// start first, and the last round of CTAs is short: 13 ragged turns 600 -> 483
+// us); the given order for many or short ones, where sorting costs more.
 __device__ __forceinline__ uint32_t sequence_of(const SeqArgs& a, uint32_t y, uint32_t* found) {
     const uint32_t n = gridDim.y;
-    if (n == 1 || n > 512) return y;
+    if (n == 1 || n > 64 || a.tokens < 256 * n) return y;
     for (uint32_t s = threadIdx.x; s < n; s += blockDim.x) {
         const uint32_t len = a.offsets[s + 1] - a.offsets[s];
         uint32_t rank = 0;
@@ -1041,12 +1053,25 @@ int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
     if (!offsets || (tokens && (!q || !k || !v || !log_decay || !beta || !out)))
         return fail(ctx, K3XB_INVALID_EXTENT, "kda_prefill arguments");
     if (!row_stride) row_stride = static_cast<uint64_t>(heads) * head_dim;
-    const SeqArgs a{q, k, v, row_stride, log_decay, beta, offsets, nullptr, tokens, heads, sequences, state, state_out, out, ctx->status_word};
+    SeqArgs a{q, k, v, row_stride, log_decay, beta, offsets, nullptr, tokens, heads, sequences, state, state_out, out, ctx->status_word, 0, ~0u};
     if (const int st = check_seq(ctx, "kda_prefill", type, sequences, heads, head_dim, a)) return st;
     PhaseScope ph(ctx, K3XB_PHASE_KDA_RECURRENCE);
     ++ctx->stats.kda_calls;
-    return type == K3XB_TYPE_F32 ? launch_prefill<float>(ctx, a, sequences, head_dim)
-                                 : launch_prefill<__nv_bfloat16>(ctx, a, sequences, head_dim);
+    const bool f32 = type == K3XB_TYPE_F32;
+    if (tokens <= 16ull * sequences) {
+        // Short sequences among these: up to 6 tokens go token by token (a
+        // chunk costs the same for 1 as for 16: with 1, 4, 8, 16 tokens each, 64
+        // sequences of 32 heads take 55, 105, 167, 295 us token by token and
+        // 140 to 148 in chunks, 300 take 237, 435, 719, 1332 and 550), the
+        // others in chunks.
+        a.below = 7;
+        if (const int st = f32 ? launch_seq<float>(ctx, a, sequences, head_dim) : launch_seq<__nv_bfloat16>(ctx, a, sequences, head_dim))
+            return st;
+        if (tokens < 7) return K3XB_OK;
+        a.from = 7;
+        a.below = ~0u;
+    }
+    return f32 ? launch_prefill<float>(ctx, a, sequences, head_dim) : launch_prefill<__nv_bfloat16>(ctx, a, sequences, head_dim);
 }
 
 int k3xb_kda_step(k3xb_ctx* ctx, const void* q, const void* k, const void* v, uint64_t row_stride, int32_t type,
@@ -1057,7 +1082,7 @@ int k3xb_kda_step(k3xb_ctx* ctx, const void* q, const void* k, const void* v, ui
         return fail(ctx, K3XB_INVALID_EXTENT, "kda_step arguments");
     if (!slots && states < sequences) return fail(ctx, K3XB_INVALID_EXTENT, "kda_step: fewer states than sequences");
     if (!row_stride) row_stride = static_cast<uint64_t>(heads) * head_dim;
-    const SeqArgs a{q, k, v, row_stride, log_decay, beta, nullptr, slots, sequences, heads, states, state, state, out, ctx->status_word};
+    const SeqArgs a{q, k, v, row_stride, log_decay, beta, nullptr, slots, sequences, heads, states, state, state, out, ctx->status_word, 0, ~0u};
     if (const int st = check_seq(ctx, "kda_step", type, sequences, heads, head_dim, a)) return st;
     PhaseScope ph(ctx, K3XB_PHASE_KDA_RECURRENCE);
     ++ctx->stats.kda_calls;

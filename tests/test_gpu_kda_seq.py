@@ -92,7 +92,7 @@ def _prefill(torch, ctx, x, lengths, h, d, state, **kw):
     return out, new
 
 
-LENGTHS = [[1], [2, 0, 3], [15, 16, 17, 1], [31, 33, 64], [63, 65], [130, 0, 1, 257, 5]]
+LENGTHS = [[1], [2, 0, 3], [8, 9, 7, 10, 0, 1, 30], [1] * 70 + [40], [15, 16, 17, 1], [31, 33, 64], [63, 65], [130, 0, 1, 257, 5]]
 
 
 @pytest.mark.parametrize("lengths", LENGTHS, ids=str)
