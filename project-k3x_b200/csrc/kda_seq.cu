@@ -84,11 +84,12 @@ __device__ __forceinline__ bool token_range(const SeqArgs& a, uint32_t s, uint32
 // bytes apart), so a row's two sums take three shuffles. Both are taken in
 // one pass over the row: o = (S diag(a)) q + delta (k . q).
 //
-// One token of each sequence is bound by its state, read and written once
-// (one B200, 32 heads of 128): 64 sequences 54 us = 5.0 TB/s, 312 of a pool of
-// 400 243 us = 5.4 TB/s, 0.77 and 0.82 of the measured copy rate; 32 rows a CTA
-// leave a thread 128 bytes in flight and 64 sequences 8192 CTAs.
-constexpr int kRows = 32, kSeqThreads = 128, kRowSets = kRows / (kSeqThreads / 8);
+// One token of each sequence is bound by its state, read and written once as a
+// stream (one B200, 32 heads of 128): 64 sequences 45 us = 6.1 TB/s, 312 of a
+// pool of 400 209 us = 6.3 TB/s, 0.93 and 0.97 of the measured copy rate. Two
+// warps of 256 bytes in flight a thread beat four of 128 (54 and 241 us) and
+// eight of 64 (66 and 292 us); without the streaming hint 49 and 202 us.
+constexpr int kRows = 32, kSeqThreads = 64, kSetRows = kSeqThreads / 8, kRowSets = kRows / kSetRows;
 
 template <int D, typename E, bool VEC>
 __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArgs a) {
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
     for (int i = 0; i < kRowSets; ++i)
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const float4 x = a.state ? *reinterpret_cast<const float4*>(a.state + base + (row + 16 * i) * D + g * 32 + sub * 4)
+            const float4 x = a.state ? __ldcs(reinterpret_cast<const float4*>(a.state + base + (row + kSetRows * i) * D + g * 32 + sub * 4))
                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             S[i][g][0] = x.x; S[i][g][1] = x.y; S[i][g][2] = x.z; S[i][g][3] = x.w;
         }
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
         float vv[kRowSets], pred[kRowSets], o[kRowSets], kq = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRowSets; ++i) {
-            vv[i] = to_f(v[at + row + 16 * i]);
+            vv[i] = to_f(v[at + row + kSetRows * i]);
             pred[i] = o[i] = 0.0f;
         }
 #pragma unroll
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) S[i][g][j] = fmaf(delta, kk[g][j], S[i][g][j]);
-            if (sub == 0) store1<E>(a.out, static_cast<size_t>(t) * P + h * D + row + 16 * i, fmaf(delta, kq, o[i]));
+            if (sub == 0) store1<E>(a.out, static_cast<size_t>(t) * P + h * D + row + kSetRows * i, fmaf(delta, kq, o[i]));
         }
     }
     if (!a.state_out) return;
@@ -175,8 +176,8 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
     for (int i = 0; i < kRowSets; ++i)
 #pragma unroll
         for (int g = 0; g < G; ++g)
-            *reinterpret_cast<float4*>(a.state_out + base + (row + 16 * i) * D + g * 32 + sub * 4) =
-                make_float4(S[i][g][0], S[i][g][1], S[i][g][2], S[i][g][3]);
+            __stcs(reinterpret_cast<float4*>(a.state_out + base + (row + kSetRows * i) * D + g * 32 + sub * 4),
+                   make_float4(S[i][g][0], S[i][g][1], S[i][g][2], S[i][g][3]));
 }
 
 // ---- chunks of 16 tokens ------------------------------------------------------
@@ -1060,10 +1061,10 @@ int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
     const bool f32 = type == K3XB_TYPE_F32;
     if (tokens <= 16ull * sequences) {
         // Short sequences among these: up to 6 tokens go token by token (a
-        // chunk costs the same for 1 as for 16: with 1, 4, 8, 16 tokens each, 64
-        // sequences of 32 heads take 55, 105, 167, 295 us token by token and
-        // 140 to 148 in chunks, 300 take 237, 435, 719, 1332 and 550), the
-        // others in chunks.
+        // chunk costs the same for 1 as for 16: 64 sequences of 32 heads take
+        // 58, 63 and 81 us with 1, 2 and 4 tokens each and 138 to 142 in chunks
+        // of 8 or 16, 300 take 231, 311, 407 and 582 to 591), the others in
+        // chunks.
         a.below = 7;
         if (const int st = f32 ? launch_seq<float>(ctx, a, sequences, head_dim) : launch_seq<__nv_bfloat16>(ctx, a, sequences, head_dim))
             return st;
