@@ -476,17 +476,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             parts.ml[part * kTile + row] = make_float2(m, l);
             wait(&bar.o_done[t], seg & 1u);
             if (n) {
-                float* dst = parts.o + (part * kTile + row) * value;
+                // through the tile's query rows, which no product reads any
+                // more: a thread has a row, a store should have a few (16-byte
+                // chunk c of row r stands at c ^ r)
+                constexpr uint32_t cols = NK > 1 ? 64 : 32, chunks = cols / 4;
+                float4* stage = reinterpret_cast<float4*>(q_smem + t * NK * kAtom) + (warp % 4) * 32 * chunks;
+                float* dst = parts.o + (part * kTile + 32 * (warp % 4)) * value;
+                const uint32_t rows = min(32u, p.rows - min(p.rows, tile * kTile + 32 * (warp % 4)));
+                for (uint32_t cc = 0; cc < value; cc += cols) {
 #pragma unroll
-                for (uint32_t cc = 0; cc < value; cc += 32) {
-                    uint32_t o[32];
-                    tc::tmem_ld32(out_at + cc, o);
-                    tc::tmem_wait_ld();
-                    if (tile * kTile + row < p.rows)
+                    for (uint32_t c0 = 0; c0 < cols; c0 += 32) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(out_at + cc + c0, o);
+                        tc::tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            *reinterpret_cast<uint4*>(dst + cc + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (uint32_t j = 0; j < 8; ++j)
+                            stage[lane * chunks + ((c0 / 4 + j) ^ (lane % chunks))] =
+                                make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
+                                            __uint_as_float(o[4 * j + 3]));
+                    }
+                    __syncwarp();
+#pragma unroll 4
+                    for (uint32_t r = lane / chunks; r < rows; r += 32 / chunks)
+                        *reinterpret_cast<float4*>(dst + r * value + cc + lane % chunks * 4) =
+                            stage[r * chunks + ((lane % chunks) ^ (r % chunks))];
+                    __syncwarp();
                 }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + static_cast<int>(t)) : "memory");   // before the next queries
                 tc::fence_before_sync();
             }
             x += s.n;
