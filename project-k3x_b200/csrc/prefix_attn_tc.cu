@@ -567,26 +567,28 @@ __device__ __forceinline__ void load_cols(const float* src, float (&x)[C]) {
     }
 }
 
-// The prefix's parts of one row of a kv head.
+// The prefix's parts of one row of a kv head, as rows of Parts (32-bit: the
+// host checks their count).
 struct RowParts {
-    size_t at, step;      // the first part's row; from one CTA's to the next one's
-    uint32_t n, halves, seg0;
+    uint32_t first, second, step;   // rows of the first CTA's part and the next one's; from CTA to CTA
+    uint32_t n, pairs;              // parts; 1: two halves to a CTA
     __device__ __forceinline__ RowParts(const PrefixPlan& p, uint32_t h, uint32_t r) {
-        const uint32_t tile = r / kTile, pair = min(tile / 2, p.pairs), jobs = p.pairs + p.odd;
+        const uint32_t tile = r / kTile, pair = min(tile / 2, p.pairs);
         const bool keys = pair == p.pairs;
         const uint32_t begin = h * p.steps_per_head + pair * p.blocks;
         const uint32_t end = begin + (keys ? (p.blocks + 1) / 2 : p.blocks);
         const uint32_t c0 = begin / p.range, c1 = (end - 1) / p.range;
         // the job is one of the segments of CTA c0 and the first one of the CTAs behind it
-        seg0 = h * jobs + pair - job_of(p, c0 * p.range).index;
-        halves = keys ? 2 : 1;
-        n = (c1 - c0 + 1) * halves;
-        step = static_cast<size_t>(p.max_seg) * 2 * kTile;
-        at = c0 * step + (keys ? 0 : tile % 2) * kTile + r % kTile;
+        const uint32_t seg0 = h * (p.pairs + p.odd) + pair - job_of(p, c0 * p.range).index;
+        pairs = keys ? 1 : 0;
+        n = (c1 - c0 + 1) << pairs;
+        step = p.max_seg * 2 * kTile;
+        second = (c0 + 1) * step + (keys ? 0 : tile % 2) * kTile + r % kTile;
+        first = second - step + seg0 * 2 * kTile;
     }
-    __device__ __forceinline__ size_t part(uint32_t i) const {
-        const uint32_t c = i / halves;
-        return at + c * step + (c ? 0 : seg0 * 2 * kTile) + (i - c * halves) * kTile;
+    __device__ __forceinline__ uint32_t part(uint32_t i) const {
+        const uint32_t c = i >> pairs, half = (i & pairs) * kTile;
+        return half + (c ? second + (c - 1) * step : first);
     }
 };
 
@@ -596,7 +598,8 @@ template <int C>
 __device__ __forceinline__ void join_prefix(Join<C> (&j)[2], const PrefixPlan& p, const Parts& parts, uint32_t h, const uint32_t (&r)[2],
                                             const bool (&there)[2], uint32_t col, uint32_t value) {
     RowParts rows[2] = {RowParts(p, h, r[0]), RowParts(p, h, r[0])};
-    rows[1].at += r[1] - r[0];
+    rows[1].first += r[1] - r[0];
+    rows[1].second += r[1] - r[0];
     if (r[1] / kTile != r[0] / kTile) rows[1] = RowParts(p, h, r[1]);
     const uint32_t n[2] = {there[0] ? rows[0].n : 0, there[1] ? rows[1].n : 0}, most = max(n[0], n[1]);
     for (uint32_t i0 = 0; i0 < most; i0 += 4) {
@@ -607,9 +610,9 @@ __device__ __forceinline__ void join_prefix(Join<C> (&j)[2], const PrefixPlan& p
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
                 if (i0 + i < n[k]) {
-                    const size_t at = rows[k].part(i0 + i);
+                    const uint32_t at = rows[k].part(i0 + i);
                     ml[k][i] = parts.ml[at];
-                    load_cols<C>(parts.o + at * value + col, x[k][i]);
+                    load_cols<C>(parts.o + static_cast<size_t>(at) * value + col, x[k][i]);
                 }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -1115,6 +1118,8 @@ int launch_attend_tc(k3xb_ctx* ctx, const AttnArgs& a, bool bf16) {
         p.range = (p.total + sms - 1) / sms;
         ctas = (p.total + p.range - 1) / p.range;
         p.max_seg = p.range / (p.odd ? (p.blocks + 1) / 2 : p.blocks) + 2;
+        if (static_cast<uint64_t>(ctas) * p.max_seg * 2 * kTile >= (1ull << 31))
+            return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: too many rows");
     }
     // Tasks for the GPU's warps three times over (twelve per SM), since
     // sequences are of unlike lengths; a split has 256 cache rows at least (by
