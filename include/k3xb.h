@@ -593,8 +593,9 @@ typedef struct {
  * heads is a multiple of kv_heads (head h reads kv head h / (heads /
  * kv_heads)); main_dim + extra_dim and value_dim at most 256. bf16 and f16
  * calls with main_dim and value_dim 64 or 128, extra_dim 0 or 64, and rows that start at
- * 16-byte boundaries run on the tensor cores, where the prefix is read once
- * for all sequences and the probabilities enter the second product rounded
+ * 16-byte boundaries (and a scale that is not 0) run on the tensor cores,
+ * where the prefix is read once for 256 rows of a kv head (sequences x nodes
+ * x grouped heads) and the probabilities enter the second product rounded
  * to `type`; other shapes take a slower general form. A suffix_len that
  * leaves no room for the drafts counts as idle and k3xb_sync reports
  * INVALID_EXTENT. */

@@ -19,7 +19,7 @@
 // Scores stay float; m is kept in log2 units (score * scale * log2 e).
 //
 // Measured (one B200, 32 heads, keys of 128 + 64, values of 128, prefix 16384):
-// 64 x 9 rows a head: prefix_kernel 203 us (0.95 PFLOP/s of tensor work, 56% of
+// 64 x 9 rows a head: prefix_kernel 201 us (0.96 PFLOP/s of tensor work, 57% of
 // the measured peak), own_kernel 69 us; 64 rows: 63 us (4.3 TB/s) and 52 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -163,10 +163,9 @@ __device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint32_t x, u
 //
 // Warps 0-3 and 4-7 are the softmax of row tile (or key half) 0 and 1, a
 // thread per row; warp 8 loads, warp 9 issues the MMAs (10 and 11 only fill
-// the warpgroup). TMEM: output 0, 1 and
-// scores 0, 1, 128 columns each; the probabilities overwrite the scores they
-// come from (two per column), and the next score tile is issued behind the
-// product that reads them.
+// the warpgroup). TMEM: output 0, 1 and scores 0, 1, 128 columns each; the
+// probabilities overwrite the scores they come from (two per column), and the
+// next score tile is issued behind the product that reads them.
 //
 // The running maximum is lazy: rows keep an old m until a score passes it by
 // more than 2^8, so that the accumulator is rescaled a few times per row

@@ -195,6 +195,25 @@ def test_prefill_in_pieces_and_in_place(torch, ctx):
     _near(torch, state, want_new, "state")
 
 
+@pytest.mark.parametrize("kept", [True, False])
+def test_prefill_in_segments(torch, ctx, kept):
+    """More chunk operands than are held at a time (1 GiB, 72 chunks of 512
+    heads): sequences begin and end in different segments, their states
+    between segments in state_out or, where that is not wanted, elsewhere."""
+    lengths, h, d = [700, 3, 590], 512, 128
+    x = _inputs(torch, sum(lengths), h, d, torch.bfloat16, 49)
+    off = torch.tensor(np.cumsum([0, *lengths]), dtype=torch.int32).cuda()
+    out = torch.empty(sum(lengths), h * d, dtype=torch.bfloat16, device="cuda")
+    state = torch.randn(3, h, d, d, generator=torch.Generator().manual_seed(11)).cuda()
+    new = torch.empty_like(state) if kept else None
+    ctx.kda_prefill(*x, off, out, state=state, state_out=new)
+    ctx.sync()
+    want_out, want_new = _want(torch, x, lengths, h, d, state)
+    _near(torch, out, want_out, "out")
+    if kept:
+        _near(torch, new, want_new, "state")
+
+
 def test_prefill_on_another_stream(torch, ctx):
     h, d = 2, 128
     x = _inputs(torch, 90, h, d, torch.float32, 53)
