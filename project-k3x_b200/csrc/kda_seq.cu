@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
     extern __shared__ __align__(16) unsigned char chunk_mem[];
     ChunkScratch<D>& sc = *reinterpret_cast<ChunkScratch<D>*>(chunk_mem);
     constexpr int NP = D / 32;   // warps
+    asm volatile("griddepcontrol.launch_dependents;");   // the scan's CTAs may start as these run out
     const uint32_t s = blockIdx.y, h = blockIdx.x % a.heads;
     uint32_t t0, t1, chunk, chunk_end, base;
     if (!token_range(a, s, t0, t1)) return;
@@ -700,6 +701,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
         const E* v = static_cast<const E*>(a.v) + h * D + blockIdx.x % slices * (16 * NW);
         uint32_t n = 0;
         bool ok = true;
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // the operands are written
         for (; ok && chunk + n < chunk_end; ++n, src += a.heads) {
             // this CTA's columns of v, for the warps to find in L2
             const uint32_t tok = t0 + (chunk + n) * kChunk + lane / 2;
@@ -942,9 +944,20 @@ int launch_scan(k3xb_ctx* ctx, const SeqArgs& a, const ChunkPlan& p, uint32_t se
         return K3XB_OK;
     });
     if (cst) return cst;
-    const dim3 grid(a.heads * (D / (16 * NW)), sequences);
-    chunk_scan_kernel<D, NW, KS, PER_SM, E><<<grid, 32 * NW * KS + 32, smem, ctx->stream>>>(a, p);
-    K3XB_LAUNCHED(ctx);
+    // starts beside the operands kernel's tail; its copying warp waits for the
+    // end of that kernel, and nothing else here reads what it writes
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.heads * (D / (16 * NW)), sequences);
+    cfg.blockDim = dim3(32 * NW * KS + 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, chunk_scan_kernel<D, NW, KS, PER_SM, E>, a, p));
+    ++ctx->stats.kernel_launches;
     return K3XB_OK;
 }
 
