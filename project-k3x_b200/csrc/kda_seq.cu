@@ -937,17 +937,22 @@ int launch_recurrent(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
 template <int D, int NW, int KS, int PER_SM, typename E>
 int launch_scan(k3xb_ctx* ctx, const SeqArgs& a, const ChunkPlan& p, uint32_t sequences) {
     static std::atomic<uint64_t> configured{0};   // per template instance
-    const size_t smem = sizeof(ScanSmem<D, NW, KS>);
+    const dim3 grid(a.heads * (D / (16 * NW)), sequences);
+    // Where every CTA can have an SM of its own it asks for more than half of
+    // the shared memory: two on one SM while others idle share its issue
+    // slots (8192 tokens of 32 heads 1087 us, 804 apart).
+    constexpr size_t need = sizeof(ScanSmem<D, NW, KS>), alone = std::max(need, size_t(116) << 10);
+    const size_t smem = static_cast<uint64_t>(grid.x) * grid.y <= static_cast<uint64_t>(ctx->sm_count) ? alone : need;
     const int cst = configure_once(ctx, configured, [&]() -> int {
         K3XB_CUDA(ctx, cudaFuncSetAttribute(chunk_scan_kernel<D, NW, KS, PER_SM, E>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            static_cast<int>(smem)));
+                                            static_cast<int>(alone)));
         return K3XB_OK;
     });
     if (cst) return cst;
     // starts beside the operands kernel's tail; its copying warp waits for the
     // end of that kernel, and nothing else here reads what it writes
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.heads * (D / (16 * NW)), sequences);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(32 * NW * KS + 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
