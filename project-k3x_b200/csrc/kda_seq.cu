@@ -618,8 +618,8 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
     }
 }
 
-// Row maxima of two rows over a quad's lanes as scale exponents.
-__device__ __forceinline__ void row_exps(float m0, float m1, int (&ex)[2]) {
+// Row maxima of two rows over a quad's lanes, and as scale exponents.
+__device__ __forceinline__ float2 row_exps(float m0, float m1, int (&ex)[2]) {
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
@@ -627,9 +627,10 @@ __device__ __forceinline__ void row_exps(float m0, float m1, int (&ex)[2]) {
     }
     ex[0] = scale_exp(m0);
     ex[1] = scale_exp(m1);
+    return make_float2(m0, m1);
 }
-__device__ __forceinline__ void row_exps(const float (&x)[2][4], int (&ex)[2]) {
-    row_exps(fmaxf(fmaxf(fabsf(x[0][0]), fabsf(x[0][1])), fmaxf(fabsf(x[1][0]), fabsf(x[1][1]))),
+__device__ __forceinline__ float2 row_exps(const float (&x)[2][4], int (&ex)[2]) {
+    return row_exps(fmaxf(fmaxf(fabsf(x[0][0]), fabsf(x[0][1])), fmaxf(fabsf(x[1][0]), fabsf(x[1][1]))),
              fmaxf(fmaxf(fabsf(x[0][2]), fabsf(x[0][3])), fmaxf(fabsf(x[1][2]), fabsf(x[1][3]))), ex);
 }
 
@@ -766,6 +767,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
         const uint32_t first = t0 + (chunk + n) * kChunk;
         const ChunkStage<D>& st = stages[n % kStages];
         int vx[2], ux[2];
+        const float2 top = row_exps(vv, vx);
         {
             float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
@@ -779,12 +781,15 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
                 m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
             }
             // a row's multiple changes when its largest element leaves
-            // [2^8, 2^15]: f16 holds it then, with 32 bits below it
-            const bool off0 = m0 > 0x1p15f || (m0 < 0x1p8f && m0 != 0.0f && sx[0] < 100);
-            const bool off1 = m1 > 0x1p15f || (m1 < 0x1p8f && m1 != 0.0f && sx[1] < 100);
+            // [2^8, 2^15]: f16 holds it then, with 32 bits below it. It stays
+            // below 2^40 over that of the values to come, so that a small
+            // state's multiple does not carry their sums past a float's end.
+            const int cap0 = top.x == 0.0f ? 126 : min(126, vx[0] + 40), cap1 = top.y == 0.0f ? 126 : min(126, vx[1] + 40);
+            const bool off0 = m0 > 0x1p15f || (m0 < 0x1p8f && m0 != 0.0f && sx[0] < cap0) || sx[0] > cap0;
+            const bool off1 = m1 > 0x1p15f || (m1 < 0x1p8f && m1 != 0.0f && sx[1] < cap1) || sx[1] > cap1;
             if (__any_sync(0xffffffffu, off0 || off1)) {
-                const int d0 = off0 ? min(scale_exp(m0) - 2, 100 - sx[0]) : 0, d1 = off1 ? min(scale_exp(m1) - 2, 100 - sx[1]) : 0;
-                const float f0 = exp2i(d0), f1 = exp2i(d1);
+                const int d0 = off0 ? min(scale_exp(m0) - 2, cap0 - sx[0]) : 0, d1 = off1 ? min(scale_exp(m1) - 2, cap1 - sx[1]) : 0;
+                const float f0 = pow2(d0), f1 = pow2(d1);
                 sx[0] += d0;
                 sx[1] += d1;
 #pragma unroll
@@ -797,7 +802,6 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
             }
         }
         uint32_t xh[4], xl[4], yh[4], yl[4];
-        row_exps(vv, vx);
         {
             const float f0 = exp2i(vx[0]), f1 = exp2i(vx[1]);
 #pragma unroll
@@ -828,9 +832,11 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
             mma_terms(ob, os, xh, xl, yh, yl);
         }
         {
-            const float fw[2] = {pow2(-st.exps[0] - sx[0]), pow2(-st.exps[0] - sx[1])};
-            const float fq[2] = {pow2(-st.exps[1] - sx[0]), pow2(-st.exps[1] - sx[1])};
-            const float fv[2] = {pow2(-st.exps[3] - vx[0]), pow2(-st.exps[3] - vx[1])};
+            // products of two powers: their exponents' sum may pass a normal
+            // float's (small values, a small state)
+            const float fs[2] = {pow2(-sx[0]), pow2(-sx[1])}, ft = pow2(-st.exps[3]), fv[2] = {pow2(-vx[0]), pow2(-vx[1])};
+            const float fw[2] = {pow2(-st.exps[0]) * fs[0], pow2(-st.exps[0]) * fs[1]};
+            const float fq[2] = {pow2(-st.exps[1]) * fs[0], pow2(-st.exps[1]) * fs[1]};
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -856,7 +862,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[i][e] = fmaf(u[i][e], fv[e / 2], -wb[i][e]);
+                for (int e = 0; e < 4; ++e) u[i][e] = fmaf(u[i][e] * ft, fv[e / 2], -wb[i][e]);
             row_exps(u, ux);
             // a product's two powers together stay within a float's
             ux[0] = min(ux[0], 126 - max(st.exps[2], st.exps[4]));
