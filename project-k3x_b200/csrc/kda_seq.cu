@@ -191,11 +191,11 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 //   S = S0 diag(p_15) + U^T (e K)
 //
 // which is the rule's own sums in another order. Decays are products of the
-// tokens' own, never quotients, so any decay from 0 on is as exact as in the
-// token form: for a pair (i, j) D_ij is split where the halves of the
-// smallest aligned block that holds both meet, D_ij = (decay from there to i)
-// (decay from j to there). Four block sizes (16, 8, 4, 2) make four products
-// of 8 upper by 8 lower rows, of which a token is in one side each.
+// tokens' own, never quotients: for a pair (i, j) D_ij is split where the
+// halves of the smallest aligned block that holds both meet, D_ij = (decay
+// from there to i) (decay from j to there). Four block sizes (16, 8, 4, 2)
+// make four products of 8 upper by 8 lower rows, of which a token is in one
+// side each.
 //
 // Two kernels. chunk_operands_kernel makes every chunk's operands, all chunks
 // and heads side by side. chunk_scan_kernel goes along the sequences: a warp
@@ -208,30 +208,45 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // chunk's operands cross memory once, 1.2 times the bytes of its inputs, as an
 // image of the shared memory that the scan copies them to.
 //
-// Measured (one B200): 8192 tokens, 32 heads of 128, f32: operands 257 us (3.5
+// Measured (one B200): 8192 tokens, 32 heads of 128, f32: operands 259 us (3.5
 // TB/s, the issue slots 53% busy: ~2150 instructions a warp and chunk, most
-// of them splits), scan 570 us, 1.1 us a chunk: a chain of products (84 MMAs a
+// of them splits), scan 555 us, 1.1 us a chunk: a chain of products (90 MMAs a
 // warp), row maxima and splits from one chunk's state to the next's.
 //
-// Every operand is carried as two f16 terms of a power-of-two multiple (hi +
-// lo, 22 bits of the largest element of its tile or row), and a product as hi
-// hi + hi lo + lo hi in f32 accumulators, the small products summed apart
-// (a tensor core truncates each sum): float accuracy at three times the MMA
+// Terms. An f16 operand is two terms of a power-of-two multiple (hi + lo: 22
+// bits down to 2^-17 of the multiple's end, 2^-39 of it below) and a product hi hi +
+// hi lo + lo hi in f32 accumulators: float accuracy at three times the MMA
 // work, where plain f16 or bf16 operands would leave the f32 state with 3
-// digits and TF32 in two terms would take twice the MMAs.
+// digits. The long products are of that kind (S by value rows, W and p Q by
+// tokens, e K and U by value rows; small products summed apart, since a
+// tensor core truncates each sum). T, V, P and U, whose elements may be of any
+// size beside each other, are three bf16 terms (24 bits at any size) in their
+// short products.
+//
+// Tokens of unlike size. What one token may lose to another's size is taken
+// out beforehand, by powers of two and thus exactly: token j's key times
+// 2^(x + dx_j), so that every token's largest is alike (up to 2^40 apart), its query
+// times 2^z_j, its decay times 2^-e_j, so that its largest channel is 1/2 to 1 (down to
+// 2^-40 from the chunk's start). With E_j the sum of the e up to j the rule holds for
+//   b_j 2^(-2 dx_j),  v_j 2^(dx_j - E_j + c),  u_j 2^(-dx_j - E_j + c),  o_j 2^(z_j - E_j)
+// in place of b, v, u and o: the powers go to T's columns, P's rows and
+// the rows' factors fw and fq. So an output is off by float roundings of its
+// own query times its own row's content, and no later token changes it.
 
 constexpr int kChunk = 16, kStages = 3;
+constexpr int kKeySpread = 40, kLeastDecay = -40;
 // Operands held at a time: longer batches go in segments of chunks.
 constexpr size_t kOperandBytes = size_t(1) << 30;
 
 template <int D>
 struct __align__(128) ChunkStage {
-    // hi, lo; [tok][channel] rows of D + 8 values: ldmatrix reads 8 of them
+    // f16 hi, lo; [tok][channel] rows of D + 8 values: ldmatrix reads 8 of them
     // without a bank conflict; 16 + 8 likewise
     __half w[2][kChunk][D + 8], q[2][kChunk][D + 8], ke[2][kChunk][D + 8];   // W, p Q, e K
-    __half t[2][kChunk][kChunk + 8], p[2][kChunk][kChunk + 8];
-    float total[D];     // p_15
-    int exps[8];        // the powers of two of w, q, ke, t, p
+    __nv_bfloat16 t[3][kChunk][kChunk + 8], p[3][kChunk][kChunk + 8];        // three bf16 terms
+    float total[D];                 // p_15
+    float fw[kChunk], fq[kChunk];   // what a token's products with w and q are still to be multiplied by
+    int exp;                        // U^T (e K) is to be multiplied by 2^exp
 };
 
 template <int D>
@@ -239,12 +254,16 @@ struct __align__(16) ChunkScratch {
     __half k[2][kChunk][D + 8];           // p K
     // per block size: 8 upper rows of k, 8 of q, 8 lower rows of k
     __half level[4][2][24][D + 8];
-    __half t[2][kChunk][kChunk + 8];
+    float T[kChunk][kChunk];
     float At[kChunk][kChunk];             // At[j][i] = A_ij
     float P[kChunk][kChunk];
     float diag[D / 32][kChunk];           // q_i . k_i by warp
     float beta[kChunk];
-    uint32_t top[6][D / 32];
+    uint32_t top[3][D / 32][kChunk / 2];  // largest |k|, |q|, decay of each token by warp: two tokens' upper halves
+    // powers of two by token: of k, q and the decay (each warp's own); of T's columns, P's rows and its diagonal
+    float sk[D / 32][kChunk], sq[D / 32][kChunk], sa[D / 32][kChunk], ft[kChunk], fp[kChunk], fd[kChunk];
+    float fx;                             // of all keys' products
+    int wexp;                             // of the products with W, besides its rows' own
 };
 
 // The chunks of a call lie in slots: sequence s from offsets[s] / 16 + s on
@@ -274,11 +293,8 @@ __device__ __forceinline__ int scale_exp(float top) {
 }
 // 2^e, e clamped to what a float holds normalised
 __device__ __forceinline__ float pow2(int e) { return exp2i(max(-126, min(127, e))); }
-
-__device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
-    hi = __float2half_rn(x);
-    lo = __float2half_rn(x - __half2float(hi));
-}
+// 2^e to the ends of a float, subnormals included (|e| up to 252)
+__device__ __forceinline__ float two_to(int e) { return pow2(e / 2) * pow2(e - e / 2); }
 
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return make_float2(x.x * y.x, x.y * y.y); }
 __device__ __forceinline__ float2 mul1(float2 x, float y) { return make_float2(x.x * y, x.y * y); }
@@ -299,6 +315,22 @@ __device__ __forceinline__ void store_pair(__half (&dst)[2][ROWS][W], int row, i
     *reinterpret_cast<uint32_t*>(&dst[1][row][col]) = lo;
 }
 
+// Two neighbours as three packed bf16 terms: 24 bits at any size.
+__device__ __forceinline__ void split_bf16(float2 x, uint32_t (&w)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(x);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        x.x -= __uint_as_float(w[i] << 16);
+        x.y -= __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -338,6 +370,33 @@ __device__ __forceinline__ void mma_terms1(float (&c)[2][4], const uint32_t (&xh
     for (int n = 0; n < 2; ++n) mma_f16(c[n], xh, yh[2 * n], yh[2 * n + 1]);
 }
 
+// c += x y^T over a chunk's tokens in bf16 terms (NX of x, in accumulator
+// layout; three of y in shared memory, `row` this lane's ldmatrix row of the
+// first), the small products first.
+template <int NX>
+__device__ __forceinline__ void split_tokens(const float (&x)[2][4], uint32_t (&xw)[3][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w[3];
+        split_bf16(make_float2(x[i / 2][i % 2 * 2], x[i / 2][i % 2 * 2 + 1]), w);
+#pragma unroll
+        for (int n = 0; n < NX; ++n) xw[n][i] = w[n];
+    }
+}
+template <int NX>
+__device__ __forceinline__ void mma_tokens(float (&c)[2][4], const uint32_t (&xw)[3][4], const __nv_bfloat16* row) {
+    uint32_t y[3][4];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) ldmatrix4<false>(y[i], row + i * kChunk * (kChunk + 8));
+#pragma unroll
+    for (int order = 2; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i < NX; ++i)
+            if (i <= order)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) mma_bf16(c[n], xw[i], y[order - i][2 * n], y[order - i][2 * n + 1]);
+}
+
 // Two neighbouring values as floats; VEC: at a multiple of two elements.
 template <typename E, bool VEC>
 __device__ __forceinline__ float2 load2(const E* p) {
@@ -351,12 +410,54 @@ __device__ __forceinline__ float2 load2(const E* p) {
     }
 }
 
-// Largest |x| of 8 tokens' pairs over a warp, as bits.
-__device__ __forceinline__ uint32_t warp_top(const float2 (&x)[8]) {
-    float m[2] = {0.0f, 0.0f};
+__device__ __forceinline__ uint32_t max_halves(uint32_t x, uint32_t y) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+}
+// Largest |x| of each of 8 tokens over a half warp, by the floats' upper
+// halves (which order like the floats): a lane ends with tokens 2 i and 2 i + 1,
+// i = lane / 4 % 4, each exchange halving the tokens that it still has.
+__device__ __forceinline__ uint32_t token_tops(const float2 (&x)[8], uint32_t lane) {
+    uint32_t m[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i % 2] = fmaxf(m[i % 2], fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
-    return __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m[0], m[1])));
+    for (int i = 0; i < 4; ++i)
+        m[i] = max_halves(__byte_perm(__float_as_uint(x[2 * i].x), __float_as_uint(x[2 * i + 1].x), 0x7632) & 0x7fff7fffu,
+                          __byte_perm(__float_as_uint(x[2 * i].y), __float_as_uint(x[2 * i + 1].y), 0x7632) & 0x7fff7fffu);
+#pragma unroll
+    for (int w = 2; w > 0; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const bool up = lane & (4 * w);
+            const uint32_t give = up ? m[i] : m[i + w], keep = up ? m[i + w] : m[i];
+            m[i] = max_halves(keep, __shfl_xor_sync(0xffffffffu, give, 4 * w));
+        }
+    m[0] = max_halves(m[0], __shfl_xor_sync(0xffffffffu, m[0], 2));
+    return max_halves(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+}
+
+// Row maxima of two rows over a quad's lanes, and as scale exponents.
+__device__ __forceinline__ float2 row_exps(float m0, float m1, int (&ex)[2]) {
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+    }
+    ex[0] = scale_exp(m0);
+    ex[1] = scale_exp(m1);
+    return make_float2(m0, m1);
+}
+__device__ __forceinline__ float2 row_exps(const float (&x)[2][4], int (&ex)[2]) {
+    return row_exps(fmaxf(fmaxf(fabsf(x[0][0]), fabsf(x[0][1])), fmaxf(fabsf(x[1][0]), fabsf(x[1][1]))),
+             fmaxf(fmaxf(fabsf(x[0][2]), fabsf(x[0][3])), fmaxf(fabsf(x[1][2]), fabsf(x[1][3]))), ex);
+}
+
+// [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
+__device__ __forceinline__ void split_rows(const float (&x)[4], const float (&y)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    split_pair(make_float2(x[0], x[1]), hi[0], lo[0]);
+    split_pair(make_float2(x[2], x[3]), hi[1], lo[1]);
+    split_pair(make_float2(y[0], y[1]), hi[2], lo[2]);
+    split_pair(make_float2(y[2], y[3]), hi[3], lo[3]);
 }
 
 // D threads: each two neighbouring channels of eight tokens, lanes 0-15 the
@@ -395,15 +496,119 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
         if (threadIdx.x < kChunk)
             bb = first + threadIdx.x < t1 ? a.beta[static_cast<size_t>(first + threadIdx.x) * a.heads + h] : 0.0f;
     };
+    // the next chunk's rows on their way to L2, 128 bytes a thread, a chunk's
+    // work before they are loaded (13 ragged turns: 500 -> 430 us)
+    auto prefetch = [&](uint32_t first) {
+        constexpr uint32_t qk = (D * sizeof(E) + 127) / 128, all = 2 * qk + (D * 4 + 127) / 128;
+        const size_t tok = first + threadIdx.x % kChunk;
+        if (tok >= t1) return;
+#pragma unroll
+        for (uint32_t p = 0; p < all; p += D / kChunk) {
+            const uint32_t x = p + threadIdx.x / kChunk;
+            const char* at = x < qk       ? reinterpret_cast<const char*>(static_cast<const E*>(a.q) + tok * a.row_stride + h * D) + 128 * x
+                             : x < 2 * qk ? reinterpret_cast<const char*>(static_cast<const E*>(a.k) + tok * a.row_stride + h * D) + 128 * (x - qk)
+                                          : reinterpret_cast<const char*>(a.log_decay + tok * P + h * D) + 128 * (x - 2 * qk);
+            if (all % (D / kChunk) == 0 || x < all) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+        }
+    };
     const uint32_t arow = lane % 16, acol = lane / 16 * 8;         // ldmatrix: left operands, and k-major ones transposed
     fetch(t0 + chunk * kChunk);
     for (; chunk < chunk_end; chunk += plan.stride) {
+        if (chunk + plan.stride < chunk_end) prefetch(t0 + (chunk + plan.stride) * kChunk);
         ChunkStage<D>& st = static_cast<ChunkStage<D>*>(plan.stages)[static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h];
-        // decays within blocks of 8 (f[0]), 8's halves (f[1]), 4's (f[2])
-        // and 2's (f[3]): upper tokens from the middle, lower ones to it
-        float2 f1[8], f2[8], pre[8], suf[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) al[i] = make_float2(expf(al[i].x), expf(al[i].y));
+        {
+            const uint32_t top[3] = {token_tops(kk, lane), token_tops(qq, lane), token_tops(al, lane)};
+            if (lane % 4 == 0)
+#pragma unroll
+                for (int e = 0; e < 3; ++e) sc.top[e][warp][4 * th + lane / 4 % 4] = top[e];
+            // q_i . k_i over the warp's channels: each exchange halves the
+            // values that a lane still sums; lane l ends with token l / 2 % 8
+            float d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = fmaf(qq[i].x, kk[i].x, qq[i].y * kk[i].y);
+#pragma unroll
+            for (int w = 8; w > 1; w >>= 1)
+#pragma unroll
+                for (int i = 0; i < w / 2; ++i) {
+                    const bool up = lane & w;
+                    const float give = up ? d[i] : d[i + w / 2], keep = up ? d[i + w / 2] : d[i];
+                    d[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+                }
+            d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+            if (lane % 2 == 0) sc.diag[warp][8 * th + lane % 16 / 2] = d[0];
+        }
+        if (threadIdx.x < kChunk) sc.beta[threadIdx.x] = bb;
+        __syncthreads();
+        float ftotal;   // p_15's power
+        {   // the tokens' powers of two, a lane each, every warp for itself
+            const uint32_t tok = lane % 16;
+            uint32_t top[3];
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                top[e] = 0;
+#pragma unroll
+                for (int w = 0; w < NP; ++w) top[e] = max(top[e], static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(sc.top[e][w])[tok]));
+            }
+            const int ek = scale_exp(__uint_as_float(top[0] << 16)), z = scale_exp(__uint_as_float(top[1] << 16));
+            const bool sized = top[0] && top[0] < 0x7f80;
+            const int least = __reduce_min_sync(0xffffffffu, sized ? ek : 1000), x = least == 1000 ? 0 : least;
+            const int dx = sized ? min(kKeySpread, ek - x) : 0;
+            // 2^ae over the decay's largest channel (up to 1.008 counts as 1)
+            const int ae = (top[2] >= 0x3f00 && top[2] <= 0x3f80) || top[2] >= 0x7f80 ? 0 : max(kLeastDecay, static_cast<int>(top[2] >> 7) - 126);
+            int sum = ae;
+#pragma unroll
+            for (int o = 1; o < kChunk; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, sum, o, kChunk);
+                if (tok >= static_cast<uint32_t>(o)) sum += y;
+            }
+            if (__any_sync(0xffffffffu, ae > 0)) {   // a decay that grows: the limits apply token by token
+                int y = 0;
+                for (int i = 0; i < kChunk; ++i) {
+                    y = max(kLeastDecay, min(-kLeastDecay, y + __shfl_sync(0xffffffffu, ae, i, kChunk)));
+                    if (tok == static_cast<uint32_t>(i)) sum = y;
+                }
+            } else {
+                sum = max(sum, kLeastDecay);
+            }
+            const int before = __shfl_up_sync(0xffffffffu, sum, 1, kChunk), end = __shfl_sync(0xffffffffu, sum, 15, kChunk), mid = end >> 1;
+            if (lane < 16) {
+                sc.sk[warp][tok] = exp2i(x + dx);
+                sc.sq[warp][tok] = exp2i(z);
+                sc.sa[warp][tok] = exp2i((tok ? before : 0) - sum);
+                if (warp == 0) {
+                    sc.beta[tok] *= exp2i(-2 * dx);
+                    sc.ft[tok] = exp2i(dx - sum + mid);
+                    sc.fp[tok] = two_to(sum - mid - z);
+                    sc.fd[tok] = exp2i(dx + sum - mid);
+                    st.fq[tok] = two_to(sum - z);
+                    if (lane == 0) {
+                        sc.fx = two_to(-x);
+                        sc.wexp = mid + 20 - x;
+                        st.exp = end - mid - x;
+                    }
+                }
+            }
+            ftotal = exp2i(end);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&sc.sa[warp][8 * th + i]);
+            const float4 y = *reinterpret_cast<const float4*>(&sc.sk[warp][8 * th + i]);
+            const float4 z = *reinterpret_cast<const float4*>(&sc.sq[warp][8 * th + i]);
+            const float fa[4] = {x.x, x.y, x.z, x.w}, fk[4] = {y.x, y.y, y.z, y.w}, fq[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                al[i + e] = mul1(al[i + e], fa[e]);
+                kk[i + e] = mul1(kk[i + e], fk[e]);
+                qq[i + e] = mul1(qq[i + e], fq[e]);
+            }
+        }
+        // decays within blocks of 8 (pre, suf), 8's halves (f1), 4's (f2) and
+        // 2's (al): upper tokens from the middle, lower ones to it
+        float2 f1[8], f2[8], pre[8], suf[8];
         const float2 one = make_float2(1.0f, 1.0f);
 #pragma unroll
         for (int b = 0; b < 8; b += 4) {
@@ -435,87 +640,39 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
         }
         // the other half's whole decay
         const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, pre[7].x, 16), __shfl_xor_sync(0xffffffffu, pre[7].y, 16));
-        float2 kp[8], qp[8], ke[8];
+        if (th) *reinterpret_cast<float2*>(&st.total[c]) = mul1(mul2(pre[7], other), ftotal);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            const int tok = 8 * th + i;
+            const float2 ks = kk[i], qs = qq[i];
             const float2 from = th ? mul2(pre[i], other) : pre[i], to = th ? suf[i] : mul2(suf[i], other);
-            kp[i] = mul2(kk[i], from);
-            qp[i] = mul2(qq[i], from);
-            ke[i] = mul2(kk[i], to);
-        }
-        {
-            uint32_t top[6] = {warp_top(kp), warp_top(qp), warp_top(ke), warp_top(kk), warp_top(qq), warp_top(al)};
-            if (lane == 0)
-#pragma unroll
-                for (int e = 0; e < 6; ++e) sc.top[e][warp] = top[e];
-            // q_i . k_i over the warp's channels: each exchange halves the
-            // values that a lane still sums; lane l ends with token l / 2 % 8
-            float d[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = fmaf(qq[i].x, kk[i].x, qq[i].y * kk[i].y);
-#pragma unroll
-            for (int w = 8; w > 1; w >>= 1)
-#pragma unroll
-                for (int i = 0; i < w / 2; ++i) {
-                    const bool up = lane & w;
-                    const float give = up ? d[i] : d[i + w / 2], keep = up ? d[i + w / 2] : d[i];
-                    d[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
-                }
-            d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
-            if (lane % 2 == 0) sc.diag[warp][8 * th + lane % 16 / 2] = d[0];
-        }
-        if (threadIdx.x < kChunk) sc.beta[threadIdx.x] = bb;
-        if (th) *reinterpret_cast<float2*>(&st.total[c]) = mul2(pre[7], other);
-        __syncthreads();
-        int ex[6];
-#pragma unroll
-        for (int e = 0; e < 6; ++e) {
-            uint32_t top = sc.top[e][0];
-#pragma unroll
-            for (int w = 1; w < NP; ++w) top = max(top, sc.top[e][w]);
-            ex[e] = e < 5 ? scale_exp(__uint_as_float(top))
-                          // a block's decays pass 1 only where a token's do: by its 8th power at most
-                          : top > 0x3f800000u ? 8 * (static_cast<int>(top >> 23) - 126) : 0;
-        }
-        const int lk = max(-126, ex[3] - ex[5]), lq = max(-126, ex[4] - ex[5]);   // the level operands' powers
-        {
-            const float sk = exp2i(ex[0]), sq = exp2i(ex[1]), se = exp2i(ex[2]), xk = exp2i(lk), xq = exp2i(lq);
-            if (threadIdx.x == 0) {
-                st.exps[1] = ex[1];
-                st.exps[2] = ex[2];
+            store_pair(sc.k, tok, c, mul2(ks, from));
+            store_pair(st.q, tok, c, mul2(qs, from));
+            store_pair(st.ke, tok, c, mul2(ks, to));
+            // blocks of 16: the second half is upper
+            const float2 g = th ? pre[i] : suf[i], k0 = mul2(ks, g);
+            store_pair(sc.level[0], th ? i : 16 + i, c, k0);
+            if (th) {
+                const float2 q0 = mul2(qs, g);
+                store_pair(sc.level[0], 8 + i, c, q0);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int tok = 8 * th + i;
-                store_pair(sc.k, tok, c, mul1(kp[i], sk));
-                store_pair(st.q, tok, c, mul1(qp[i], sq));
-                store_pair(st.ke, tok, c, mul1(ke[i], se));
-                const float2 ks = mul1(kk[i], xk), qs = mul1(qq[i], xq);
-                // blocks of 16: the second half is upper
-                const float2 g = th ? pre[i] : suf[i], k0 = mul2(ks, g);
-                store_pair(sc.level[0], th ? i : 16 + i, c, k0);
-                if (th) {
-                    const float2 q0 = mul2(qs, g);
-                    store_pair(sc.level[0], 8 + i, c, q0);
-                }
-#pragma unroll
-                for (int l = 1; l < 4; ++l) {
-                    const int half = 8 >> l;
-                    const int row = 4 * th + i / (2 * half) * half + i % half;   // of its side's 8
-                    const float2 f = l == 1 ? f1[i] : l == 2 ? f2[i] : i % 2 ? al[i] : one;
-                    const float2 kl = mul2(ks, f);
-                    if (i & half) {
-                        const float2 ql = mul2(qs, f);
-                        store_pair(sc.level[l], row, c, kl);
-                        store_pair(sc.level[l], 8 + row, c, ql);
-                    } else {
-                        store_pair(sc.level[l], 16 + row, c, kl);
-                    }
+            for (int l = 1; l < 4; ++l) {
+                const int half = 8 >> l;
+                const int row = 4 * th + i / (2 * half) * half + i % half;   // of its side's 8
+                const float2 f = l == 1 ? f1[i] : l == 2 ? f2[i] : i % 2 ? al[i] : one;
+                const float2 kl = mul2(ks, f);
+                if (i & half) {
+                    const float2 ql = mul2(qs, f);
+                    store_pair(sc.level[l], row, c, kl);
+                    store_pair(sc.level[l], 8 + row, c, ql);
+                } else {
+                    store_pair(sc.level[l], 16 + row, c, kl);
                 }
             }
         }
-        __syncthreads();
         if (chunk + plan.stride < chunk_end) fetch(t0 + (chunk + plan.stride) * kChunk);
+        __syncthreads();
         for (int l = warp; l < 4; l += NP) {
             float b[4] = {}, x[4] = {};
 #pragma unroll
@@ -534,19 +691,19 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                 }
             }
             const int half = 8 >> l, u = lane / 4, i = u / half * 2 * half + half + u % half;
-            const float fk = pow2(-lk), fq = pow2(-lq);
+            const float fx = sc.fx;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int w = lane % 4 * 2 + e, j = w / half * 2 * half + w % half;
                 if (u / half != w / half) continue;
-                sc.At[j][i] = (b[e] + x[e]) * fk * fk;
-                sc.P[i][j] = (b[2 + e] + x[2 + e]) * fk * fq;
+                sc.At[j][i] = (b[e] + x[e]) * fx * fx;
+                sc.P[i][j] = (b[2 + e] + x[2 + e]) * sc.fp[i] * fx;
             }
         }
         __syncthreads();
         if (warp == 0) {   // T, a lane per column, one row's multiple after the other
             const uint32_t j = lane % 16;
-            float x[kChunk], top = 0.0f;
+            float x[kChunk];
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) x[i] = 0.0f;
 #pragma unroll
@@ -557,47 +714,43 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
             }
             const float b = sc.beta[j];
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-                x[i] *= b;
-                top = fmaxf(top, fabsf(x[i]));
-            }
-            const int e = scale_exp(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
-            if (lane == 0) {
-                st.exps[3] = e;
-                st.exps[0] = e + ex[0] - 20;
-            }
-            const float f = exp2i(e);
-            if (lane < 16)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) {
-                    split_half(x[i] * f, sc.t[0][i][j], sc.t[1][i][j]);
-                    st.t[0][i][j] = sc.t[0][i][j];
-                    st.t[1][i][j] = sc.t[1][i][j];
-                }
-        }
-        if (warp == NP - 1) {   // P
-            float x[8], top = 0.0f;
-            const int j = lane % 16;
-#pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                const int i = 2 * m + lane / 16;
-                x[m] = i > j ? sc.P[i][j] : 0.0f;
-                if (i == j)
-#pragma unroll
-                    for (int w = 0; w < NP; ++w) x[m] += sc.diag[w][i];
-                top = fmaxf(top, fabsf(x[m]));
-            }
-            const int e = scale_exp(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))));
-            if (lane == 0) st.exps[4] = e;
-            const float f = exp2i(e);
-#pragma unroll
-            for (int m = 0; m < 8; ++m) split_half(x[m] * f, st.p[0][2 * m + lane / 16][j], st.p[1][2 * m + lane / 16][j]);
+            for (int i = 0; i < kChunk / 2; ++i) sc.T[8 * th + i][j] = (th ? x[8 + i] : x[i]) * b;   // a half warp has half of the rows
         }
         __syncthreads();
+        for (int e = threadIdx.x; e < kChunk * kChunk / 2; e += D) {   // T and P for the scan
+            const int i = e / 8, j = e % 8 * 2;
+            uint32_t w[3];
+            split_bf16(mul2(*reinterpret_cast<const float2*>(&sc.T[i][j]), *reinterpret_cast<const float2*>(&sc.ft[j])), w);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) *reinterpret_cast<uint32_t*>(&st.t[n][i][j]) = w[n];
+            float2 x = *reinterpret_cast<const float2*>(&sc.P[i][j]);
+            float diag = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) diag += sc.diag[n][i];
+            diag *= sc.fd[i];
+            x.x = i > j ? x.x : i == j ? diag : 0.0f;
+            x.y = i > j + 1 ? x.y : i == j + 1 ? diag : 0.0f;
+            split_bf16(x, w);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) *reinterpret_cast<uint32_t*>(&st.p[n][i][j]) = w[n];
+        }
         {   // W = T (p K): 16 sums of products below 2^30, kept as multiples of 2^20
+            float x[2][4];   // rows lane / 4 and 8 on, each by a power of its own
+            int e[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = *reinterpret_cast<const float2*>(&sc.T[lane / 4 + 8 * (i % 2)][8 * (i / 2) + lane % 4 * 2]);
+                x[i / 2][i % 2 * 2] = v.x;
+                x[i / 2][i % 2 * 2 + 1] = v.y;
+            }
+            row_exps(x, e);
+            if (warp == 0 && lane % 4 < 2) st.fw[lane / 4 + lane % 4 * 8] = two_to(sc.wexp - (lane % 4 ? e[1] : e[0]));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[i][n] *= exp2i(e[n / 2]);
             uint32_t xh[4], xl[4];
-            ldmatrix4<false>(xh, &sc.t[0][arow][acol]);
-            ldmatrix4<false>(xl, &sc.t[1][arow][acol]);
+            split_rows(x[0], x[1], xh, xl);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int col = warp * 32 + 16 * j;
@@ -618,29 +771,6 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
     }
 }
 
-// Row maxima of two rows over a quad's lanes, and as scale exponents.
-__device__ __forceinline__ float2 row_exps(float m0, float m1, int (&ex)[2]) {
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-    }
-    ex[0] = scale_exp(m0);
-    ex[1] = scale_exp(m1);
-    return make_float2(m0, m1);
-}
-__device__ __forceinline__ float2 row_exps(const float (&x)[2][4], int (&ex)[2]) {
-    return row_exps(fmaxf(fmaxf(fabsf(x[0][0]), fabsf(x[0][1])), fmaxf(fabsf(x[1][0]), fabsf(x[1][1]))),
-             fmaxf(fmaxf(fabsf(x[0][2]), fabsf(x[0][3])), fmaxf(fabsf(x[1][2]), fabsf(x[1][3]))), ex);
-}
-
-// [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
-__device__ __forceinline__ void split_rows(const float (&x)[4], const float (&y)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-    split_pair(make_float2(x[0], x[1]), hi[0], lo[0]);
-    split_pair(make_float2(x[2], x[3]), hi[1], lo[1]);
-    split_pair(make_float2(y[0], y[1]), hi[2], lo[2]);
-    split_pair(make_float2(y[2], y[3]), hi[3], lo[3]);
-}
 template <int D, int NW, int KS>
 struct __align__(128) ScanSmem {
     ChunkStage<D> stage[kStages];
@@ -729,6 +859,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
         return;
     }
     constexpr int DK = D / KS;   // this warp's key channels, from k0 on
+    constexpr int NV = sizeof(E) == 2 ? 1 : 3;   // bf16 values are one term
     const uint32_t half = warp % KS, k0 = half * DK;
     const uint32_t row0 = blockIdx.x % slices * (16 * NW) + warp / KS * 16;
     const uint32_t g = lane / 4, t = lane % 4, P = a.heads * D;
@@ -766,8 +897,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
     for (uint32_t n = 0; chunk + n < chunk_end; ++n) {
         const uint32_t first = t0 + (chunk + n) * kChunk;
         const ChunkStage<D>& st = stages[n % kStages];
-        int vx[2], ux[2];
-        const float2 top = row_exps(vv, vx);
+        int ux[2];
         {
             float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
@@ -781,14 +911,17 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
                 m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
             }
             // a row's multiple changes when its largest element leaves
-            // [2^8, 2^15]: f16 holds it then, with 32 bits below it. It stays
-            // below 2^40 over that of the values to come, so that a small
-            // state's multiple does not carry their sums past a float's end.
-            const int cap0 = top.x == 0.0f ? 126 : min(126, vx[0] + 40), cap1 = top.y == 0.0f ? 126 : min(126, vx[1] + 40);
-            const bool off0 = m0 > 0x1p15f || (m0 < 0x1p8f && m0 != 0.0f && sx[0] < cap0) || sx[0] > cap0;
-            const bool off1 = m1 > 0x1p15f || (m1 < 0x1p8f && m1 != 0.0f && sx[1] < cap1) || sx[1] > cap1;
+            // [2^8, 2^15]: f16 holds it then, with 32 bits below it
+            const bool off0 = m0 > 0x1p15f || (m0 < 0x1p8f && m0 != 0.0f && sx[0] < 126) || sx[0] > 30;
+            const bool off1 = m1 > 0x1p15f || (m1 < 0x1p8f && m1 != 0.0f && sx[1] < 126) || sx[1] > 30;
             if (__any_sync(0xffffffffu, off0 || off1)) {
-                const int d0 = off0 ? min(scale_exp(m0) - 2, cap0 - sx[0]) : 0, d1 = off1 ? min(scale_exp(m1) - 2, cap1 - sx[1]) : 0;
+                // it stays below 2^40 over that of the values to come, so that a
+                // small state's multiple does not carry their sums past a float's end
+                int vx[2];
+                const float2 top = row_exps(vv, vx);
+                const int cap0 = top.x == 0.0f ? 126 : min(126, vx[0] + 40), cap1 = top.y == 0.0f ? 126 : min(126, vx[1] + 40);
+                const bool in0 = m0 == 0.0f || (m0 >= 0x1p8f && m0 <= 0x1p15f), in1 = m1 == 0.0f || (m1 >= 0x1p8f && m1 <= 0x1p15f);
+                const int d0 = min(in0 ? 0 : scale_exp(m0) - 2, cap0 - sx[0]), d1 = min(in1 ? 0 : scale_exp(m1) - 2, cap1 - sx[1]);
                 const float f0 = pow2(d0), f1 = pow2(d1);
                 sx[0] += d0;
                 sx[1] += d1;
@@ -801,26 +934,15 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
                 }
             }
         }
-        uint32_t xh[4], xl[4], yh[4], yl[4];
-        {
-            const float f0 = exp2i(vx[0]), f1 = exp2i(vx[1]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                vv[i][0] *= f0;
-                vv[i][1] *= f0;
-                vv[i][2] *= f1;
-                vv[i][3] *= f1;
-            }
-            split_rows(vv[0], vv[1], xh, xl);
-        }
+        uint32_t xh[4], xl[4], yh[4], yl[4], vw[3][4];
+        split_tokens<NV>(vv, vw);
         if (chunk + n + 1 < chunk_end) fetch(first + kChunk);
         tc::mbar_pass(&bar.full[n % kStages], n / kStages & 1u, abort);
         __syncwarp();
+        uint32_t uw[3][4];
         // T V, W S0^T and (p Q) S0^T
         float u[2][4] = {}, wb[2][4] = {}, ws[2][4] = {}, ob[2][4] = {}, os[2][4] = {};
-        ldmatrix4<false>(yh, &st.t[0][mrow][mcol]);
-        ldmatrix4<false>(yl, &st.t[1][mrow][mcol]);
-        mma_terms1(u, xh, xl, yh, yl);
+        mma_tokens<NV>(u, vw, &st.t[0][mrow][mcol]);
 #pragma unroll
         for (int j = 0; j < DK / 16; ++j) {
             split_rows(S[2 * j], S[2 * j + 1], xh, xl);
@@ -832,18 +954,16 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
             mma_terms(ob, os, xh, xl, yh, yl);
         }
         {
-            // products of two powers: their exponents' sum may pass a normal
-            // float's (small values, a small state)
-            const float fs[2] = {pow2(-sx[0]), pow2(-sx[1])}, ft = pow2(-st.exps[3]), fv[2] = {pow2(-vx[0]), pow2(-vx[1])};
-            const float fw[2] = {pow2(-st.exps[0]) * fs[0], pow2(-st.exps[0]) * fs[1]};
-            const float fq[2] = {pow2(-st.exps[1]) * fs[0], pow2(-st.exps[1]) * fs[1]};
+            const float fs[2] = {pow2(-sx[0]), pow2(-sx[1])};
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
+                const float2 fw = *reinterpret_cast<const float2*>(&st.fw[8 * i + 2 * t]), fq = *reinterpret_cast<const float2*>(&st.fq[8 * i + 2 * t]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    wb[i][e] = (wb[i][e] + ws[i][e]) * fw[e / 2];
-                    ob[i][e] = (ob[i][e] + os[i][e]) * fq[e / 2];
+                    wb[i][e] = (wb[i][e] + ws[i][e]) * fs[e / 2] * (e % 2 ? fw.y : fw.x);
+                    ob[i][e] = (ob[i][e] + os[i][e]) * fs[e / 2] * (e % 2 ? fq.y : fq.x);
                 }
+            }
             if constexpr (KS > 1) {   // the halves' sums, in the same order in both warps
                 float4 (*part)[2][2][32] = bar.part[n % 2][warp / KS];
 #pragma unroll
@@ -862,23 +982,21 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[i][e] = fmaf(u[i][e] * ft, fv[e / 2], -wb[i][e]);
+                for (int e = 0; e < 4; ++e) u[i][e] -= wb[i][e];
+            split_tokens<3>(u, uw);
             row_exps(u, ux);
-            // a product's two powers together stay within a float's
-            ux[0] = min(ux[0], 126 - max(st.exps[2], st.exps[4]));
-            ux[1] = min(ux[1], 126 - max(st.exps[2], st.exps[4]));
+            // a product's powers together stay within a float's
+            ux[0] = min(ux[0], 126 + sx[0] + st.exp);
+            ux[1] = min(ux[1], 126 + sx[1] + st.exp);
             const float f0 = pow2(ux[0]), f1 = pow2(ux[1]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                u[i][0] *= f0;
-                u[i][1] *= f0;
-                u[i][2] *= f1;
-                u[i][3] *= f1;
-            }
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[i][e] *= e < 2 ? f0 : f1;
             split_rows(u[0], u[1], xh, xl);
         }
         {   // S = S diag(total) + U^T (e K)
-            const float f0 = pow2(sx[0] - ux[0] - st.exps[2]), f1 = pow2(sx[1] - ux[1] - st.exps[2]);
+            const float f0 = pow2(sx[0] - ux[0] + st.exp), f1 = pow2(sx[1] - ux[1] + st.exp);
 #pragma unroll
             for (int j = 0; j < DK / 16; ++j) {
                 float c[2][4] = {};
@@ -899,17 +1017,14 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
         }
         {   // O = (p Q) S0^T + P U
             float c[2][4] = {};
-            ldmatrix4<false>(yh, &st.p[0][mrow][mcol]);
-            ldmatrix4<false>(yl, &st.p[1][mrow][mcol]);
-            mma_terms1(c, xh, xl, yh, yl);
-            const float fp[2] = {pow2(-ux[0] - st.exps[4]), pow2(-ux[1] - st.exps[4])};
+            mma_tokens<3>(c, uw, &st.p[0][mrow][mcol]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (KS > 1 && i != static_cast<int>(half)) continue;   // a half writes one tile of tokens
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t tok = first + 8 * i + 2 * t + e % 2;
-                    const float o = fmaf(c[i][e], fp[e / 2], ob[i][e]);
+                    const float o = c[i][e] + ob[i][e];
                     if (tok < t1) store1<E>(a.out, static_cast<size_t>(tok) * P + h * D + row0 + g + 8 * (e / 2), o);
                 }
             }

@@ -1,5 +1,6 @@
 """k3xb_kda_prefill value by value: every token's row of outputs and every row
-of the state against the rule in 64 bits, at magnitudes all over a float's range.
+of the state against the rule in 64 bits, with inputs whose tokens differ by
+many orders of magnitude.
 
 Tolerances. Let R be a value row's content without cancellation: a token takes
 it to max(a) R + |beta| (|v| + |S| |a k|) |k| (2-norms over the key channels; R
@@ -135,6 +136,40 @@ def test_small_and_large_values(torch, ctx, scale, where):
         x[2] *= 1e10
     state[..., rows, :] *= scale
     _run(torch, ctx, x, [60], state)
+
+
+@pytest.mark.parametrize("gate", ["mixed", "none", "fast"])
+@pytest.mark.parametrize("which,low,high", [("q", -10, 10), ("k", -8, 0), ("v", -10, 10), ("beta", -10, 0), ("all", -6, 0)])
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+def test_tokens_of_unlike_size(torch, ctx, gate, which, low, high, kind):
+    x = _inputs(torch, 75, 2, 128, 17, gate)
+    g = torch.Generator().manual_seed(len(which) + high)
+    for i, n in enumerate(NAMES):
+        if n in (which, "log_decay") or (which == "all" and n != "log_decay"):
+            if n != "log_decay":
+                f = 10.0 ** (low + (high - low) * torch.rand(75, 2, generator=g))
+                x[i] = x[i] * (f if n == "beta" else f[..., None]).cuda()
+    _run(torch, ctx, x, [75], _state(torch, 1, 2, 128), getattr(torch, kind))
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "beta"])
+@pytest.mark.parametrize("size", [1e10, 1e-10, 0.0])
+@pytest.mark.parametrize("at", [15, 31, 36])
+def test_one_token_of_another_size(torch, ctx, which, size, at):
+    """The tokens before it, in its chunk too, keep their accuracy."""
+    x = _inputs(torch, 37, 2, 128, 19)
+    x[NAMES.index(which)][at] *= size
+    _run(torch, ctx, x, [37], _state(torch, 1, 2, 128))
+
+
+@pytest.mark.parametrize("at", [0, 1, 24, 31])
+def test_content_that_is_forgotten_at_once(torch, ctx, at):
+    """A token that empties every channel after contents of 1e9, and small ones behind it."""
+    x = _inputs(torch, 45, 2, 128, 21)
+    x[3][at] = -60.0
+    x[2][at:] *= 1e-3
+    x[2][:at] *= 1e6
+    _run(torch, ctx, x, [45], 1e9 * _state(torch, 1, 2, 128))
 
 
 def test_one_head_or_sequence_of_another_size(torch, ctx):
