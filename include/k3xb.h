@@ -540,10 +540,15 @@ int k3xb_kda_commit(k3xb_ctx* ctx, const float* state, const int32_t* parent,
  * (state [S][h][d][d], V-first, NULL: zeros) and after (state_out, NULL: not
  * kept; may be `state`) are float; an empty sequence's state is copied.
  * out [tokens][h*d] of `type`, each value rounded once. head_dim 32, 64 or
- * 128; states 16-byte aligned. All sums are float-precision sums in an order of their own:
- * results agree with the token-by-token calls to float tolerance, not bit
- * for bit (k3xb_kda_tree keeps the reference's order). Offsets that are no
- * ranges leave their sequences out and k3xb_sync reports INVALID_EXTENT. */
+ * 128; states 16-byte aligned. All sums are float-precision sums in an order
+ * of their own: results agree with the token-by-token calls to float
+ * tolerance, not bit for bit (k3xb_kda_tree keeps the reference's order). Each
+ * output is off by roundings of its own query's size times its own state row's,
+ * whatever the sizes of the other tokens (keys up to 2^40 apart within 16
+ * tokens); no token's outputs depend on a later one. What an infinity or NaN
+ * reaches by the rule becomes an infinity or NaN, and nothing else does.
+ * Offsets that are no ranges leave their sequences out and k3xb_sync reports
+ * INVALID_EXTENT. */
 int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
                      uint64_t row_stride, int32_t type, const float* log_decay,
                      const float* beta, const uint32_t* offsets, uint32_t sequences,

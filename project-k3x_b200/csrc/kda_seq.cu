@@ -232,9 +232,12 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // in place of b, v, u and o: the powers go to T's columns, P's rows and
 // the rows' factors fw and fq. So an output is off by float roundings of its
 // own query times its own row's content, and no later token changes it.
+//
+// Infinities and NaN become NaN where the rule takes them: in their token's
+// outputs and, but for a query's, in all later ones (a value's or a state's in its own row).
 
 constexpr int kChunk = 16, kStages = 3;
-constexpr int kKeySpread = 40, kLeastDecay = -40;
+constexpr int kKeySpread = 40, kLeastDecay = -40, kMostDecay = 100;
 // Operands held at a time: longer batches go in segments of chunks.
 constexpr size_t kOperandBytes = size_t(1) << 30;
 
@@ -452,6 +455,27 @@ __device__ __forceinline__ float2 row_exps(const float (&x)[2][4], int (&ex)[2])
              fmaxf(fmaxf(fabsf(x[0][2]), fabsf(x[0][3])), fmaxf(fabsf(x[1][2]), fabsf(x[1][3]))), ex);
 }
 
+// The first tokens of two rows (16 tokens in accumulator layout) whose elements
+// are not finite (kChunk: none; the second row's above the first's 8 bits);
+// zeros take the place of such elements.
+constexpr int kNone = kChunk | kChunk << 8;
+__device__ __forceinline__ int first_bad(float (&x)[2][4], uint32_t t) {
+    int bad[2] = {kChunk, kChunk};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!isfinite(x[i][e])) {
+                bad[e / 2] = min(bad[e / 2], static_cast<int>(8 * i + 2 * t) + e % 2);
+                x[i][e] = 0.0f;
+            }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) bad[r] = min(bad[r], __shfl_xor_sync(0xffffffffu, bad[r], o));
+    return bad[0] | bad[1] << 8;
+}
+
 // [16 rows][16] in accumulator layout (two n-tiles) as the two terms of a left operand.
 __device__ __forceinline__ void split_rows(const float (&x)[4], const float (&y)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
     split_pair(make_float2(x[0], x[1]), hi[0], lo[0]);
@@ -541,7 +565,8 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
         }
         if (threadIdx.x < kChunk) sc.beta[threadIdx.x] = bb;
         __syncthreads();
-        float ftotal;   // p_15's power
+        float ftotal;      // p_15's power
+        uint32_t poison;   // the first token with a key, decay or beta that is not finite
         {   // the tokens' powers of two, a lane each, every warp for itself
             const uint32_t tok = lane % 16;
             uint32_t top[3];
@@ -552,11 +577,14 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                 for (int w = 0; w < NP; ++w) top[e] = max(top[e], static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(sc.top[e][w])[tok]));
             }
             const int ek = scale_exp(__uint_as_float(top[0] << 16)), z = scale_exp(__uint_as_float(top[1] << 16));
-            const bool sized = top[0] && top[0] < 0x7f80;
+            const float be = sc.beta[tok];
+            const uint32_t odd = __ballot_sync(0xffffffffu, top[0] >= 0x7f80 || top[2] >= 0x7f80 || !(fabsf(be) < INFINITY));
+            poison = odd ? min(16, __ffs(odd) - 1) : 16;
+            const bool sized = top[0] && tok < poison;
             const int least = __reduce_min_sync(0xffffffffu, sized ? ek : 1000), x = least == 1000 ? 0 : least;
             const int dx = sized ? min(kKeySpread, ek - x) : 0;
             // 2^ae over the decay's largest channel (up to 1.008 counts as 1)
-            const int ae = (top[2] >= 0x3f00 && top[2] <= 0x3f80) || top[2] >= 0x7f80 ? 0 : max(kLeastDecay, static_cast<int>(top[2] >> 7) - 126);
+            const int ae = (top[2] >= 0x3f00 && top[2] <= 0x3f80) || tok >= poison ? 0 : max(kLeastDecay, min(kMostDecay, static_cast<int>(top[2] >> 7) - 126));
             int sum = ae;
 #pragma unroll
             for (int o = 1; o < kChunk; o <<= 1) {
@@ -566,7 +594,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
             if (__any_sync(0xffffffffu, ae > 0)) {   // a decay that grows: the limits apply token by token
                 int y = 0;
                 for (int i = 0; i < kChunk; ++i) {
-                    y = max(kLeastDecay, min(-kLeastDecay, y + __shfl_sync(0xffffffffu, ae, i, kChunk)));
+                    y = max(kLeastDecay, min(kMostDecay, y + __shfl_sync(0xffffffffu, ae, i, kChunk)));
                     if (tok == static_cast<uint32_t>(i)) sum = y;
                 }
             } else {
@@ -578,11 +606,11 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                 sc.sq[warp][tok] = exp2i(z);
                 sc.sa[warp][tok] = exp2i((tok ? before : 0) - sum);
                 if (warp == 0) {
-                    sc.beta[tok] *= exp2i(-2 * dx);
-                    sc.ft[tok] = exp2i(dx - sum + mid);
+                    sc.beta[tok] = tok < poison ? be * exp2i(-2 * dx) : 0.0f;
+                    sc.ft[tok] = pow2(dx - sum + mid);
                     sc.fp[tok] = two_to(sum - mid - z);
-                    sc.fd[tok] = exp2i(dx + sum - mid);
-                    st.fq[tok] = two_to(sum - z);
+                    sc.fd[tok] = pow2(dx + sum - mid);
+                    st.fq[tok] = tok < poison ? two_to(sum - z) : NAN;
                     if (lane == 0) {
                         sc.fx = two_to(-x);
                         sc.wexp = mid + 20 - x;
@@ -590,7 +618,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                     }
                 }
             }
-            ftotal = exp2i(end);
+            ftotal = poison < 16 ? NAN : exp2i(end);
         }
         __syncwarp();
 #pragma unroll
@@ -671,6 +699,12 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                 }
             }
         }
+        // From `poison` on fq, and at the end the state's factor, are NaN. Zeros
+        // in p K and T keep the tokens before clear of it (T's and P's own zeros
+        // times a NaN would not).
+        if (poison < 16)
+            for (int i = max(0, static_cast<int>(poison) - static_cast<int>(8 * th)); i < 8; ++i)
+                store_pair(sc.k, 8 * th + i, c, make_float2(0.0f, 0.0f));
         if (chunk + plan.stride < chunk_end) fetch(t0 + (chunk + plan.stride) * kChunk);
         __syncthreads();
         for (int l = warp; l < 4; l += NP) {
@@ -714,7 +748,8 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
             }
             const float b = sc.beta[j];
 #pragma unroll
-            for (int i = 0; i < kChunk / 2; ++i) sc.T[8 * th + i][j] = (th ? x[8 + i] : x[i]) * b;   // a half warp has half of the rows
+            for (int i = 0; i < kChunk / 2; ++i)   // a half warp has half of the rows
+                sc.T[8 * th + i][j] = 8 * th + i < poison ? (th ? x[8 + i] : x[i]) * b : 0.0f;
         }
         __syncthreads();
         for (int e = threadIdx.x; e < kChunk * kChunk / 2; e += D) {   // T and P for the scan
@@ -894,12 +929,27 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
     // k-major ones, transposed (lanes 0-7: tile 0, k 0-7; 8-15: k 8-15; 16-31: tile 1)
     const uint32_t krow = lane % 16, kcol = lane / 16 * 8;
     int sx[2] = {0, 0};   // S holds the state's rows times 2^sx
+    // A value that is not finite would meet T's zeros above the diagonal: a
+    // zero stands for it, and after the chunk its row's state and this lane's
+    // outputs from its token on become NaN.
+    int spoilt = kNone;
+    auto spoil = [&](uint32_t first) {
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t at = 8 * (i / 4) + 2 * t + i % 2, r = i / 2 % 2;
+            if ((KS > 1 && i / 4 != static_cast<int>(half)) || static_cast<int>(at) < (r ? spoilt >> 8 : spoilt & 255) || first + at >= t1) continue;
+            store1<E>(a.out, static_cast<size_t>(first + at) * P + h * D + row0 + g + 8 * r, NAN);
+        }
+    };
     for (uint32_t n = 0; chunk + n < chunk_end; ++n) {
         const uint32_t first = t0 + (chunk + n) * kChunk;
         const ChunkStage<D>& st = stages[n % kStages];
         int ux[2];
         {
-            float m0 = 0.0f, m1 = 0.0f;
+            float m0 = 0.0f, m1 = 0.0f, zero[2] = {0.0f, 0.0f};   // zero: NaN where a value is not finite
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) zero[i] = fmaf(vv[i][e], 0.0f, zero[i]);
 #pragma unroll
             for (int j = 0; j < DK / 8; ++j) {
                 m0 = fmaxf(m0, fmaxf(fabsf(S[j][0]), fabsf(S[j][1])));
@@ -914,7 +964,10 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
             // [2^8, 2^15]: f16 holds it then, with 32 bits below it
             const bool off0 = m0 > 0x1p15f || (m0 < 0x1p8f && m0 != 0.0f && sx[0] < 126) || sx[0] > 30;
             const bool off1 = m1 > 0x1p15f || (m1 < 0x1p8f && m1 != 0.0f && sx[1] < 126) || sx[1] > 30;
-            if (__any_sync(0xffffffffu, off0 || off1)) {
+            if (__any_sync(0xffffffffu, off0 || off1 || zero[0] + zero[1] != 0.0f || spoilt != kNone)) {
+                const int before = spoilt;
+                if (before != kNone) spoil(first - kChunk);
+                spoilt = first_bad(vv, t);
                 // it stays below 2^40 over that of the values to come, so that a
                 // small state's multiple does not carry their sums past a float's end
                 int vx[2];
@@ -922,7 +975,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
                 const int cap0 = top.x == 0.0f ? 126 : min(126, vx[0] + 40), cap1 = top.y == 0.0f ? 126 : min(126, vx[1] + 40);
                 const bool in0 = m0 == 0.0f || (m0 >= 0x1p8f && m0 <= 0x1p15f), in1 = m1 == 0.0f || (m1 >= 0x1p8f && m1 <= 0x1p15f);
                 const int d0 = min(in0 ? 0 : scale_exp(m0) - 2, cap0 - sx[0]), d1 = min(in1 ? 0 : scale_exp(m1) - 2, cap1 - sx[1]);
-                const float f0 = pow2(d0), f1 = pow2(d1);
+                const float f0 = (before & 255) < kChunk ? NAN : pow2(d0), f1 = before >> 8 < kChunk ? NAN : pow2(d1);
                 sx[0] += d0;
                 sx[1] += d1;
 #pragma unroll
@@ -1032,8 +1085,9 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&bar.empty[n % kStages]);
     }
+    if (spoilt != kNone) spoil(t0 + (chunk_end - 1) * kChunk);
     if (!state_out) return;
-    const float f0 = pow2(-sx[0]), f1 = pow2(-sx[1]);
+    const float f0 = (spoilt & 255) < kChunk ? NAN : pow2(-sx[0]), f1 = spoilt >> 8 < kChunk ? NAN : pow2(-sx[1]);
 #pragma unroll
     for (int j = 0; j < DK / 8; ++j) {
         *reinterpret_cast<float2*>(state_out + state_at + 8 * j) = make_float2(S[j][0] * f0, S[j][1] * f0);

@@ -1,6 +1,6 @@
 """k3xb_kda_prefill value by value: every token's row of outputs and every row
 of the state against the rule in 64 bits, with inputs whose tokens differ by
-many orders of magnitude.
+many orders of magnitude, infinities and NaN.
 
 Tolerances. Let R be a value row's content without cancellation: a token takes
 it to max(a) R + |beta| (|v| + |S| |a k|) |k| (2-norms over the key channels; R
@@ -10,6 +10,8 @@ starts at the row's norm). A sum of 128 float products is off by at most 128 *
 depends on a later one. A bf16 output is rounded once more, by 2^-8 of itself.
 Products below the smallest normal float may vanish: 256 * 2^-126 at most.
 """
+import math
+
 import numpy as np
 import pytest
 
@@ -170,6 +172,35 @@ def test_content_that_is_forgotten_at_once(torch, ctx, at):
     x[2][at:] *= 1e-3
     x[2][:at] *= 1e6
     _run(torch, ctx, x, [45], 1e9 * _state(torch, 1, 2, 128))
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which,at,col", [("q", 9, 3), ("k", 9, 100), ("v", 9, 64), ("beta", 9, 0), ("log_decay", 9, 77), ("v", 31, 0),
+                                          ("k", 15, 0), ("k", 0, 5), ("v", 0, 127), ("log_decay", 16, 2), ("q", 34, 8)])
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+def test_infinities_and_nan_reach_later_tokens_only(torch, ctx, bad, which, at, col, kind):
+    if which == "log_decay" and bad == -math.inf:
+        bad = 1e30   # exp gives infinity; -inf is a decay of zero
+    dtype = getattr(torch, kind)
+    x = _inputs(torch, 35, 2, 128, 23)
+    state = _state(torch, 1, 2, 128)
+    clean, _ = _prefill(torch, ctx, x, [35], state, dtype)
+    i = NAMES.index(which)
+    if which == "beta":
+        x[i][at, 0] = bad
+    else:
+        x[i][at, 0, col] = bad
+    out, new = _run(torch, ctx, x, [35], state, dtype)
+    assert torch.equal(out[:at], clean[:at])
+    assert torch.equal(out[:, 1], clean[:, 1]), "the other head"
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_state_rows_do_not_mix(torch, ctx, bad):
+    x = _inputs(torch, 40, 1, 128, 29)
+    state = _state(torch, 1, 1, 128)
+    state[0, 0, 17, 99] = bad
+    _run(torch, ctx, x, [40], state)
 
 
 def test_one_head_or_sequence_of_another_size(torch, ctx):
