@@ -1114,7 +1114,13 @@ int launch_attend_tc(k3xb_ctx* ctx, const AttnArgs& a, bool bf16) {
     p.total = own.prefix ? 0 : p.steps_per_head * a.kv_heads;
     uint32_t ctas = 0;
     if (p.total) {
-        p.range = (p.total + sms - 1) / sms;
+        // A tensor core truncates each sum, 16 keys at a time, so a part of n keys may
+        // be short by n / 16 2^-24: 2^-13 (f16) or 2^-10 (bf16) at most in 2^15 and 2^18
+        // keys, an eighth and a quarter of what rounding the output costs.
+        // Where that many lie in a CTA's range, the ranges go in several rounds.
+        const uint32_t most = bf16 ? 2048 : 256;   // steps
+        const uint64_t rounds = p.blocks > most ? (p.total + static_cast<uint64_t>(sms) * most - 1) / (static_cast<uint64_t>(sms) * most) : 1;
+        p.range = static_cast<uint32_t>((p.total + sms * rounds - 1) / (sms * rounds));
         ctas = (p.total + p.range - 1) / p.range;
         p.max_seg = p.range / (p.odd ? (p.blocks + 1) / 2 : p.blocks) + 2;
         if (static_cast<uint64_t>(ctas) * p.max_seg * 2 * kTile >= (1ull << 31))
