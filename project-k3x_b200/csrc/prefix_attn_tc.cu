@@ -36,6 +36,10 @@ namespace k3xb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+template <bool BF16>
+constexpr float kLazy = BF16 ? 8.0f : 2.0f;
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.0f : 13.0f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -168,9 +172,11 @@ __device__ __forceinline__ Segment segment_at(const PrefixPlan& p, uint32_t x, u
 // next score tile is issued behind the product that reads them.
 //
 // The running maximum is lazy: rows keep an old m until a score passes it by
-// more than 2^8, so that the accumulator is rescaled a few times per row
-// instead of once per block; p <= 2^8 then, which float sums and both 16-bit
-// types hold. The sum is of the unrounded p.
+// more than kLazy powers of two, so that the accumulator is rescaled a few times
+// per row instead of once per block (p <= 2^8 of it then with bf16, 2^2 with
+// f16). The sum is of the unrounded p. f16 ends at 2^-24: there the base that p
+// is relative to lies kLift powers below m, so that p ends at 2^15 and keeps its
+// 11 bits down to 2^-27 of the largest, and 2^-38 of it is the least that counts.
 template <bool BF16, uint32_t NK, uint32_t NV>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_constant__ CUtensorMap map_k,
                                                         const __grid_constant__ CUtensorMap map_e,
@@ -429,9 +435,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
                 if (i == 0) {
                     m = mx;
-                } else if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+                } else if (__any_sync(0xffffffffu, mx > m + kLazy<BF16>)) {
                     // the product of the block before is done: its scores' successor is
-                    const float mn = mx > m + 8.0f ? mx : m;
+                    const float mn = mx > m + kLazy<BF16> ? mx : m;
                     const float keep = mn == -INFINITY ? 1.0f : ex2(m - mn);
                     l *= keep;
                     m = mn;
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
                         tc::tmem_st16(out_at + cc, o);
                     }
                 }
-                const float off = m == -INFINITY ? 0.0f : m;
+                const float off = m == -INFINITY ? 0.0f : m - kLift<BF16>;
                 // x * c - off for two columns at a time, the sums too
                 const uint64_t c2 = pair_of(c, c), off2 = pair_of(-off, -off);
                 uint64_t sum[2] = {0, 0};
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const __grid_
             }
             // the segment's part
             const size_t part = (static_cast<size_t>(blockIdx.x) * p.max_seg + seg) * 2 + t;
-            parts.ml[part * kTile + row] = make_float2(m, l);
+            parts.ml[part * kTile + row] = make_float2(m - kLift<BF16>, l);
             wait(&bar.o_done[t], seg & 1u);
             if (n) {
                 // through the tile's query rows, which no product reads any
@@ -849,7 +855,8 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
                     }
             }
         }
-        const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        // p is relative to m, in f16 to kLift powers below it (as in prefix_kernel)
+        const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0] - kLift<BF16>, m[1] == -INFINITY ? 0.0f : m[1] - kLift<BF16>};
         float pr[2][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -926,7 +933,7 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
     for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t == 0) sm_ml[all][g + 8 * i] = make_float2(m[i], l[i]);
+        if (t == 0) sm_ml[all][g + 8 * i] = make_float2(m[i] - kLift<BF16>, l[i]);
 #pragma unroll
         for (int x = 0; x < H; ++x)
 #pragma unroll

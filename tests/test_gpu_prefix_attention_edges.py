@@ -29,6 +29,41 @@ def ctx(torch):
     c.close()
 
 
+def _flat_tail(torch, ctx, S, N, prefix, own, sink):
+    """One position (of the prefix, or of the own rows where there is none)
+    25.5 powers of two above all others, which hold the value 1: what they add up
+    to is the output."""
+    q = torch.zeros(S, N, 1, 64, dtype=torch.float16, device="cuda")
+    q[..., 0] = 16.0
+    k, v = (torch.zeros(prefix or own, 1, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    k[sink, 0, 0] = 25.5 * math.log(2.0) * 8.0 / 16.0   # the scale is 1 / 8
+    v[:] = 1.0
+    v[sink] = 0.0
+    score = float(k[sink, 0, 0]) * 16.0 / 8.0
+    small = torch.zeros(1, N, 1, 64, dtype=torch.float16, device="cuda")
+    suffix = [(torch.cat([t, small[0]]) if not prefix else small[0])[None].expand(S, -1, -1, -1) for t in (k, v)]
+    out = torch.empty(S, N, 1, 64, dtype=torch.float16, device="cuda")
+    lens = torch.full((S,), 0 if prefix else own, dtype=torch.int32, device="cuda")
+    ctx.prefix_attention(q, k if prefix else None, v if prefix else None, suffix[0], suffix[1], lens, [-1] * N, out)
+    ctx.sync()
+    n = (prefix or own) - 1
+    want = n / (math.exp(score) + n + 1)   # the node itself holds the value 0
+    err = float((out.double() - want).abs().max())
+    assert err <= (2.0 * F16 + 1e-5) * want, (err, want)
+
+
+@pytest.mark.parametrize("sink", [0, 199999, 399999])
+def test_f16_flat_tail_of_a_long_prefix(torch, ctx, sink):
+    """Rows for every SM to see the whole prefix."""
+    _flat_tail(torch, ctx, 600, 64, 400000, 0, sink)
+
+
+@pytest.mark.parametrize("sink", [0, 15000])
+def test_f16_flat_tail_of_own_rows(torch, ctx, sink):
+    """Sequences enough for one task to see all of one's rows."""
+    _flat_tail(torch, ctx, 6000, 1, 0, 20000, sink)
+
+
 @pytest.mark.parametrize("kind", ["float16", "bfloat16"])
 def test_long_flat_sums(torch, ctx, kind):
     """As many equal positions as one task may sum: rows for every SM to see
