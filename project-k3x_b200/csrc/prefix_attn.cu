@@ -162,6 +162,13 @@ extern "C" int k3xb_prefix_attention(k3xb_ctx* ctx, const k3xb_prefix_attention_
     if (io->prefix.rows > 0x7fffffffu || io->suffix.rows > 0x7fffffffu || io->suffix.rows < io->nodes)
         return bad("the suffix holds fewer rows than nodes, or a row count passes 2^31");
     if (!std::isfinite(io->scale)) return bad("scale must be finite");
+    if (io->type != K3XB_TYPE_F32 && io->type != K3XB_TYPE_BF16 && io->type != K3XB_TYPE_F16) return bad("type must be f32, bf16 or f16");
+    const size_t el = io->type == K3XB_TYPE_F32 ? 4 : 2;
+    auto off = [&](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
+    bool odd = off(io->q, el) || off(io->out, el) || off(io->lse, 4) || off(io->suffix_len, 4);
+    for (const k3xb_kv_rows* x : {&io->prefix, &io->suffix})
+        odd = odd || (x->rows && (off(x->k, el) || off(x->v, el) || (io->extra_dim && off(x->extra, el))));
+    if (odd) return bad("an array is not aligned to its type");
     AttnArgs a{};
     a.S = io->sequences;
     a.N = io->nodes;
@@ -191,7 +198,6 @@ extern "C" int k3xb_prefix_attention(k3xb_ctx* ctx, const k3xb_prefix_attention_
     switch (io->type) {
         case K3XB_TYPE_F32: return launch_rows<float>(ctx, a);
         case K3XB_TYPE_BF16: return launch_rows<__nv_bfloat16>(ctx, a);
-        case K3XB_TYPE_F16: return launch_rows<__half>(ctx, a);
-        default: return bad("type must be f32, bf16 or f16");
+        default: return launch_rows<__half>(ctx, a);
     }
 }

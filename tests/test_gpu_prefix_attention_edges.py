@@ -4,11 +4,13 @@ Tolerances as in test_gpu_prefix_attention.py: 2 u of sum p |v| for
 probabilities and outputs rounded to the type (u = 2^-8 bf16, 2^-11 f16), 1e-5
 of it for float scores and sums.
 """
+import ctypes as C
 import math
 
 import pytest
 
 from gpu_util import torch_cuda
+from test_gpu_prefix_attention import _case
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +82,42 @@ def test_long_flat_sums(torch, ctx, kind):
     err = float((out.double() - want).abs().max()) / want
     assert err <= 2.0 * (F16 if kind == "float16" else 2.0 ** -8) + 1e-5, err
     assert float((lse.double() - math.log(rows + 1)).abs().max()) <= 1e-5
+
+
+@pytest.mark.parametrize("kind,el", [("bfloat16", 2), ("float16", 2), ("float32", 4)])
+def test_arrays_off_their_alignment_are_refused(torch, ctx, kind, el):
+    """Refused on the host: no kernel sees such a pointer."""
+    import k3xb
+    c = _case(torch, 2, 2, 4, 2, 64, 64, 64, 30, [3, 4], kind, 940)
+    lens = torch.tensor(c["lens"], dtype=torch.int32).cuda()
+    out = torch.empty(2, 2, 4, 64, dtype=c["q"].dtype, device="cuda")
+    lse = torch.empty(2, 2, 4, device="cuda")
+    parent = (C.c_int32 * 2)(-1, 0)
+    io = k3xb.PrefixAttentionIO(sequences=2, nodes=2, heads=4, kv_heads=2, main_dim=64, extra_dim=64, value_dim=64,
+                                type={"float32": 0, "bfloat16": 1, "float16": 2}[kind], scale=0.1,
+                                parent=C.addressof(parent), q=c["q"].data_ptr(), suffix_len=lens.data_ptr(), out=out.data_ptr(),
+                                lse=lse.data_ptr())
+    for src, rows in ((io.prefix, "prefix"), (io.suffix, "suffix")):
+        src.k, src.v, src.extra = (c[rows + n].data_ptr() for n in ("_k", "_v", "_extra"))
+        src.rows = c[rows + "_k"].shape[-3]
+    call = ctx.lib.k3xb_prefix_attention
+    assert call(ctx.h, C.byref(io)) == 0
+    ctx.sync()
+    clean = out.clone()
+    out.fill_(7.0)
+    torch.cuda.synchronize()
+    for obj, field, step in [(io, "q", el), (io, "out", el), (io, "lse", 4), (io, "suffix_len", 4)] + [
+            (src, n, el) for src in (io.prefix, io.suffix) for n in ("k", "v", "extra")]:
+        at = getattr(obj, field)
+        for shift in range(1, step):
+            setattr(obj, field, at + shift)
+            assert call(ctx.h, C.byref(io)) == k3xb.INVALID_EXTENT, (field, shift)
+        setattr(obj, field, at)
+    io.type = 3
+    assert call(ctx.h, C.byref(io)) == k3xb.INVALID_EXTENT
+    ctx.sync()
+    assert bool((out == 7.0).all())
+    io.type = {"float32": 0, "bfloat16": 1, "float16": 2}[kind]
+    assert call(ctx.h, C.byref(io)) == 0
+    ctx.sync()
+    assert torch.equal(out, clean)
