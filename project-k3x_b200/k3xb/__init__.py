@@ -447,6 +447,9 @@ class Context:
         (S,) or ()); any strides with a contiguous last dimension."""
         if k is None or not k.numel():
             return _NO_ROWS
+        dims = len(lead) + 3
+        if k.dim() != dims or v is None or v.dim() != dims or (extra_dim and extra is not None and extra.dim() != dims - 1):
+            raise K3xbError(INVALID_EXTENT, "cache: expected k and v as rows of heads, and extra as rows")
         rows = k.shape[len(lead)]
         ks, vs = k.stride(), v.stride()
         bad = (k.shape != (*lead, rows, kv_heads, main) or v.shape != (*lead, rows, kv_heads, value) or k.dtype is not dtype or
@@ -474,6 +477,8 @@ class Context:
         suffix_len [S] int32 on the device; parent [N] on the host; out
         [S][N][heads][value]; lse [S][N][heads] float32 or None; scale default
         1 / sqrt(main + extra)."""
+        if q.dim() != 4 or suffix_k.dim() != 4 or suffix_v.dim() != 4:
+            raise K3xbError(INVALID_EXTENT, "q must be [S][N][heads][dim], suffix_k and suffix_v [S][capacity][kv_heads][dim]")
         S, N, heads, width = q.shape
         _, _, kv_heads, main = suffix_k.shape
         value, extra, dtype, device = suffix_v.shape[3], width - main, q.dtype, self.device

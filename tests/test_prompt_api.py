@@ -55,3 +55,25 @@ def test_host_tensors_are_refused():
     with pytest.raises(k3xb.K3xbError) as e:
         k3xb.Context._kv_rows(k, k, None, (1,), 2, 64, 64, 0, torch.float32, 0)
     assert e.value.status == k3xb.INVALID_EXTENT
+
+
+@pytest.mark.parametrize("q,k,v", [((2, 4, 64), (2, 9, 4, 64), (2, 9, 4, 64)), ((2, 1, 4, 64), (2, 9, 64), (2, 9, 4, 64)),
+                                   ((2, 1, 4, 64), (2, 9, 4, 64), (9, 4, 64))])
+def test_other_ranks_are_refused(q, k, v):
+    import torch
+
+    import k3xb
+    ctx = types.SimpleNamespace(device=0)
+    with pytest.raises(k3xb.K3xbError) as e:
+        k3xb.Context.prefix_attention(ctx, torch.zeros(q), None, None, torch.zeros(k), torch.zeros(v), None, [-1], None)
+    assert e.value.status == k3xb.INVALID_EXTENT
+
+
+@pytest.mark.parametrize("v", [None, (9, 4)])
+def test_a_prefix_without_values_is_refused(v):
+    import torch
+
+    import k3xb
+    with pytest.raises(k3xb.K3xbError) as e:
+        k3xb.Context._kv_rows(torch.zeros(9, 4, 64), v and torch.zeros(v), None, (), 4, 64, 64, 0, torch.float32, 0)
+    assert e.value.status == k3xb.INVALID_EXTENT
