@@ -1109,9 +1109,13 @@ int launch_attend_tc(k3xb_ctx* ctx, const AttnArgs& a, bool bf16) {
     p.blocks = static_cast<uint32_t>((static_cast<uint64_t>(a.prefix_len) + kTile - 1) / kTile);
     OwnPlan own{};
     own.row_tiles = (a.N * group + 15) / 16;
-    // One sequence shares its prefix with nobody: its few rows read it with
-    // their own (32 heads, one token after 700: 24 -> 20 us).
-    own.prefix = a.S == 1 && own.row_tiles <= 4;
+    // One sequence's few rows read a short prefix with their own rows, which saves
+    // a launch and a wait (32 heads of 128 + 64 / 128, one row: prefixes of 200 and 400
+    // 12.1 and 13.6 us, apart 14.4 and 14.5; 700 and 2000 18.0 and 28.6, apart 15.4 and 19.6;
+    // 16 rows of each of 2 tiles a head: 128 17.5, apart 17.8; 256 21.7, apart 18.5;
+    // 4 tiles of one kv head: 700 18.4, apart 19.9; 1500 23.0, apart 18.8).
+    own.prefix = a.S == 1 && own.row_tiles <= 4 && a.prefix_len <= 1024 &&
+                 static_cast<uint64_t>(a.kv_heads) * own.row_tiles * a.prefix_len <= 96ull * sms;
     const uint32_t tiles = (p.rows + kTile - 1) / kTile;
     p.pairs = tiles / 2;
     p.odd = tiles % 2;

@@ -10,7 +10,7 @@ import math
 import pytest
 
 from gpu_util import torch_cuda
-from test_gpu_prefix_attention import _case
+from test_gpu_prefix_attention import _case, _chain, _check
 
 pytestmark = pytest.mark.gpu
 
@@ -82,6 +82,15 @@ def test_long_flat_sums(torch, ctx, kind):
     err = float((out.double() - want).abs().max()) / want
     assert err <= 2.0 * (F16 if kind == "float16" else 2.0 ** -8) + 1e-5, err
     assert float((lse.double() - math.log(rows + 1)).abs().max()) <= 1e-5
+
+
+@pytest.mark.parametrize("heads,kv_heads,main,extra,value", [(8, 8, 128, 64, 128), (16, 2, 64, 0, 64), (16, 1, 128, 64, 128)])
+@pytest.mark.parametrize("N", [1, 4, 9])
+@pytest.mark.parametrize("prefix", [400, 1024, 1025, 3333])
+def test_one_sequence(torch, ctx, heads, kv_heads, main, extra, value, N, prefix):
+    """A short prefix goes with the own rows, a long one on its own."""
+    c = _case(torch, 1, N, heads, kv_heads, main, extra, value, prefix, [37], "bfloat16", 950 + prefix + N)
+    _check(torch, ctx, c, _chain(N))
 
 
 @pytest.mark.parametrize("kind,el", [("bfloat16", 2), ("float16", 2), ("float32", 4)])
