@@ -130,3 +130,43 @@ def test_arrays_off_their_alignment_are_refused(torch, ctx, kind, el):
     assert call(ctx.h, C.byref(io)) == 0
     ctx.sync()
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("S", [2, 3])
+def test_prefix_past_32_bits(torch, ctx, S):
+    """The tensor maps step over more than 2^31 key elements; the last rows decide."""
+    rows, heads = 530000, 32
+    q = torch.zeros(S, 1, heads, 128, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 16.0
+    k = torch.zeros(rows, heads, 128, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros(rows, heads, 128, dtype=torch.bfloat16, device="cuda")
+    k[-1, :, 0] = 30.0
+    v[-1] = torch.arange(heads, device="cuda").to(torch.bfloat16)[:, None]
+    own = torch.zeros(S, 2, heads, 128, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty(S, 1, heads, 128, dtype=torch.bfloat16, device="cuda")
+    ctx.prefix_attention(q, k, v, own, own, torch.zeros(S, dtype=torch.int32).cuda(), [-1], out)
+    ctx.sync()
+    weight = 1.0 / (1.0 + rows * math.exp(-480.0 / math.sqrt(128)))
+    want = weight * torch.arange(heads, dtype=torch.float64, device="cuda")[:, None].expand(heads, 128)
+    assert bool(((out[:, 0].double() - want).abs() <= 2.0 ** -7 * want).all())
+
+
+@pytest.mark.parametrize("kind,heads,rows", [("bfloat16", 32, 190000), ("bfloat16", 33, 190000), ("float32", 3, 1900000)])
+def test_own_rows_past_32_bits(torch, ctx, kind, heads, rows):
+    """The last sequence's last rows lie past 2^31 elements, and decide."""
+    S, dtype = 3, getattr(torch, kind)
+    q = torch.zeros(S, 1, heads, 128, dtype=dtype, device="cuda")
+    q[..., 0] = 16.0
+    k, v = (torch.zeros(S, rows, heads, 128, dtype=dtype, device="cuda") for _ in range(2))
+    k[:, -2, :, 0] = 30.0
+    v[:, -2] = torch.arange(1, heads + 1, device="cuda").to(dtype)[:, None]
+    v[:, -1] = 5.0   # the node's own row
+    out = torch.empty(S, 1, heads, 128, dtype=dtype, device="cuda")
+    lens = torch.tensor([3, 1000, rows - 1], dtype=torch.int32)
+    ctx.prefix_attention(q, None, None, k, v, lens.cuda(), [-1], out)
+    ctx.sync()
+    far = math.exp(-480.0 / math.sqrt(128))
+    total = 1.0 + (rows - 1) * far
+    want = (torch.arange(1, heads + 1, dtype=torch.float64, device="cuda")[:, None].expand(heads, 128) + 5.0 * far) / total
+    assert bool(((out[2, 0].double() - want).abs() <= 2.0 ** -7 * want).all())
+    assert not out[:2].any()
