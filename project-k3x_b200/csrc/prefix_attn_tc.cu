@@ -536,12 +536,22 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&x)[4], uin
 
 struct OwnPlan {
     uint32_t row_tiles;   // 16-row tiles of a sequence's rows per kv head
-    uint32_t splits;      // tasks along a sequence's keys
+    uint32_t splits;      // tasks along a sequence's keys, where it is long enough
+    uint32_t least;       // tiles of 16 keys that a task has at least
     uint32_t tasks;       // [kv head][row tile][split] of a sequence
+    uint32_t warps;       // 1 or 4 to a task
     uint32_t prefix;      // 1: the tasks read the prefix too
     float* o;             // [seq][kv head][row tile][split][16][value] where splits > 1
     float2* ml;           // [seq][kv head][row tile][split][16]
 };
+
+// The tasks that a sequence's keys are split into: what its length on the
+// device asks for (the host knows the cache's capacity only).
+__device__ __forceinline__ uint32_t splits_of(const OwnPlan& own, uint32_t tiles) { return max(1u, min(own.splits, tiles / own.least)); }
+__device__ __forceinline__ uint32_t tiles_of(const AttnArgs& a, const OwnPlan& own, int32_t len, uint32_t& prefix) {
+    prefix = own.prefix && len >= 0 ? (a.prefix_len + 15) / 16 : 0;
+    return len < 0 ? 0 : prefix + (static_cast<uint32_t>(len) + a.N + 15) / 16;
+}
 
 // A running join of parts for one row and C of its columns.
 template <int C>
@@ -687,23 +697,25 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
     const uint32_t all = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     float (*sm_o)[LD] = reinterpret_cast<float (*)[LD]>(buf[all]);
     uint4 (*sm_q)[2][32] = reinterpret_cast<uint4 (*)[2][32]>(buf[all / W * W]);
-    const uint32_t warp = all % W, mine = all / W, task = blockIdx.x * (4 / W) + mine;   // warp of a task; task of the CTA
-    if (task >= own.tasks) return;   // a whole warp (W = 1); with W = 4 there is a CTA per task
+    const uint32_t warp = all % W, mine = all / W, rows_at = blockIdx.x * (4 / W) + mine;   // warp of a task; task of the CTA
+    if (rows_at >= a.kv_heads * own.row_tiles) return;   // a whole warp (W = 1); with W = 4 there is a CTA per task
     auto sync = [&] {
         if constexpr (W == 1) __syncwarp();
         else __syncthreads();
     };
-    const uint32_t split = task % own.splits, rt = task / own.splits % own.row_tiles;
-    const uint32_t h = task / own.splits / own.row_tiles, s = blockIdx.y;
+    // splits come last: where sequences are short, theirs have nothing to do
+    const uint32_t split = blockIdx.z, rt = rows_at % own.row_tiles, h = rows_at / own.row_tiles, s = blockIdx.y;
+    const uint32_t task = rows_at * own.splits + split;
     const uint32_t group = a.heads / a.kv_heads, rows = a.N * group;
     const int32_t len = own_rows(a, s);
     const float c = fabsf(a.scale) * kLog2e;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     // this task's tiles of 16 keys: first the prefix's, where they are read
     // here, then the sequence's own
-    const uint32_t pre = own.prefix && len >= 0 ? (a.prefix_len + 15) / 16 : 0;
-    const uint32_t tiles = len < 0 ? 0 : pre + (static_cast<uint32_t>(len) + a.N + 15) / 16;
-    const uint32_t per_split = (tiles + own.splits - 1) / own.splits, end = min(tiles, (split + 1) * per_split);
+    uint32_t pre;
+    const uint32_t tiles = tiles_of(a, own, len, pre), splits = splits_of(own, tiles);
+    if (split >= splits) return;   // (those that there are wait for the prefix kernel, and thus this kernel's end)
+    const uint32_t per_split = (tiles + splits - 1) / splits, end = min(tiles, (split + 1) * per_split);
     uint32_t tile = split * per_split + warp;
 
     const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -946,7 +958,8 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
     sync();
     constexpr int C = DV / 32;
     const uint32_t col = lane * C, here = min(16u, rows - rt * 16);
-    if (own.splits == 1 && p.total) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix's parts
     for (uint32_t row = 2 * warp; row < here; row += 2 * W) {   // two rows at a time
         Join<C> j[2];
         const bool there[2] = {true, row + 1 < here};
@@ -959,13 +972,13 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
                 load_cols<C>(&buf[mine * W + w][(row + i) * LD + col], x);
                 j[i].add(sm_ml[mine * W + w][row + i], x);
             }
-            if (own.splits == 1) continue;
+            if (splits == 1) continue;
             const size_t at = (static_cast<size_t>(s) * own.tasks + task) * 16 + row + i;
             if (lane == 0) own.ml[at] = make_float2(j[i].m, j[i].l);
 #pragma unroll
             for (int e = 0; e < C; ++e) own.o[at * DV + col + e] = j[i].o[e];
         }
-        if (own.splits > 1) continue;
+        if (splits > 1) continue;
         const uint32_t r[2] = {rt * 16 + row, rt * 16 + row + there[1]};
         if (p.total && len >= 0) join_prefix<C>(j, p, parts, h, {s * rows + r[0], s * rows + r[1]}, there, col, DV);
 #pragma unroll
@@ -974,7 +987,7 @@ __global__ void __launch_bounds__(kOwnThreads, DQ + DV <= 192 ? 3 : 2) own_kerne
     }
 }
 
-// The join on its own, where own_kernel split the keys: a warp per two rows.
+// The join on its own, of sequences whose keys own_kernel split: a warp per two rows.
 template <int DV, bool BF16>
 __global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant__ AttnArgs a, const PrefixPlan p,
                                                            const Parts parts, const OwnPlan own) {
@@ -983,20 +996,24 @@ __global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant
     const uint32_t group = a.heads / a.kv_heads, rows = a.N * group;
     const uint32_t col = threadIdx.x % 32 * C, here = min(16u, rows - rt * 16);
     const int32_t len = own_rows(a, s);
+    uint32_t pre;
+    const uint32_t splits = splits_of(own, tiles_of(a, own, len, pre));
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (splits == 1) return;
     for (uint32_t row = threadIdx.x / 32 * 2; row < here; row += 8) {
         Join<C> j[2];
         const bool there[2] = {true, row + 1 < here};
         const uint32_t r[2] = {rt * 16 + row, rt * 16 + row + there[1]};
         if (len >= 0) {
             const size_t at = (static_cast<size_t>(s) * own.tasks + blockIdx.x * own.splits) * 16 + row;
-            for (uint32_t k0 = 0; k0 < own.splits; k0 += 6) {   // six splits' loads in flight
+            for (uint32_t k0 = 0; k0 < splits; k0 += 6) {   // six splits' loads in flight
                 float x[2][6][C];
                 float2 ml[2][6];
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                     for (uint32_t k = 0; k < 6; ++k)
-                        if (there[i] && k0 + k < own.splits) {
+                        if (there[i] && k0 + k < splits) {
                             ml[i][k] = own.ml[at + 16 * (k0 + k) + i];
                             load_cols<C>(own.o + (at + 16 * (k0 + k) + i) * DV + col, x[i][k]);
                         }
@@ -1004,7 +1021,7 @@ __global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant
                 for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
                     for (uint32_t k = 0; k < 6; ++k)
-                        if (there[i] && k0 + k < own.splits) j[i].add(ml[i][k], x[i][k]);
+                        if (there[i] && k0 + k < splits) j[i].add(ml[i][k], x[i][k]);
             }
             if (p.total) join_prefix<C>(j, p, parts, h, {s * rows + r[0], s * rows + r[1]}, there, col, DV);
         }
@@ -1017,26 +1034,24 @@ __global__ void __launch_bounds__(kOwnThreads) join_kernel(const __grid_constant
 template <int DQ, int DV, bool BF16>
 int launch_own(k3xb_ctx* ctx, const AttnArgs& a, const PrefixPlan& p, const Parts& parts, const OwnPlan& own) {
     cudaLaunchConfig_t cfg{};
-    // a warp per task from as many tasks on as the GPU holds warps (64 x 32
-    // tasks: 116 us with two warps each, 110 with one; 6 x 64 tasks: 50 us with
-    // one warp each, 38 with four)
-    const bool many = static_cast<uint64_t>(own.tasks) * a.S >= 8ull * ctx->sm_count;
-    cfg.gridDim = dim3(many ? (own.tasks + 3) / 4 : own.tasks, a.S);
+    const uint32_t ctas = a.kv_heads * own.row_tiles;
+    cfg.gridDim = dim3(own.warps == 1 ? (ctas + 3) / 4 : ctas, a.S, own.splits);
     cfg.blockDim = dim3(kOwnThreads);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    // beside the prefix kernel's tail (it waits there before it joins); a
-    // split launch leaves the join, and the wait, to join_kernel
-    cfg.numAttrs = p.total && own.splits == 1 ? 1 : 0;
-    if (many) K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16, 1>, a, p, parts, own));
+    // beside the prefix kernel's tail (it waits there before it joins or ends)
+    cfg.numAttrs = p.total ? 1 : 0;
+    if (own.warps == 1) K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16, 1>, a, p, parts, own));
     else K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, own_kernel<DQ, DV, BF16, 4>, a, p, parts, own));
     ++ctx->stats.kernel_launches;
     if (own.splits > 1) {
-        join_kernel<DV, BF16><<<dim3(a.kv_heads * own.row_tiles, a.S), kOwnThreads, 0, ctx->stream>>>(a, p, parts, own);
-        K3XB_LAUNCHED(ctx);
+        cfg.gridDim = dim3(ctas, a.S);
+        cfg.numAttrs = 1;   // it waits for the parts at its start
+        K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, join_kernel<DV, BF16>, a, p, parts, own));
+        ++ctx->stats.kernel_launches;
     }
     return K3XB_OK;
 }
@@ -1137,12 +1152,22 @@ int launch_attend_tc(k3xb_ctx* ctx, const AttnArgs& a, bool bf16) {
         if (static_cast<uint64_t>(ctas) * p.max_seg * 2 * kTile >= (1ull << 31))
             return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: too many rows");
     }
-    // Tasks for the GPU's warps three times over (twelve per SM), since
-    // sequences are of unlike lengths; a split has 256 cache rows at least (by
-    // the capacity: lengths are on the device), or 64 where latency counts.
+    // A task has one warp where there are tasks for every one that the GPU holds (64 x 32
+    // tasks: 116 us with two warps each, 110 with one), else four (6 x 64 tasks:
+    // 50 us with one, 38 with four).
     const uint64_t whole = static_cast<uint64_t>(a.S) * a.kv_heads * own.row_tiles;
-    const uint64_t rows_read = a.capacity + (own.prefix ? static_cast<uint64_t>(a.prefix_len) : 0), least = own.prefix ? 64 : 256;
-    own.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((36 * sms + whole - 1) / whole, rows_read / least)));
+    own.warps = whole >= 8ull * sms ? 1 : 4;
+    // Room for three times as many warps as the GPU holds (twelve per SM), since
+    // sequences are of unlike lengths; how many tasks a sequence becomes is up to its
+    // length on the device, 512 keys to one at least (48 sequences of up to
+    // 2100, 16 heads of 64: 64 us; 256 and 1024 66 and 73 us), or 64 where latency
+    // counts. Lengths, not the capacity, so that a cache with room for 16384 costs
+    // no more than a full one (21 x 5 rows after 5003 + up to 331: 37.4 us; by
+    // capacity 69).
+    own.least = own.prefix ? 4 : 32;
+    const uint64_t rows_read = a.capacity + (own.prefix ? static_cast<uint64_t>(a.prefix_len) : 0);
+    const uint64_t wanted = own.prefix ? 36 * sms : 36 * sms / own.warps;
+    own.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((wanted + whole - 1) / whole, rows_read / (16 * own.least))));
     if (static_cast<uint64_t>(a.kv_heads) * own.row_tiles * own.splits >= (1ull << 31))
         return fail(ctx, K3XB_INVALID_EXTENT, "prefix_attention: too many rows per sequence");
     own.tasks = a.kv_heads * own.row_tiles * own.splits;

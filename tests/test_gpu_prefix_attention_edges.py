@@ -93,6 +93,18 @@ def test_one_sequence(torch, ctx, heads, kv_heads, main, extra, value, N, prefix
     _check(torch, ctx, c, _chain(N))
 
 
+@pytest.mark.parametrize("S,heads,kv_heads,lens", [(3, 4, 2, [0, 700, 5000]), (5, 8, 8, [1100, -1, 15, 2600, 511]), (300, 8, 4, [3, 600, 1500, 0, 77])])
+@pytest.mark.parametrize("prefix", [0, 333])
+@pytest.mark.parametrize("spare", [0, 9000])
+def test_roomy_caches(torch, ctx, S, heads, kv_heads, lens, prefix, spare):
+    """Sequences of unlike lengths in caches with room for far longer ones: some
+    become several tasks, some one, some none."""
+    lens = [lens[i % len(lens)] for i in range(S)]
+    spare = spare if S < 100 else min(spare, 900)
+    c = _case(torch, S, 2, heads, kv_heads, 64, 64, 64, prefix, lens, "bfloat16", 970 + S + prefix, spare=spare)
+    _check(torch, ctx, c, _chain(2))
+
+
 @pytest.mark.parametrize("kind,el", [("bfloat16", 2), ("float16", 2), ("float32", 4)])
 def test_arrays_off_their_alignment_are_refused(torch, ctx, kind, el):
     """Refused on the host: no kernel sees such a pointer."""
