@@ -548,7 +548,7 @@ int k3xb_kda_commit(k3xb_ctx* ctx, const float* state, const int32_t* parent,
  * tokens); no token's outputs depend on a later one. What an infinity or NaN
  * reaches by the rule becomes an infinity or NaN, and nothing else does.
  * Offsets that are no ranges leave their sequences out and k3xb_sync reports
- * INVALID_EXTENT. */
+ * INVALID_EXTENT (where ranges overlap, sequences with one may be off too). */
 int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
                      uint64_t row_stride, int32_t type, const float* log_decay,
                      const float* beta, const uint32_t* offsets, uint32_t sequences,

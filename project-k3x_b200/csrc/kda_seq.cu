@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
     const E* k = static_cast<const E*>(a.k);
     const E* v = static_cast<const E*>(a.v);
     uint32_t t0, t1;
+    asm volatile("griddepcontrol.launch_dependents;");   // chunks of other sequences may start
     if (!token_range(a, s, t0, t1)) return;
     const int32_t slot = a.slots ? a.slots[s] : static_cast<int32_t>(s);
     const bool outside = slot >= 0 && static_cast<uint32_t>(slot) >= a.states;
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // outputs and, but for a query's, in all later ones (a value's or a state's in its own row).
 
 constexpr int kChunk = 16, kStages = 3;
+constexpr uint32_t kShort = 9;   // sequences below go token by token where there are some
 constexpr int kKeySpread = 40, kLeastDecay = -40, kMostDecay = 100;
 // Operands held at a time: longer batches go in segments of chunks.
 constexpr size_t kOperandBytes = size_t(1) << 30;
@@ -274,7 +276,7 @@ struct __align__(16) ChunkScratch {
 // most the distance). A segment is a range of slots.
 struct ChunkPlan {
     uint32_t slot0, slots;     // this segment
-    uint32_t stride;           // chunks that a CTA of the first kernel steps over
+    uint32_t sequences, stride;   // slots that a CTA of the first kernel steps over
     void* stages;              // [slots][heads] ChunkStage
     const float* carry_in;     // states at the segment's start of sequences that began before it
     float* carry_out;          // states at its end
@@ -286,6 +288,35 @@ __device__ __forceinline__ void segment_chunks(const ChunkPlan& p, uint32_t s, u
     const uint32_t n = (t1 - t0 + kChunk - 1) / kChunk;
     first = min(n, p.slot0 > base ? p.slot0 - base : 0u);
     last = min(n, p.slot0 + p.slots > base ? p.slot0 + p.slots - base : 0u);
+}
+
+// The chunk in a slot (whole warps): its first token and its sequence's end,
+// found in the offsets, 32 of them at a time (up to 31 sequences' in `mine`, a
+// lane each); false where the slot holds none.
+__device__ __forceinline__ bool chunk_in(const SeqArgs& a, const ChunkPlan& p, uint32_t slot, uint32_t lane, uint32_t mine, uint32_t& first,
+                                         uint32_t& t1) {
+    uint32_t s = 0, t0;
+    if (p.sequences < 32) {
+        const uint32_t found = __ballot_sync(0xffffffffu, lane < p.sequences && mine / kChunk + lane <= slot);
+        if (!found) return false;
+        s = 31 - __clz(found);
+        t0 = __shfl_sync(0xffffffffu, mine, s);
+        t1 = __shfl_sync(0xffffffffu, mine, s + 1);
+    } else {
+        for (uint32_t n = p.sequences; n > 1;) {
+            const uint32_t step = (n + 31) / 32, i = lane * step;
+            const uint32_t found = __ballot_sync(0xffffffffu, i < n && a.offsets[s + i] / kChunk + s + i <= slot);
+            if (!found) return false;
+            const uint32_t k = 31 - __clz(found);
+            s += k * step;
+            n = min(step, n - k * step);
+        }
+        t0 = a.offsets[s];
+        t1 = a.offsets[s + 1];
+    }
+    const uint32_t chunk = slot - (t0 / kChunk + s);
+    first = t0 + chunk * kChunk;
+    return t0 <= t1 && t1 <= a.tokens && t1 - t0 >= a.from && t1 - t0 < a.below && chunk < (t1 - t0 + kChunk - 1) / kChunk;
 }
 
 // The power of two that takes a maximum to [2^14, 2^15) (f16 ends at 2^16);
@@ -492,12 +523,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
     ChunkScratch<D>& sc = *reinterpret_cast<ChunkScratch<D>*>(chunk_mem);
     constexpr int NP = D / 32;   // warps
     asm volatile("griddepcontrol.launch_dependents;");   // the scan's CTAs may start as these run out
-    const uint32_t s = blockIdx.y, h = blockIdx.x % a.heads;
-    uint32_t t0, t1, chunk, chunk_end, base;
-    if (!token_range(a, s, t0, t1)) return;
-    segment_chunks(plan, s, t0, t1, chunk, chunk_end, base);
-    chunk += blockIdx.x / a.heads;
-    if (chunk >= chunk_end) return;
+    const uint32_t h = blockIdx.x % a.heads;
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, th = lane / 16, P = a.heads * D;
     const uint32_t c = warp * 32 + lane % 16 * 2;
     const E* q = static_cast<const E*>(a.q) + h * D + c;
@@ -507,7 +533,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
     // leave everything as it is
     float2 kk[8], qq[8], al[8];
     float bb = 0.0f;
-    auto fetch = [&](uint32_t first) {
+    auto fetch = [&](uint32_t first, uint32_t t1) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t tok = first + 8 * th + i;
@@ -522,7 +548,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
     };
     // the next chunk's rows on their way to L2, 128 bytes a thread, a chunk's
     // work before they are loaded (13 ragged turns: 500 -> 430 us)
-    auto prefetch = [&](uint32_t first) {
+    auto prefetch = [&](uint32_t first, uint32_t t1) {
         constexpr uint32_t qk = (D * sizeof(E) + 127) / 128, all = 2 * qk + (D * 4 + 127) / 128;
         const size_t tok = first + threadIdx.x % kChunk;
         if (tok >= t1) return;
@@ -536,10 +562,19 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
         }
     };
     const uint32_t arow = lane % 16, acol = lane / 16 * 8;         // ldmatrix: left operands, and k-major ones transposed
-    fetch(t0 + chunk * kChunk);
-    for (; chunk < chunk_end; chunk += plan.stride) {
-        if (chunk + plan.stride < chunk_end) prefetch(t0 + (chunk + plan.stride) * kChunk);
-        ChunkStage<D>& st = static_cast<ChunkStage<D>*>(plan.stages)[static_cast<size_t>(base + chunk - plan.slot0) * a.heads + h];
+    uint32_t slot = blockIdx.x / a.heads, first, t1;
+    const uint32_t mine = a.offsets[min(lane, plan.sequences)];
+    auto seek = [&] {   // from `slot` on
+        while (slot < plan.slots && !chunk_in(a, plan, plan.slot0 + slot, lane, mine, first, t1)) slot += plan.stride;
+        return slot < plan.slots;
+    };
+    bool more = seek();
+    if (more) fetch(first, t1);
+    while (more) {
+        ChunkStage<D>& st = static_cast<ChunkStage<D>*>(plan.stages)[static_cast<size_t>(slot) * a.heads + h];
+        slot += plan.stride;
+        more = seek();
+        if (more) prefetch(first, t1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) al[i] = make_float2(expf(al[i].x), expf(al[i].y));
         {
@@ -705,7 +740,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
         if (poison < 16)
             for (int i = max(0, static_cast<int>(poison) - static_cast<int>(8 * th)); i < 8; ++i)
                 store_pair(sc.k, 8 * th + i, c, make_float2(0.0f, 0.0f));
-        if (chunk + plan.stride < chunk_end) fetch(t0 + (chunk + plan.stride) * kChunk);
+        if (more) fetch(first, t1);
         __syncthreads();
         for (int l = warp; l < 4; l += NP) {
             float b[4] = {}, x[4] = {};
@@ -804,6 +839,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
         }
         __syncthreads();
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // ends after the token form before it
 }
 
 template <int D, int NW, int KS>
@@ -1171,12 +1207,21 @@ int launch_chunks_as(k3xb_ctx* ctx, const SeqArgs& a, uint32_t sequences) {
         p.slot0 = x;
         p.slots = std::min(step, slots - x);
         // sixteen CTAs for each that the GPU holds at a time (three per SM), so
-        // that sequences of unlike lengths even out and a CTA has chunks to
-        // load ahead; no more than an average sequence's chunks
-        const uint64_t wanted = (48ull * ctx->sm_count + static_cast<uint64_t>(a.heads) * sequences - 1) / (static_cast<uint64_t>(a.heads) * sequences);
-        p.stride = static_cast<uint32_t>(std::min<uint64_t>(wanted, (p.slots + sequences - 1) / sequences));
-        chunk_operands_kernel<D, E, VEC><<<dim3(p.stride * a.heads, sequences), D, sizeof(ChunkScratch<D>), ctx->stream>>>(a, p);
-        K3XB_LAUNCHED(ctx);
+        // that they even out and a CTA has chunks to load ahead
+        p.sequences = sequences;
+        p.stride = static_cast<uint32_t>(std::min<uint64_t>((48ull * ctx->sm_count + a.heads - 1) / a.heads, p.slots));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(p.stride * a.heads);
+        cfg.blockDim = dim3(D);
+        cfg.dynamicSmemBytes = sizeof(ChunkScratch<D>);
+        cfg.stream = ctx->stream;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = x == 0 && a.from ? 1 : 0;   // beside the token form of the short sequences
+        K3XB_CUDA(ctx, cudaLaunchKernelEx(&cfg, chunk_operands_kernel<D, E, VEC>, a, p));
+        ++ctx->stats.kernel_launches;
         // few sequences: an SM for every 32 rows, with two warps to a row
         // group; else two CTAs per SM where there are that many
         int st;
@@ -1252,17 +1297,18 @@ int k3xb_kda_prefill(k3xb_ctx* ctx, const void* q, const void* k, const void* v,
     PhaseScope ph(ctx, K3XB_PHASE_KDA_RECURRENCE);
     ++ctx->stats.kda_calls;
     const bool f32 = type == K3XB_TYPE_F32;
-    if (tokens <= 16ull * sequences) {
-        // Short sequences among these: up to 6 tokens go token by token (a
-        // chunk costs the same for 1 as for 16: 64 sequences of 32 heads take
-        // 58, 63 and 81 us with 1, 2 and 4 tokens each and 138 to 142 in chunks
-        // of 8 or 16, 300 take 231, 311, 407 and 582 to 591), the others in
-        // chunks.
-        a.below = 7;
+    if (tokens <= 16ull * sequences || sequences >= 16) {
+        // Short sequences are likely, or there may be many beside long ones: up to
+        // 8 tokens go token by token, the others in chunks (a chunk costs the same
+        // for 1 as for 16: 64 sequences of 32 heads take 55, 76 and 134 us with 1, 4
+        // and 8 tokens each and 136 to 140 in chunks, 300 take 229, 404, 596 and 589
+        // to 609, 16 take 12, 21, 31 and 40). Where there are none this costs a
+        // launch beside the first kernel's start.
+        a.below = kShort;
         if (const int st = f32 ? launch_seq<float>(ctx, a, sequences, head_dim) : launch_seq<__nv_bfloat16>(ctx, a, sequences, head_dim))
             return st;
-        if (tokens < 7) return K3XB_OK;
-        a.from = 7;
+        if (tokens < kShort) return K3XB_OK;
+        a.from = kShort;
         a.below = ~0u;
     }
     return f32 ? launch_prefill<float>(ctx, a, sequences, head_dim) : launch_prefill<__nv_bfloat16>(ctx, a, sequences, head_dim);

@@ -237,3 +237,14 @@ def test_segments_row_by_row(torch, ctx, kept):
             if kept:
                 _check(torch, new[s, h0:h0 + 128], st, R, f"state {s}, heads {h0}", "state")
         first += n
+
+
+@pytest.mark.parametrize("lengths", [[300] + [1] * 16, [1] * 20 + [130] + [3] * 9 + [8, 9, 0, 7], [0, 5, 0, 200] * 8, [(7 * i) % 40 for i in range(33)],
+                                     [(11 * i) % 29 for i in range(1100)]], ids=["one long first", "one long between", "with empty ones", "33", "1100"])
+@pytest.mark.parametrize("d,h", [(32, 1), (128, 2)])
+def test_long_and_short_sequences_together(torch, ctx, lengths, d, h):
+    """Some go token by token, some in chunks; the chunks are found in the offsets."""
+    if len(lengths) > 1000 and d == 128:
+        lengths = lengths[:100]
+    x = _inputs(torch, sum(lengths), h, d, 41 + len(lengths))
+    _run(torch, ctx, x, lengths, _state(torch, len(lengths), h, d))
