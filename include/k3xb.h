@@ -544,8 +544,9 @@ int k3xb_kda_commit(k3xb_ctx* ctx, const float* state, const int32_t* parent,
  * of their own: results agree with the token-by-token calls to float
  * tolerance, not bit for bit (k3xb_kda_tree keeps the reference's order). Each
  * output is off by roundings of its own query's size times its own state row's,
- * whatever the sizes of the other tokens (keys up to 2^40 apart within 16
- * tokens); no token's outputs depend on a later one. What an infinity or NaN
+ * whatever the sizes of the other tokens (within 16 of them: keys up to 2^40
+ * apart, and decays of all channels together to 2^-80); no token's outputs
+ * depend on a later one. What an infinity or NaN
  * reaches by the rule becomes an infinity or NaN, and nothing else does.
  * Offsets that are no ranges leave their sequences out and k3xb_sync reports
  * INVALID_EXTENT (where ranges overlap, sequences with one may be off too). */

@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // out beforehand, by powers of two and thus exactly: token j's key times
 // 2^(x + dx_j), so that every token's largest is alike (up to 2^40 apart), its query
 // times 2^z_j, its decay times 2^-e_j, so that its largest channel is 1/2 to 1 (down to
-// 2^-40 from the chunk's start). With E_j the sum of the e up to j the rule holds for
+// 2^-80 from the chunk's start). With E_j the sum of the e up to j the rule holds for
 //   b_j 2^(-2 dx_j),  v_j 2^(dx_j - E_j + c),  u_j 2^(-dx_j - E_j + c),  o_j 2^(z_j - E_j)
 // in place of b, v, u and o: the powers go to T's columns, P's rows and
 // the rows' factors fw and fq. So an output is off by float roundings of its
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 
 constexpr int kChunk = 16, kStages = 3;
 constexpr uint32_t kShort = 9;   // sequences below go token by token where there are some
-constexpr int kKeySpread = 40, kLeastDecay = -40, kMostDecay = 100;
+constexpr int kKeySpread = 40, kLeastDecay = -80, kMostDecay = 100;
 // Operands held at a time: longer batches go in segments of chunks.
 constexpr size_t kOperandBytes = size_t(1) << 30;
 
@@ -1004,11 +1004,11 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
                 const int before = spoilt;
                 if (before != kNone) spoil(first - kChunk);
                 spoilt = first_bad(vv, t);
-                // it stays below 2^40 over that of the values to come, so that a
+                // it stays below 2^90 over that of the values to come, so that a
                 // small state's multiple does not carry their sums past a float's end
                 int vx[2];
                 const float2 top = row_exps(vv, vx);
-                const int cap0 = top.x == 0.0f ? 126 : min(126, vx[0] + 40), cap1 = top.y == 0.0f ? 126 : min(126, vx[1] + 40);
+                const int cap0 = top.x == 0.0f ? 126 : min(126, vx[0] + 90), cap1 = top.y == 0.0f ? 126 : min(126, vx[1] + 90);
                 const bool in0 = m0 == 0.0f || (m0 >= 0x1p8f && m0 <= 0x1p15f), in1 = m1 == 0.0f || (m1 >= 0x1p8f && m1 <= 0x1p15f);
                 const int d0 = min(in0 ? 0 : scale_exp(m0) - 2, cap0 - sx[0]), d1 = min(in1 ? 0 : scale_exp(m1) - 2, cap1 - sx[1]);
                 const float f0 = (before & 255) < kChunk ? NAN : pow2(d0), f1 = before >> 8 < kChunk ? NAN : pow2(d1);

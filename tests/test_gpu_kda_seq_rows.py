@@ -248,3 +248,12 @@ def test_long_and_short_sequences_together(torch, ctx, lengths, d, h):
         lengths = lengths[:100]
     x = _inputs(torch, sum(lengths), h, d, 41 + len(lengths))
     _run(torch, ctx, x, lengths, _state(torch, len(lengths), h, d))
+
+
+@pytest.mark.parametrize("at", [15, 30])
+def test_a_small_state_before_a_large_value(torch, ctx, at):
+    """Contents of 1e-20 are read out exactly up to the token that brings 1e12."""
+    x = _inputs(torch, 40, 2, 128, 43)
+    x[2][:at] *= 1e-20
+    x[2][at] *= 1e12
+    _run(torch, ctx, x, [40], 1e-20 * _state(torch, 1, 2, 128))
