@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                 sc.sq[warp][tok] = exp2i(z);
                 sc.sa[warp][tok] = exp2i((tok ? before : 0) - sum);
                 if (warp == 0) {
-                    sc.beta[tok] = tok < poison ? be * exp2i(-2 * dx) : 0.0f;
+                    sc.beta[tok] = sized ? be * exp2i(-2 * dx) : 0.0f;   // a zero key writes nothing, whatever its u
                     sc.ft[tok] = pow2(dx - sum + mid);
                     sc.fp[tok] = two_to(sum - mid - z);
                     sc.fd[tok] = pow2(dx + sum - mid);

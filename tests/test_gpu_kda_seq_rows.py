@@ -257,3 +257,13 @@ def test_a_small_state_before_a_large_value(torch, ctx, at):
     x[2][:at] *= 1e-20
     x[2][at] *= 1e12
     _run(torch, ctx, x, [40], 1e-20 * _state(torch, 1, 2, 128))
+
+
+@pytest.mark.parametrize("at", [0, 14, 15])
+def test_a_zero_key_beside_small_contents(torch, ctx, at):
+    """A token without a key writes nothing, however large its value is."""
+    x = _inputs(torch, 20, 2, 128, 47)
+    x[2] *= 1e-9
+    x[2][at] *= 1e21
+    x[1][at] = 0.0
+    _run(torch, ctx, x, [20], 1e-9 * _state(torch, 1, 2, 128))
