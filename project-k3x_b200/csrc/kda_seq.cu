@@ -931,6 +931,9 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
     }
     constexpr int DK = D / KS;   // this warp's key channels, from k0 on
     constexpr int NV = sizeof(E) == 2 ? 1 : 3;   // bf16 values are one term
+    // U in P U: for bf16 outputs two terms, off by 2^-18 of the products, where
+    // the outputs' own rounding takes 2^-9 (13 ragged turns 922 -> 904 us)
+    constexpr int NU = sizeof(E) == 2 ? 2 : 3;
     const uint32_t half = warp % KS, k0 = half * DK;
     const uint32_t row0 = blockIdx.x % slices * (16 * NW) + warp / KS * 16;
     const uint32_t g = lane / 4, t = lane % 4, P = a.heads * D;
@@ -1072,7 +1075,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) u[i][e] -= wb[i][e];
-            split_tokens<3>(u, uw);
+            split_tokens<NU>(u, uw);
             row_exps(u, ux);
             // a product's powers together stay within a float's
             ux[0] = min(ux[0], 126 + sx[0] + st.exp);
@@ -1106,7 +1109,7 @@ __global__ void __launch_bounds__(32 * NW * KS + 32, PER_SM) chunk_scan_kernel(c
         }
         {   // O = (p Q) S0^T + P U
             float c[2][4] = {};
-            mma_tokens<3>(c, uw, &st.p[0][mrow][mcol]);
+            mma_tokens<NU>(c, uw, &st.p[0][mrow][mcol]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (KS > 1 && i != static_cast<int>(half)) continue;   // a half writes one tile of tokens
