@@ -601,8 +601,9 @@ typedef struct {
  * calls with main_dim and value_dim 64 or 128, extra_dim 0 or 64, and rows that start at
  * 16-byte boundaries (and a scale that is not 0) run on the tensor cores,
  * where the prefix is read once for 256 rows of a kv head (sequences x nodes
- * x grouped heads) and the probabilities enter the second product rounded
- * to `type`; other shapes take a slower general form. A suffix_len that
+ * x grouped heads; one sequence's short prefix once for 16) and the
+ * probabilities enter the second product rounded to `type` (in f16 down to
+ * 2^-38 of a row's largest); other shapes take a slower general form. A suffix_len that
  * leaves no room for the drafts counts as idle and k3xb_sync reports
  * INVALID_EXTENT. */
 typedef struct {

@@ -206,12 +206,12 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // memory. (Both in one kernel, with producer warps beside the scan's, the
 // producers took 7900 cycles a chunk and the scan 2700, and half the GPU was
 // idle at one sequence: 8192 tokens of 32 heads 2.48 ms, apart 1.23.) A
-// chunk's operands cross memory once, 1.2 times the bytes of its inputs, as an
+// chunk's operands cross memory once, 1.3 times the bytes of its inputs, as an
 // image of the shared memory that the scan copies them to.
 //
-// Measured (one B200): 8192 tokens, 32 heads of 128, f32: operands 259 us (3.5
-// TB/s, the issue slots 53% busy: ~2150 instructions a warp and chunk, most
-// of them splits), scan 555 us, 1.1 us a chunk: a chain of products (90 MMAs a
+// Measured (one B200): 8192 tokens, 32 heads of 128, f32: operands 266 us (3.6
+// TB/s, the issue slots 53% busy: ~2250 instructions a warp and chunk, most
+// of them splits), scan 563 us, 1.1 us a chunk: a chain of products (96 MMAs a
 // warp), row maxima and splits from one chunk's state to the next's.
 //
 // Terms. An f16 operand is two terms of a power-of-two multiple (hi + lo: 22
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
             bb = first + threadIdx.x < t1 ? a.beta[static_cast<size_t>(first + threadIdx.x) * a.heads + h] : 0.0f;
     };
     // the next chunk's rows on their way to L2, 128 bytes a thread, a chunk's
-    // work before they are loaded (13 ragged turns: 500 -> 430 us)
+    // work before they are loaded (13 ragged turns: 978 -> 922 us in all)
     auto prefetch = [&](uint32_t first, uint32_t t1) {
         constexpr uint32_t qk = (D * sizeof(E) + 127) / 128, all = 2 * qk + (D * 4 + 127) / 128;
         const size_t tok = first + threadIdx.x % kChunk;
@@ -852,8 +852,8 @@ struct __align__(128) ScanSmem {
 };
 
 // The blockIdx.y-th sequence of the batch, the longest ones first (they then
-// start first, and the last round of CTAs is short: 13 ragged turns 600 -> 483
-// us); the given order for many or short ones, where sorting costs more.
+// start first, and the last round of CTAs is short: 13 ragged turns 1027 -> 922
+// us in all); the given order for many or short ones, where sorting costs more.
 __device__ __forceinline__ uint32_t sequence_of(const SeqArgs& a, uint32_t y, uint32_t* found) {
     const uint32_t n = gridDim.y;
     if (n == 1 || n > 64 || a.tokens < 256 * n) return y;
@@ -1154,7 +1154,8 @@ int launch_scan(k3xb_ctx* ctx, const SeqArgs& a, const ChunkPlan& p, uint32_t se
     const dim3 grid(a.heads * (D / (16 * NW)), sequences);
     // Where every CTA can have an SM of its own it asks for more than half of
     // the shared memory: two on one SM while others idle share its issue
-    // slots (8192 tokens of 32 heads 1087 us, 804 apart).
+    // slots (8192 tokens of 32 heads 1087 us so, 804 apart, when the kernel's
+    // registers left room for two).
     constexpr size_t need = sizeof(ScanSmem<D, NW, KS>), alone = std::max(need, size_t(116) << 10);
     const size_t smem = static_cast<uint64_t>(grid.x) * grid.y <= static_cast<uint64_t>(ctx->sm_count) ? alone : need;
     const int cst = configure_once(ctx, configured, [&]() -> int {

@@ -8,19 +8,21 @@
 //    tcgen05, so that a prefix row crosses HBM once for up to 256 rows. The
 //    work is one flat list of 128-key steps over (kv head, row tiles), cut
 //    into equal ranges, one per CTA; a range that ends inside a row tile
-//    leaves a part: the running maximum m, sum l and unnormalised output o
-//    of its keys.
+//    leaves a part: the running maximum m (less kLift), sum l and
+//    unnormalised output o of its keys. One sequence's short prefix goes
+//    with 2 instead.
 // 2. own_kernel: a sequence's own rows and its draft rows for 16 rows at a
 //    time on mma.sync (a sequence has few rows; the bound is the read of its
 //    cache). It runs beside the tail of 1 and then joins the parts:
 //       M = max m_i,  out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
-// 3. join_kernel, only where 2 split a long cache into several CTAs.
+// 3. join_kernel, only where 2 may split long caches into several CTAs, for
+//    the sequences that it did split.
 //
 // Scores stay float; m is kept in log2 units (score * scale * log2 e).
 //
 // Measured (one B200, 32 heads, keys of 128 + 64, values of 128, prefix 16384):
-// 64 x 9 rows a head: prefix_kernel 201 us (0.96 PFLOP/s of tensor work, 57% of
-// the measured peak), own_kernel 69 us; 64 rows: 63 us (4.3 TB/s) and 52 us.
+// 64 x 9 rows a head: prefix_kernel 198 us (0.97 PFLOP/s of tensor work, 58% of
+// the measured peak), own_kernel 66 us; 64 rows: 60 us (4.5 TB/s) and 49 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
