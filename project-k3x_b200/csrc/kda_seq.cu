@@ -263,7 +263,7 @@ struct __align__(16) ChunkScratch {
     float At[kChunk][kChunk];             // At[j][i] = A_ij
     float P[kChunk][kChunk];
     float diag[D / 32][kChunk];           // q_i . k_i by warp
-    float beta[kChunk];
+    float beta[kChunk], bs[kChunk];       // as they are, and as the evened tokens have them
     uint32_t top[3][D / 32][kChunk / 2];  // largest |k|, |q|, decay of each token by warp: two tokens' upper halves
     // powers of two by token: of k, q and the decay (each warp's own); of T's columns, P's rows and its diagonal
     float sk[D / 32][kChunk], sq[D / 32][kChunk], sa[D / 32][kChunk], ft[kChunk], fp[kChunk], fd[kChunk];
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
                 sc.sq[warp][tok] = exp2i(z);
                 sc.sa[warp][tok] = exp2i((tok ? before : 0) - sum);
                 if (warp == 0) {
-                    sc.beta[tok] = sized ? be * exp2i(-2 * dx) : 0.0f;   // a zero key writes nothing, whatever its u
+                    sc.bs[tok] = sized ? be * exp2i(-2 * dx) : 0.0f;   // a zero key writes nothing, whatever its u
                     sc.ft[tok] = pow2(dx - sum + mid);
                     sc.fp[tok] = two_to(sum - mid - z);
                     sc.fd[tok] = pow2(dx + sum - mid);
@@ -777,11 +777,11 @@ __global__ void __launch_bounds__(D, D == 128 ? 3 : 1) chunk_operands_kernel(con
             for (int i = 0; i < kChunk; ++i) x[i] = 0.0f;
 #pragma unroll
             for (int m = 0; m < kChunk; ++m) {
-                x[m] = fmaf(-sc.beta[m], x[m], m == static_cast<int>(j) ? 1.0f : 0.0f);
+                x[m] = fmaf(-sc.bs[m], x[m], m == static_cast<int>(j) ? 1.0f : 0.0f);
 #pragma unroll
                 for (int i = m + 1; i < kChunk; ++i) x[i] = fmaf(sc.At[m][i], x[m], x[i]);
             }
-            const float b = sc.beta[j];
+            const float b = sc.bs[j];
 #pragma unroll
             for (int i = 0; i < kChunk / 2; ++i)   // a half warp has half of the rows
                 sc.T[8 * th + i][j] = 8 * th + i < poison ? (th ? x[8 + i] : x[i]) * b : 0.0f;
