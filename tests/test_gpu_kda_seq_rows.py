@@ -267,3 +267,35 @@ def test_a_zero_key_beside_small_contents(torch, ctx, at):
     x[2][at] *= 1e21
     x[1][at] = 0.0
     _run(torch, ctx, x, [20], 1e-9 * _state(torch, 1, 2, 128))
+
+
+@pytest.mark.parametrize("lengths", [[90], [100] + [1] * 20 + [30]], ids=["chunks", "tokens and chunks"])
+def test_in_a_graph(torch, ctx, lengths):
+    """A captured call, replayed on other inputs and other lengths."""
+    T, h, d, S = sum(lengths), 2, 128, len(lengths)
+    x, other = _inputs(torch, T, h, d, 53), _inputs(torch, T, h, d, 54)
+    state = _state(torch, S, h, d)
+    want, want_new = _prefill(torch, ctx, other, lengths[::-1], state)
+    flat = [t.reshape(T, h * d).contiguous() for t in x[:4]] + [x[4]]
+    off = torch.tensor(np.cumsum([0, *lengths]), dtype=torch.int32).cuda()
+    out, new = torch.empty(T, h * d, device="cuda"), torch.empty_like(state)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ctx.use_stream(side)
+        try:
+            ctx.kda_prefill(*flat, off, out, state=state, state_out=new)
+            side.synchronize()
+            with torch.cuda.graph(graph, stream=side):
+                ctx.kda_prefill(*flat, off, out, state=state, state_out=new)
+        finally:
+            ctx.use_stream()
+    for t, o in zip(flat, other):
+        t.copy_(o.reshape(t.shape))
+    off.copy_(torch.tensor(np.cumsum([0, *lengths[::-1]]), dtype=torch.int32))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(T, h, d), want) and torch.equal(new, want_new)

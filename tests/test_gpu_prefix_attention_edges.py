@@ -10,7 +10,7 @@ import math
 import pytest
 
 from gpu_util import torch_cuda
-from test_gpu_prefix_attention import _case, _chain, _check
+from test_gpu_prefix_attention import _case, _chain, _check, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -182,3 +182,38 @@ def test_own_rows_past_32_bits(torch, ctx, kind, heads, rows):
     want = (torch.arange(1, heads + 1, dtype=torch.float64, device="cuda")[:, None].expand(heads, 128) + 5.0 * far) / total
     assert bool(((out[2, 0].double() - want).abs() <= 2.0 ** -7 * want).all())
     assert not out[:2].any()
+
+
+@pytest.mark.parametrize("S,lens", [(3, [1500, 20, 900]), (1, [40])])
+def test_in_a_graph(torch, ctx, S, lens):
+    """All launch forms of a call, replayed on other inputs and lengths."""
+    c = _case(torch, S, 2, 4, 2, 128, 64, 128, 700, lens, "bfloat16", 990 + S, spare=600)
+    other = _case(torch, S, 2, 4, 2, 128, 64, 128, 700, lens[::-1], "bfloat16", 991 + S, spare=600)
+    want, want_lse = _run(torch, ctx, other, _chain(2))
+    device = torch.tensor(c["lens"], dtype=torch.int32).cuda()
+    out, lse = torch.empty_like(want), torch.empty_like(want_lse)
+
+    def call():
+        ctx.prefix_attention(c["q"], c["prefix_k"], c["prefix_v"], c["suffix_k"], c["suffix_v"], device, _chain(2), out,
+                             prefix_extra=c["prefix_extra"], suffix_extra=c["suffix_extra"], lse=lse)
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ctx.use_stream(side)
+        try:
+            call()
+            side.synchronize()
+            with torch.cuda.graph(graph, stream=side):
+                call()
+        finally:
+            ctx.use_stream()
+    for n in ("q", "prefix_k", "prefix_v", "prefix_extra", "suffix_k", "suffix_v", "suffix_extra"):
+        c[n].copy_(other[n])
+    device.copy_(torch.tensor(other["lens"], dtype=torch.int32))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
