@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kSeqThreads) kda_recurrent_kernel(const SeqArg
 // tokens, e K and U by value rows; small products summed apart, since a
 // tensor core truncates each sum). T, V, P and U, whose elements may be of any
 // size beside each other, are three bf16 terms (24 bits at any size) in their
-// short products.
+// short products (U two in P U for bf16 outputs).
 //
 // Tokens of unlike size. What one token may lose to another's size is taken
 // out beforehand, by powers of two and thus exactly: token j's key times
